@@ -98,6 +98,9 @@ int moe_expert_layout(int32_t hidden, int32_t inter, int32_t group, moe_expert_l
 int moe_engine_create(const moe_dims_t* dims, int device, moe_engine_t** out);
 void moe_engine_destroy(moe_engine_t* e);
 int moe_engine_sync(moe_engine_t* e);
+/* No counterpart in the reference.  The engine's stream (a cudaStream_t), for hosts that order work of their own streams
+ * around *_dev calls with events; it does not synchronise with the default stream.  Owned by the engine. */
+int moe_engine_stream(const moe_engine_t* e, void** cuda_stream);
 int moe_engine_dims(const moe_engine_t* e, moe_dims_t* out);
 
 /* ── resident expert store ───────────────────────────────────────────────────
@@ -306,6 +309,88 @@ void moe_model_snapshot_free(moe_snapshot_t* snap);
 typedef enum { MOE_ST_K_CACHE = 0, MOE_ST_V_CACHE = 1, MOE_ST_CONV = 2, MOE_ST_SSM = 3 } moe_state_tensor_t;
 int moe_model_state_host(moe_engine_t* e, int32_t layer, int32_t which, float* host, int64_t floats, int32_t to_device);
 int moe_model_set_pos(moe_engine_t* e, int64_t pos);
+
+/* ── rotary positions ────────────────────────────────────────────────────────
+ * apply_rotary_emb (src/math_util.rs:136-168) as an operator of its own: half and interleaved layouts, part of the head,
+ * scaled for contexts longer than the trained one.  Pair i of a head's first rotary_dim elements turns by position *
+ * theta^(-2i / rotary_dim).  Angles are formed in 64 bits on the host:
+ * moe_rope_table_host fills f32 [n_positions, rotary_dim]: cosines, then sines, of positions first_position ...  Scalings:
+ *   MOE_ROPE_LINEAR  every frequency divided by factor
+ *   MOE_ROPE_NTK     theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   MOE_ROPE_YARN    frequencies that make fewer than beta_slow turns over original_positions divided by factor, those
+ *                    of more than beta_fast kept, a linear ramp over the pair index between; table times 0.1 ln factor + 1
+ * moe_rope_dev rotates num_heads heads of n_tokens rows (f32 or bf16; element strides; any alignment of the type) by the
+ * table's row positions_dev[token]; elements from rotary_dim on are copied.  In place (out_dev == x_dev) with equal strides.
+ * A position outside the table leaves the rotated part of that row unwritten and is MOE_ERR_INVALID at the next
+ * moe_engine_sync. */
+typedef enum { MOE_ROPE_PLAIN = 0, MOE_ROPE_LINEAR = 1, MOE_ROPE_NTK = 2, MOE_ROPE_YARN = 3 } moe_rope_scaling_t;
+typedef struct {
+    double theta, factor, beta_fast, beta_slow;
+    int64_t original_positions;
+    int32_t rotary_dim, scaling;
+} moe_rope_params_t;
+typedef struct {
+    const float* cos_sin;  /* device, f32 [n_positions, rotary_dim] as moe_rope_table_host lays it out */
+    int64_t n_positions;
+    int32_t rotary_dim, interleaved;
+} moe_rope_t;
+int moe_rope_table_host(const moe_rope_params_t* p, int64_t first_position, int64_t n_positions, float* cos_sin_host);
+int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int64_t x_token_stride, int64_t x_head_stride,
+                 void* out_dev, int64_t out_token_stride, int64_t out_head_stride, int32_t dtype, int64_t n_tokens,
+                 int32_t num_heads, int32_t head_dim, const int32_t* positions_dev);
+
+/* ── paged KV cache in 4 bits, many sequences ────────────────────────────────
+ * No counterpart in the reference, whose caches are f32, contiguous and hold one sequence (src/cache.rs:32-94): what
+ * serving several sequences or contexts beyond max_seq needs next to the 4-bit weights.  Keys and values are held by the
+ * codec of moe_pack_int4_* (64 elements to a bf16 scale and bias; 18 bytes per 16 elements of K and V together, against
+ * 128 in f32).  The caller owns the pages (moe_kv4_page_bytes each, one allocation per layer, 16-byte aligned) and hands
+ * them to sequences through a page table; nothing is kept between calls.
+ *
+ * A call works on n_seqs sequences: rows q_start[b] .. q_start[b + 1] - 1 of its activations are the LAST positions of
+ * sequence b, which holds seq_lens[b] positions including them; position p lies in page page_table[b, p / page_size].
+ * q_start (increasing), seq_lens and page_table are device memory, read on the device; the fields below them bound what
+ * they hold.  Table entries beyond a sequence's length are not read.  Rows beyond q_start[n_seqs] and rows of a sequence
+ * that has more rows than positions (an idle slot: one row, length 0) carry no position: append skips them, gather and
+ * attention write zeros for the latter and leave the former as they are.  Entries that break the bounds, or lead outside
+ * the cache, touch no memory; they are MOE_ERR_INVALID at the next moe_engine_sync.
+ *
+ * moe_kv4_append_dev     stores the rows' keys and values [n_tokens, num_kv_heads, head_dim] (f32 or bf16, element strides),
+ *                        keys rotated on the way when rope is given: by the position, or by rope_positions_dev[row].  Each
+ *                        position of the cache is written at most once per call (sequences share no pages being written).
+ *                        Values are finite; a group of 64 that holds an infinity or NaN is stored as NaN.
+ * moe_kv4_gather_dev     the rows' stored keys and values as f32 or bf16 [n_tokens, num_kv_heads, head_dim], contiguous;
+ *                        with q_start the running sum of seq_lens it reads whole sequences back.
+ * moe_kv4_attention_dev  softmax attention of the rows' queries [n_tokens, num_heads, head_dim], already rotated, over the
+ *                        positions up to their own (window > 0: the last `window` of them); query head h reads KV head
+ *                        h / (num_heads / num_kv_heads); scale multiplies the scores.  With gate the result is multiplied by
+ *                        sigmoid(gate) (the output gate of the full-attention layers, src/engine/qwen35_moe/cpu.rs:218-347).
+ *                        out is [n_tokens, num_heads, head_dim] of the queries' type, contiguous; it must not overlap them.
+ *                        bf16 rows: products of f16 operands exact to 11 bits, sums and softmax in f32; f32 rows: operands
+ *                        split in two, f32 results to about 2^-21.
+ * head_dim is 64, 128 or 256; page_size a multiple of 16. */
+typedef struct {
+    void* pages;           /* device, [num_pages, moe_kv4_page_bytes] */
+    int64_t num_pages;
+    int32_t page_size, num_kv_heads, head_dim;
+} moe_kv4_cache_t;
+typedef struct {
+    const int32_t* q_start;     /* device, [n_seqs + 1] */
+    const int32_t* seq_lens;    /* device, [n_seqs] */
+    const int32_t* page_table;  /* device, [n_seqs, max_pages] */
+    int32_t n_seqs, n_tokens, max_pages;
+    int32_t max_seq_len, max_q_len; /* no sequence holds more positions / has more rows */
+} moe_kv4_batch_t;
+int moe_kv4_page_bytes(int32_t page_size, int32_t num_kv_heads, int32_t head_dim, int64_t* bytes);
+int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, const void* k_dev,
+                       int64_t k_token_stride, int64_t k_head_stride, const void* v_dev, int64_t v_token_stride,
+                       int64_t v_head_stride, int32_t dtype, const moe_rope_t* rope /* nullable */,
+                       const int32_t* rope_positions_dev /* nullable */);
+int moe_kv4_gather_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, void* k_out_dev,
+                       void* v_out_dev, int32_t dtype);
+int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, const void* q_dev,
+                          int64_t q_token_stride, int64_t q_head_stride, const void* gate_dev /* nullable */,
+                          int64_t gate_token_stride, int64_t gate_head_stride, void* out_dev, int32_t dtype, int32_t num_heads,
+                          float scale, int32_t window);
 
 /* ── telemetry ───────────────────────────────────────────────────────────────
  * set_record_telemetry / Engine::telemetry (src/engine.rs:13-23, 80-84); keys

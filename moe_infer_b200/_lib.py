@@ -51,6 +51,31 @@ class ModelAttnDims(C.Structure):
 ST_K_CACHE, ST_V_CACHE, ST_CONV, ST_SSM = range(4)  # moe_state_tensor_t
 
 
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = range(4)  # moe_rope_scaling_t
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("theta", C.c_double), ("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("original_positions", C.c_int64), ("rotary_dim", C.c_int32), ("scaling", C.c_int32)]
+
+
+class RopeTable(C.Structure):
+    """moe_rope_t: device table [n_positions, rotary_dim] of cosines, then sines."""
+    _fields_ = [("cos_sin", C.c_void_p), ("n_positions", C.c_int64), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class Kv4Cache(C.Structure):
+    """moe_kv4_cache_t: the pages of one layer's 4-bit KV cache (device memory of the caller's)."""
+    _fields_ = [("pages", C.c_void_p), ("num_pages", C.c_int64), ("page_size", C.c_int32), ("num_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32)]
+
+
+class Kv4Batch(C.Structure):
+    """moe_kv4_batch_t: which rows are the last positions of which sequences (device int32 arrays, host bounds)."""
+    _fields_ = [("q_start", C.c_void_p), ("seq_lens", C.c_void_p), ("page_table", C.c_void_p), ("n_seqs", C.c_int32),
+                ("n_tokens", C.c_int32), ("max_pages", C.c_int32), ("max_seq_len", C.c_int32), ("max_q_len", C.c_int32)]
+
+
 class LayerPtrs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("experts", "post_norm", "router_bf16", "router_w", "router_s", "router_b",
                                           "shared", "sgate_w", "sgate_s", "sgate_b")]
@@ -111,6 +136,15 @@ SIGNATURES = {
     "moe_mtp_reset": (_i, [_vp]),
     "moe_mtp_rollback": (_i, [_vp, _i64]),
     "moe_mtp_pos": (_i, [_vp, C.POINTER(_i64)]),
+    "moe_engine_stream": (_i, [_vp, _pp]),
+    "moe_rope_table_host": (_i, [C.POINTER(RopeParams), _i64, _i64, _vp]),
+    "moe_rope_dev": (_i, [_vp, C.POINTER(RopeTable), _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _vp]),
+    "moe_kv4_page_bytes": (_i, [_i32, _i32, _i32, C.POINTER(_i64)]),
+    "moe_kv4_append_dev": (_i, [_vp, C.POINTER(Kv4Cache), C.POINTER(Kv4Batch), _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+                                C.POINTER(RopeTable), _vp]),
+    "moe_kv4_gather_dev": (_i, [_vp, C.POINTER(Kv4Cache), C.POINTER(Kv4Batch), _vp, _vp, _i32]),
+    "moe_kv4_attention_dev": (_i, [_vp, C.POINTER(Kv4Cache), C.POINTER(Kv4Batch), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32,
+                                   _i32, C.c_float, _i32]),
     "moe_set_record_telemetry": (None, [_i]),
     "moe_get_record_telemetry": (_i, []),
     "moe_telemetry_get": (_i, [_vp, C.POINTER(C.c_char_p), C.POINTER(C.c_double), C.POINTER(_i)]),

@@ -35,6 +35,33 @@ int cuda_fail(cudaError_t err, const char* what, const char* file, int line);
         }                                   \
     } while (0)
 
+// Makes an engine's device current for a call and puts the caller's back.
+struct DeviceScope {
+    int prev = -1;
+    bool changed = false;
+    cudaError_t status;
+    explicit DeviceScope(int device) {
+        status = cudaGetDevice(&prev);
+        if (status == cudaSuccess && prev != device) {
+            status = cudaSetDevice(device);
+            changed = status == cudaSuccess;
+        }
+    }
+    ~DeviceScope() {
+        if (changed) cudaSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// Whether rows of `dim` elements at a * sa + b * sb (a < na, b < nb) are disjoint: one index steps over the other's extent.
+inline bool rows_disjoint(int64_t na, int64_t sa, int64_t nb, int64_t sb, int64_t dim) {
+    if (sa < 0 || sb < 0) return false;
+    const bool a_outer = (nb <= 1 || sb >= dim) && (na <= 1 || sa >= (nb - 1) * sb + dim);
+    const bool b_outer = (na <= 1 || sa >= dim) && (nb <= 1 || sb >= (na - 1) * sa + dim);
+    return a_outer || b_outer;
+}
+
 // One 4-bit tensor on the device: u32 words, bf16 scales, bf16 biases.
 struct Q4Dev {
     const uint32_t* w = nullptr;
@@ -191,6 +218,13 @@ struct ModelAttnState {
     bool lin_split = true;                   // DeltaNet core as 256-thread CTAs per block of state rows (gated norm in the out projection)
 };
 
+// Work area of the attention over the paged 4-bit cache (kv4_attn.cu): partial results of work units split over CTAs.
+struct Kv4State {
+    float* work = nullptr;
+    size_t work_bytes = 0;
+    int occupancy[64] = {};                  // resident CTAs per SM of each kernel variant (0: not asked yet)
+};
+
 }  // namespace moe
 
 struct moe_engine {
@@ -243,6 +277,7 @@ struct moe_engine {
     moe::HeadState head;
     moe::MtpAttnState mtp;
     moe::ModelAttnState attn;
+    moe::Kv4State kv4;
 };
 
 namespace moe {
@@ -313,6 +348,8 @@ size_t attn_state_bytes(const moe_engine* e);
 int attn_state_io(moe_engine* e, int layer, int which, float* host, int64_t floats, bool to_device);
 int attn_state_copy(moe_engine* e, uint8_t* buf, bool save);
 void attn_destroy(moe_engine* e);
+void kv4_destroy(moe_engine* e);
+int check_rope(const moe_rope_t* r, int32_t head_dim);
 int head_reserve(moe_engine* e, int32_t n);
 void head_destroy(moe_engine* e);
 int refresh_layer_table(moe_engine* e);

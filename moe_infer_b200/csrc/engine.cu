@@ -184,6 +184,18 @@ static int poll_device_error(moe_engine* e) {
                       e->dims.num_experts);
             return MOE_ERR_INVALID;
         }
+        if (flag == 12u) {
+            set_error("an entry of the page table is outside the cache; the result of the last call is invalid");
+            return MOE_ERR_INVALID;
+        }
+        if (flag == 13u) {
+            set_error("a position is outside the rotary table; the result of the last call is invalid");
+            return MOE_ERR_INVALID;
+        }
+        if (flag == 14u) {
+            set_error("q_start or seq_lens disagree with n_tokens, max_q_len or max_seq_len; the result of the last call is invalid");
+            return MOE_ERR_INVALID;
+        }
         set_error("a bounded device-side wait gave up (code %u); the result of the last call is invalid", flag);
         return MOE_ERR_DEVICE_WAIT;
     }
@@ -307,6 +319,7 @@ void moe_engine_destroy(moe_engine_t* e) {
     head_destroy(e);
     mtp_destroy(e);
     attn_destroy(e);
+    kv4_destroy(e);
     if (e->layers_dev) cudaFree(e->layers_dev);
     if (e->io_dev) cudaFree(e->io_dev);
     if (e->ev0) cudaEventDestroy(e->ev0);
@@ -320,6 +333,12 @@ int moe_engine_sync(moe_engine_t* e) {
     MOE_REQUIRE(e, "null engine");
     MOE_CUDA(cudaStreamSynchronize(e->stream));
     return poll_device_error(e);
+}
+
+int moe_engine_stream(const moe_engine_t* e, void** cuda_stream) {
+    MOE_REQUIRE(e && cuda_stream, "null argument");
+    *cuda_stream = e->stream;
+    return MOE_OK;
 }
 
 int moe_engine_dims(const moe_engine_t* e, moe_dims_t* out) {

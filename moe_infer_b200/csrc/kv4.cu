@@ -1,0 +1,366 @@
+// Writing and reading back the paged 4-bit KV cache (page format: kv4.cuh).
+//
+// Append: key (rotated on the way) and value rows -> nibbles and (scale, bias) pairs, bit for bit the codec of pack.cu:
+//   scale = (max - min) / 15, nibble = trunc((x - min) * (1 / scale) + 0.5), scale and bias = min stored in bf16.
+// Memory bound (f32, head 256: 2 KB read, 288 B written per position and head).  A sub-warp of D / 8 lanes takes one quad
+// (four positions that share words of V) of one head's keys or values; a lane holds eight elements of the four positions,
+// so a group's minimum and maximum are three shuffles, the rotation partner is a second (cached) load or sits in the same
+// lane, a lane's eight nibbles are one word of K, and the four positions' bytes of V meet in the lane that stores them.
+#include "kv4.cuh"
+
+namespace moe {
+
+struct Kv4AppendArgs {
+    Kv4View cache;
+    Kv4Seqs seqs;
+    const void *k, *v;
+    int64_t kt, kh, vt, vh;
+    const float* table;        // null: no rotation
+    int64_t n_positions;
+    int rotary, interleaved, quads;
+    const int32_t* rope_positions;
+    int vec_k, vec_v, vec_partner;
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Quantises the eight elements a lane holds of its group of 64 (eight consecutive lanes): nibbles as one word, element i in
+// bits 4 i; the group's pair, equal in the eight lanes.
+__device__ __forceinline__ uint32_t kv4_quant8(const float (&x)[8], uint32_t& pair) {
+    float mn = x[0], mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        mn = min_nan(mn, x[i]);
+        mx = max_nan(mx, x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (mx == mn) mx = __fadd_rn(mn, 1.0f);
+    const float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
+    const float inv = __fdiv_rn(1.0f, scale);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = __fadd_rn(__fmul_rn(__fsub_rn(x[i], mn), inv), 0.5f);
+        word |= min(__float2uint_rz(t), 15u) << (4 * i);
+    }
+    pair = (uint32_t)f32_to_bf16_ref(scale) | (uint32_t)f32_to_bf16_ref(mn) << 16;
+    // not finite, or too large for its pair to be: both halves NaN (the attention kernel looks at the scale alone)
+    const bool ok = fabsf(mn) < INFINITY && fabsf(scale) < INFINITY && (pair & 0x7F80u) != 0x7F80u && (pair & 0x7F800000u) != 0x7F800000u;
+    if (!ok) pair = 0x7FC07FC0u;
+    return ok ? word : 0u;
+}
+
+// Byte offset inside a block's K nibbles of the word that holds elements 8 l .. 8 l + 7 of position t.
+template <int D>
+__device__ __forceinline__ int kv4_k_offset(int l, int t) {
+    constexpr int U = D >= 128 ? 2 : 1;
+    const int g = l >> 3, c = (l >> 1) & 3, j = l & 1;
+    return (g / U) * (512 * U) + ((t & 1) * 8 + (t >> 1)) * (32 * U) + c * (8 * U) + (g % U) * 8 + j * 4;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsigned int* err) {
+    constexpr int LPT = D / 8, SUB = 32 / LPT;
+    const int lane = threadIdx.x & 31, sub = lane / LPT, l = lane % LPT;
+    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * SUB + sub;
+    const int per_quad = 2 * a.cache.kv_heads;
+    const int64_t bq = item / per_quad;
+    const int r = (int)(item - bq * per_quad);
+    const bool is_v = r >= a.cache.kv_heads;
+    const int h = is_v ? r - a.cache.kv_heads : r;
+    const int64_t b64 = bq / a.quads;
+    Kv4Seq s{0, 0, 0};
+    if (b64 < a.seqs.n_seqs) s = kv4_seq(a.seqs, (int)b64, err);
+    const int b = (int)b64;
+    const int first = max(s.len - s.q_len, 0);                       // first position this call writes
+    const int q0 = (first & ~3) + 4 * (int)(bq - b64 * a.quads);     // this quad's first position
+    const int row_of = s.row0 + s.q_len - s.len;                     // row = row_of + position
+    uint8_t* blk = nullptr;
+    if (q0 < s.len && s.len > first) blk = kv4_block(a.cache, a.seqs, b, h, q0, kv4_block_bytes(D), err);
+    const int lo = blk ? max(first - q0, 0) : 4, hi = blk ? min(s.len - q0, 4) : 0;
+
+    float x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+        if (i < lo || i >= hi) continue;
+        const int64_t row = row_of + (q0 + i);
+        const T* src = is_v ? (const T*)a.v + row * a.vt + (int64_t)h * a.vh : (const T*)a.k + row * a.kt + (int64_t)h * a.kh;
+        ld_act8(src + 8 * l, is_v ? a.vec_v : a.vec_k, x[i]);
+        if (is_v || !a.table || 8 * l >= a.rotary) continue;
+        const int64_t pos = a.rope_positions ? a.rope_positions[row] : q0 + i;
+        if (pos < 0 || pos >= a.n_positions) {
+            atomicExch(err, kErrRopePos);
+            continue;
+        }
+        const float* cs = a.table + pos * a.rotary;
+        const int half = a.rotary >> 1;
+        if (a.interleaved) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                const int p = (8 * l + k) >> 1;
+                if (8 * l + k >= a.rotary) break;
+                const float c = cs[p], sn = cs[half + p], u = x[i][k], w = x[i][k + 1];
+                x[i][k] = __fsub_rn(__fmul_rn(u, c), __fmul_rn(w, sn));
+                x[i][k + 1] = __fadd_rn(__fmul_rn(u, sn), __fmul_rn(w, c));
+            }
+        } else if (a.vec_partner) {  // half a multiple of 8: a lane's elements have one sign and their partners are contiguous
+            const bool second = 8 * l >= half;
+            float o[8], c[8], sn[8];
+            ld_act8(src + (second ? 8 * l - half : 8 * l + half), true, o);
+            const int p = second ? 8 * l - half : 8 * l;
+            ld_act8(cs + p, true, c);
+            ld_act8(cs + half + p, true, sn);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                x[i][k] = second ? __fadd_rn(__fmul_rn(o[k], sn[k]), __fmul_rn(x[i][k], c[k]))
+                                 : __fsub_rn(__fmul_rn(x[i][k], c[k]), __fmul_rn(o[k], sn[k]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int d = 8 * l + k;
+                if (d >= a.rotary) break;
+                const bool second = d >= half;
+                const int p = second ? d - half : d;
+                const float o = ld_act(src + (second ? d - half : d + half)), c = cs[p], sn = cs[half + p];
+                x[i][k] = second ? __fadd_rn(__fmul_rn(o, sn), __fmul_rn(x[i][k], c)) : __fsub_rn(__fmul_rn(x[i][k], c), __fmul_rn(o, sn));
+            }
+        }
+    }
+    uint32_t word[4], pair[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) word[i] = kv4_quant8(x[i], pair[i]);
+    if (hi <= lo) return;
+
+    const int t0 = q0 % kKv4Block;  // 0, 4, 8 or 12
+    uint8_t* nib = blk + (is_v ? 9 * D : 0);
+    if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= lo && i < hi) *reinterpret_cast<uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i)) = word[i];
+    } else {
+        // bytes of the four positions, elements (2x, 2x + 1): word x of the lane's 16
+        uint8_t* dst = nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16;
+        uint32_t w[4];
+#pragma unroll
+        for (int x4 = 0; x4 < 4; ++x4) {
+            w[x4] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[x4] |= (word[i] >> (8 * x4) & 0xFFu) << (8 * i);
+        }
+        if (lo == 0 && hi == 4) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int x4 = 0; x4 < 4; ++x4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= lo && i < hi) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
+        }
+    }
+    if ((l & 7) == 0) {
+        uint32_t* pd = reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0;
+        if (lo == 0 && hi == 4) {
+            *reinterpret_cast<uint4*>(pd) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i >= lo && i < hi) pd[i] = pair[i];
+        }
+    }
+}
+
+// The way back: same mapping, values = nibble * scale + bias (the product is exact, so one rounding).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4View cache, Kv4Seqs seqs, int quads, T* k_out, T* v_out, int vec, unsigned int* err) {
+    constexpr int LPT = D / 8, SUB = 32 / LPT;
+    const int lane = threadIdx.x & 31, sub = lane / LPT, l = lane % LPT;
+    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * SUB + sub;
+    const int per_quad = 2 * cache.kv_heads;
+    const int64_t bq = item / per_quad;
+    const int r = (int)(item - bq * per_quad);
+    const bool is_v = r >= cache.kv_heads;
+    const int h = is_v ? r - cache.kv_heads : r;
+    const int64_t b64 = bq / quads;
+    if (b64 >= seqs.n_seqs) return;
+    const int b = (int)b64;
+    const Kv4Seq s = kv4_seq(seqs, b, err);
+    // positions of the rows, those without one (negative) among them: quads are aligned to the position, also below zero
+    const int first = s.len - s.q_len;
+    const int q0 = (first & ~3) + 4 * (int)(bq - b64 * quads);
+    if (q0 >= s.len) return;
+    T* out = is_v ? v_out : k_out;
+    const uint8_t* blk = q0 >= 0 ? kv4_block(cache, seqs, b, h, q0, kv4_block_bytes(D), err) : nullptr;
+    uint32_t word[4] = {}, pair[4] = {};
+    if (blk) {
+        const int t0 = q0 % kKv4Block;
+        const uint8_t* nib = blk + (is_v ? 9 * D : 0);
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word[i] = *reinterpret_cast<const uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i));
+        } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x4 = 0; x4 < 4; ++x4) word[i] |= (w[x4] >> (8 * i) & 0xFFu) << (8 * x4);
+        }
+        const uint4 p = *reinterpret_cast<const uint4*>(nib + 8 * D + ((l >> 3) * 16 + t0) * 4);
+        pair[0] = p.x; pair[1] = p.y; pair[2] = p.z; pair[3] = p.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pos = q0 + i;
+        if (pos < first || pos >= s.len) continue;
+        const float scale = __uint_as_float(pair[i] << 16), bias = __uint_as_float(pair[i] & 0xFFFF0000u);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf((float)(word[i] >> (4 * k) & 15u), scale, bias);
+        const int64_t row = s.row0 + (pos - first);
+        st_act8(out + (row * cache.kv_heads + h) * D + 8 * l, vec, v);
+    }
+}
+
+int check_kv4(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b) {
+    MOE_REQUIRE(c && b, "kv4: null argument");
+    MOE_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "kv4: head_dim (%d) must be 64, 128 or 256", c->head_dim);
+    MOE_REQUIRE(c->page_size > 0 && c->page_size % kKv4Block == 0 && c->page_size <= 65536, "kv4: page_size (%d) must be a positive multiple of 16 up to 65536", c->page_size);
+    MOE_REQUIRE(c->num_kv_heads > 0 && c->num_kv_heads <= 65536, "kv4: num_kv_heads (%d) must be positive", c->num_kv_heads);
+    MOE_REQUIRE(c->num_pages >= 0 && c->num_pages <= 0x7FFFFFFF, "kv4: num_pages out of range");
+    MOE_REQUIRE(c->pages || c->num_pages == 0, "kv4: null pages");
+    MOE_REQUIRE(((uintptr_t)c->pages & 15) == 0, "kv4: pages must be 16-byte aligned");
+    MOE_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0 && b->max_pages >= 0 && b->max_seq_len >= 0 && b->max_q_len >= 0, "kv4: negative size in the batch");
+    MOE_REQUIRE(b->max_seq_len <= 0x7FFF0000, "kv4: max_seq_len out of range");
+    MOE_REQUIRE(b->n_seqs == 0 || (b->q_start && b->seq_lens), "kv4: null q_start or seq_lens");
+    MOE_REQUIRE(b->n_seqs == 0 || b->max_pages == 0 || b->page_table, "kv4: null page_table");
+    return MOE_OK;
+}
+Kv4View kv4_view(const moe_kv4_cache_t* c) { return Kv4View{(uint8_t*)c->pages, c->num_pages, c->page_size, c->num_kv_heads}; }
+Kv4Seqs kv4_seqs(const moe_kv4_batch_t* b) {
+    return Kv4Seqs{b->q_start, b->seq_lens, b->page_table, b->n_seqs, b->n_tokens, b->max_pages, b->max_seq_len, b->max_q_len};
+}
+
+// blocks of four warps that cover every (sequence, quad, head, key or value)
+static int64_t quad_blocks(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b, int quads) {
+    const int64_t per_block = 4 * (256 / c->head_dim);
+    return ((int64_t)b->n_seqs * quads * 2 * c->num_kv_heads + per_block - 1) / per_block;
+}
+static int quads_of(const moe_kv4_batch_t* b) {  // q rows touch at most this many aligned quads of positions
+    const int q = b->max_q_len < b->n_tokens ? b->max_q_len : b->n_tokens;
+    return (int)(((int64_t)q + 2) / 4 + 1);
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_kv4_page_bytes(int32_t page_size, int32_t num_kv_heads, int32_t head_dim, int64_t* bytes) {
+    MOE_REQUIRE(bytes, "kv4: null argument");
+    const moe_kv4_cache_t c{nullptr, 0, page_size, num_kv_heads, head_dim};
+    const moe_kv4_batch_t b{};
+    int rc = check_kv4(&c, &b);
+    if (rc) return rc;
+    *bytes = (int64_t)(page_size / kKv4Block) * num_kv_heads * kv4_block_bytes(head_dim);
+    return MOE_OK;
+}
+
+int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, const void* k_dev,
+                       int64_t k_token_stride, int64_t k_head_stride, const void* v_dev, int64_t v_token_stride,
+                       int64_t v_head_stride, int32_t dtype, const moe_rope_t* rope, const int32_t* rope_positions_dev) {
+    MOE_REQUIRE(e, "kv4_append: null engine");
+    int rc = check_kv4(cache, batch);
+    if (rc) return rc;
+    MOE_REQUIRE(dtype == MOE_DT_F32 || dtype == MOE_DT_BF16, "kv4_append: keys and values are f32 or bf16 (got dtype %d)", dtype);
+    if (rope && (rc = check_rope(rope, cache->head_dim))) return rc;
+    MOE_REQUIRE(rope || !rope_positions_dev, "kv4_append: rope positions without a rope table");
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_q_len == 0) return MOE_OK;
+    MOE_REQUIRE(k_dev && v_dev, "kv4_append: null argument");
+    const uintptr_t amask = dtype == MOE_DT_F32 ? 3 : 1;
+    MOE_REQUIRE((((uintptr_t)k_dev | (uintptr_t)v_dev) & amask) == 0, "kv4_append: misaligned pointer");
+    MOE_REQUIRE(k_token_stride >= 0 && k_head_stride >= 0 && v_token_stride >= 0 && v_head_stride >= 0, "kv4_append: negative stride");
+    DeviceScope scope(e->device);
+    MOE_CUDA(scope.status);
+    const int vec = dtype == MOE_DT_F32 ? 4 : 8;
+    Kv4AppendArgs a{};
+    a.cache = kv4_view(cache);
+    a.seqs = kv4_seqs(batch);
+    a.k = k_dev; a.v = v_dev;
+    a.kt = k_token_stride; a.kh = k_head_stride; a.vt = v_token_stride; a.vh = v_head_stride;
+    if (rope) {
+        a.table = rope->cos_sin;
+        a.n_positions = rope->n_positions;
+        a.rotary = rope->rotary_dim;
+        a.interleaved = rope->interleaved;
+    }
+    a.rope_positions = rope_positions_dev;
+    a.quads = quads_of(batch);
+    a.vec_k = ((uintptr_t)k_dev & 15) == 0 && (k_token_stride | k_head_stride) % vec == 0;
+    a.vec_v = ((uintptr_t)v_dev & 15) == 0 && (v_token_stride | v_head_stride) % vec == 0;
+    a.vec_partner = a.vec_k && a.rotary % 16 == 0 && ((uintptr_t)a.table & 15) == 0;
+    const int64_t blocks = quad_blocks(cache, batch, a.quads);
+    MOE_REQUIRE(blocks < 0x7FFFFFFF, "kv4_append: too many rows for one call");
+    unsigned int* err = e->dec_sync + 2;
+    auto run = [&](auto kernel) { kernel<<<(unsigned)blocks, 128, 0, e->stream>>>(a, err); };
+    const bool f32 = dtype == MOE_DT_F32;
+    switch (cache->head_dim) {
+        case 64: f32 ? run(kv4_append_kernel<float, 64>) : run(kv4_append_kernel<__nv_bfloat16, 64>); break;
+        case 128: f32 ? run(kv4_append_kernel<float, 128>) : run(kv4_append_kernel<__nv_bfloat16, 128>); break;
+        default: f32 ? run(kv4_append_kernel<float, 256>) : run(kv4_append_kernel<__nv_bfloat16, 256>); break;
+    }
+    e->launches++;
+    MOE_CUDA(cudaGetLastError());
+    return MOE_OK;
+}
+
+int moe_kv4_gather_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, void* k_out_dev, void* v_out_dev,
+                       int32_t dtype) {
+    MOE_REQUIRE(e, "kv4_gather: null engine");
+    int rc = check_kv4(cache, batch);
+    if (rc) return rc;
+    MOE_REQUIRE(dtype == MOE_DT_F32 || dtype == MOE_DT_BF16, "kv4_gather: outputs are f32 or bf16 (got dtype %d)", dtype);
+    if (batch->n_seqs == 0 || batch->n_tokens == 0 || batch->max_q_len == 0) return MOE_OK;
+    MOE_REQUIRE(k_out_dev && v_out_dev, "kv4_gather: null argument");
+    const uintptr_t amask = dtype == MOE_DT_F32 ? 3 : 1;
+    MOE_REQUIRE((((uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & amask) == 0, "kv4_gather: misaligned pointer");
+    DeviceScope scope(e->device);
+    MOE_CUDA(scope.status);
+    const int quads = quads_of(batch);
+    const int64_t blocks = quad_blocks(cache, batch, quads);
+    MOE_REQUIRE(blocks < 0x7FFFFFFF, "kv4_gather: too many rows for one call");
+    const int vec = (((uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & 15) == 0;
+    unsigned int* err = e->dec_sync + 2;
+    auto run = [&](auto kernel, auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        kernel<<<(unsigned)blocks, 128, 0, e->stream>>>(kv4_view(cache), kv4_seqs(batch), quads, (T*)k_out_dev, (T*)v_out_dev, vec, err);
+    };
+    const bool f32 = dtype == MOE_DT_F32;
+    float* f = nullptr;
+    __nv_bfloat16* h = nullptr;
+    switch (cache->head_dim) {
+        case 64: f32 ? run(kv4_gather_kernel<float, 64>, f) : run(kv4_gather_kernel<__nv_bfloat16, 64>, h); break;
+        case 128: f32 ? run(kv4_gather_kernel<float, 128>, f) : run(kv4_gather_kernel<__nv_bfloat16, 128>, h); break;
+        default: f32 ? run(kv4_gather_kernel<float, 256>, f) : run(kv4_gather_kernel<__nv_bfloat16, 256>, h); break;
+    }
+    e->launches++;
+    MOE_CUDA(cudaGetLastError());
+    return MOE_OK;
+}
+
+}  // extern "C"

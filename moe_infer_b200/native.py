@@ -13,6 +13,7 @@ from typing import Optional, Sequence, Tuple
 import numpy as np
 
 from . import _lib as L
+from ._lib import Kv4Batch, Kv4Cache, RopeTable  # noqa: F401  (arguments of the kv4 / rope methods)
 
 
 @dataclass
@@ -408,6 +409,43 @@ class NativeEngine:
         L.check(self.lib.moe_mtp_pos(self.h, C.byref(p)))
         return p.value
 
+    # ── rotary positions, paged 4-bit KV cache ───────────────────────────
+    def stream(self) -> int:
+        """The engine's CUDA stream (cudaStream_t as an integer)."""
+        p = C.c_void_p()
+        L.check(self.lib.moe_engine_stream(self.h, C.byref(p)))
+        return p.value or 0
+
+    def rope_dev(self, rope: RopeTable, x: int, out: int, positions: int, dtype: int, n_tokens: int, heads: int, head_dim: int,
+                 x_strides: Optional[Tuple[int, int]] = None, out_strides: Optional[Tuple[int, int]] = None) -> None:
+        """Rotates [n_tokens, heads, head_dim]; strides are (token, head) in elements, contiguous by default."""
+        xs = x_strides or (heads * head_dim, head_dim)
+        os_ = out_strides or (heads * head_dim, head_dim)
+        L.check(self.lib.moe_rope_dev(self.h, rope, x, xs[0], xs[1], out, os_[0], os_[1], dtype, n_tokens, heads, head_dim,
+                                      positions))
+
+    def kv4_append_dev(self, cache: Kv4Cache, batch: Kv4Batch, k: int, v: int, dtype: int, *, rope: Optional[RopeTable] = None,
+                       rope_positions: int = 0, k_strides: Optional[Tuple[int, int]] = None,
+                       v_strides: Optional[Tuple[int, int]] = None) -> None:
+        """Stores the batch rows' keys (rotated when rope is given) and values; strides are (token, head) in elements."""
+        dense = (cache.num_kv_heads * cache.head_dim, cache.head_dim)
+        ks, vs = k_strides or dense, v_strides or dense
+        L.check(self.lib.moe_kv4_append_dev(self.h, cache, batch, k, ks[0], ks[1], v, vs[0], vs[1], dtype, rope,
+                                            rope_positions or None))
+
+    def kv4_gather_dev(self, cache: Kv4Cache, batch: Kv4Batch, k_out: int, v_out: int, dtype: int) -> None:
+        """The batch rows' stored keys and values, [n_tokens, num_kv_heads, head_dim] each."""
+        L.check(self.lib.moe_kv4_gather_dev(self.h, cache, batch, k_out, v_out, dtype))
+
+    def kv4_attention_dev(self, cache: Kv4Cache, batch: Kv4Batch, q: int, out: int, dtype: int, heads: int, *, scale: float,
+                          window: int = 0, gate: int = 0, q_strides: Optional[Tuple[int, int]] = None,
+                          gate_strides: Optional[Tuple[int, int]] = None) -> None:
+        """Attention of the batch rows' (rotated) queries [n_tokens, heads, head_dim] over the cache; strides as above."""
+        dense = (heads * cache.head_dim, cache.head_dim)
+        qs, gs = q_strides or dense, gate_strides or dense
+        L.check(self.lib.moe_kv4_attention_dev(self.h, cache, batch, q, qs[0], qs[1], gate or None, gs[0], gs[1], out, dtype,
+                                               heads, scale, window))
+
     def telemetry(self) -> dict:
         n = C.c_int(0)
         L.check(self.lib.moe_telemetry_get(self.h, None, None, C.byref(n)))
@@ -450,6 +488,22 @@ class NativeEngine:
 
     def alloc(self, nbytes: int) -> DevBuf:
         return DevBuf(self, nbytes)
+
+
+def rope_table(rotary_dim: int, n_positions: int, theta: float, *, scaling: int = L.ROPE_PLAIN, factor: float = 1.0,
+               original_positions: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0, first_position: int = 0) -> np.ndarray:
+    """Cosines, then sines, of the rotary angles of every position: float32 [n_positions, rotary_dim]."""
+    p = L.RopeParams(theta, factor, beta_fast, beta_slow, original_positions, rotary_dim, scaling)
+    out = np.empty((n_positions, rotary_dim), np.float32)
+    L.check(L.load().moe_rope_table_host(C.byref(p), first_position, n_positions, L.ptr(out)))
+    return out
+
+
+def kv4_page_bytes(page_size: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of one page of a 4-bit KV cache."""
+    n = C.c_int64()
+    L.check(L.load().moe_kv4_page_bytes(page_size, num_kv_heads, head_dim, C.byref(n)))
+    return n.value
 
 
 def load_layer_weights(eng: NativeEngine, layer: int, *, post_norm_w, router_bf16=None, router_q4=None,
