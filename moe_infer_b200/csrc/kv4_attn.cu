@@ -20,22 +20,9 @@
 // (prompts): one CTA per unit over the positions its rows see, nothing to join.
 #include <math.h>
 
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 
 namespace moe {
-
-struct AttnArgs {
-    Kv4View cache;
-    Kv4Seqs seqs;
-    const void* q;
-    const void* gate;        // null: none
-    void* out;
-    int64_t qt, qh, gt, gh;  // element strides
-    int heads, group;        // query heads; query heads per KV head
-    float scale_log2;        // scale * log2(e)
-    int window;              // 0: none
-    float* part;             // partial results: per slot [rows][D] sums, [rows] maxima, [rows] sums of weights
-};
 
 template <int D_, bool F32_, int MT_, int TB_, bool SPLIT_>
 struct AttnCfg {
@@ -148,33 +135,12 @@ __device__ AttnPlan attn_scan(const AttnArgs& a, int nthreads, long long (&red)[
 }
 
 // ─── small device pieces ────────────────────────────────────────────────────
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// four nibble pairs of a word as f16 pairs of n - 8: word bits {0-3, 16-19}, {4-7, 20-23}, {8-11, 24-27}, {12-15, 28-31}.
-// 0x6400 | n is the f16 number 1024 + n, 0x6400 | n << 4 is 1024 + 16 n; both subtractions are exact.
-__device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
-    const __half2 m1032 = bits_h2(0xE408E408u), sixteenth = bits_h2(0x2C002C00u), m72 = bits_h2(0xD480D480u);
-    const uint32_t w8 = w >> 8;
-    o[0] = h2_bits(__hadd2(bits_h2((w & 0x000F000Fu) | 0x64006400u), m1032));
-    o[1] = h2_bits(__hfma2(bits_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, m72));
-    o[2] = h2_bits(__hadd2(bits_h2((w8 & 0x000F000Fu) | 0x64006400u), m1032));
-    o[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00F000F0u) | 0x64006400u), sixteenth, m72));
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 
 template <class C, typename T>
 __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
@@ -831,7 +797,7 @@ void kv4_destroy(moe_engine* e) {
     e->kv4 = Kv4State{};
 }
 
-static int kv4_reserve(moe_engine* e, size_t bytes) {
+int kv4_reserve(moe_engine* e, size_t bytes) {
     if (bytes <= e->kv4.work_bytes) return MOE_OK;
     MOE_CUDA(cudaStreamSynchronize(e->stream));
     if (e->kv4.work) cudaFree(e->kv4.work);
@@ -890,6 +856,9 @@ static int launch_attn(moe_engine* e, const AttnArgs& a) {
         return (all < per_seq * n ? all : per_seq * n) * a.cache.kv_heads;
     };
     constexpr int TB = 4 / (D / 64);
+    if constexpr (!F32) {
+        if (kv4_prompt_fits<D>(e, a)) return launch_kv4_prompt<D>(e, a);
+    }
     if (q_rows > 2 * R1 && units(4 * R1) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(4 * R1));
     if (q_rows > 2 * R1) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(4 * R1));
     if (q_rows > R1) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(2 * R1));

@@ -1,0 +1,51 @@
+// What the kernels of the attention over the 4-bit cache share (kv4_attn.cu, kv4_prompt.cu).
+#pragma once
+#include "kv4.cuh"
+
+namespace moe {
+
+struct AttnArgs {
+    Kv4View cache;
+    Kv4Seqs seqs;
+    const void* q;
+    const void* gate;        // null: none
+    void* out;
+    int64_t qt, qh, gt, gh;  // element strides
+    int heads, group;        // query heads; query heads per KV head
+    float scale_log2;        // scale * log2(e)
+    int window;              // 0: none
+    float* part;             // work area of the call
+};
+
+int kv4_reserve(moe_engine* e, size_t bytes);
+// Prompts of bf16 rows on the fifth-generation tensor cores; whether the call suits that path
+template <int D>
+bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a);
+template <int D>
+int launch_kv4_prompt(moe_engine* e, AttnArgs a);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// four nibble pairs of a word as f16 pairs of n - 8: word bits {0-3, 16-19}, {4-7, 20-23}, {8-11, 24-27}, {12-15, 28-31}.
+// 0x6400 | n is the f16 number 1024 + n, 0x6400 | n << 4 is 1024 + 16 n; both subtractions are exact.
+__device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
+    const __half2 m1032 = bits_h2(0xE408E408u), sixteenth = bits_h2(0x2C002C00u), m72 = bits_h2(0xD480D480u);
+    const uint32_t w8 = w >> 8;
+    o[0] = h2_bits(__hadd2(bits_h2((w & 0x000F000Fu) | 0x64006400u), m1032));
+    o[1] = h2_bits(__hfma2(bits_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, m72));
+    o[2] = h2_bits(__hadd2(bits_h2((w8 & 0x000F000Fu) | 0x64006400u), m1032));
+    o[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00F000F0u) | 0x64006400u), sixteenth, m72));
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+#endif
+
+}  // namespace moe

@@ -1,0 +1,502 @@
+// Attention of many rows (prompts, chunks of prompts) over the 4-bit cache, bf16 rows, on tcgen05.
+//
+// With hundreds of rows per position the products dominate (4 D flops per row, head and position) and every position is
+// read by many row tiles, so the positions the call sees are first expanded, once, into f16 tiles of 128 positions that
+// lie in memory exactly as the MMAs want them in shared memory (K-major, 128-byte swizzle): a tile then arrives by plain
+// bulk copies.  f16 values of a tile are scaled by a power of two of its own, so any range of values keeps 11 bits.
+//
+// Attention kernel: a CTA owns 128 rows (of the query heads that share a KV head) and walks its positions.  One thread
+// copies, one issues MMAs, four warps hold a row per thread:
+//   S = Q K^T (128 x 128, two buffers in tensor memory)  ->  w = exp2(S f - m)  ->  f16 P in shared memory  ->  O += P V
+// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 (the weights of a row
+// share one reference, so the result does not depend on when).  QK of the next tile runs under the softmax of this one.
+#include <math.h>
+
+#include "kv4_attn.cuh"
+#include "umma.cuh"
+
+namespace moe {
+
+constexpr int kPtTile = 128;                 // positions of a tile, rows of a CTA
+constexpr int kPtMeta = 8;                   // ints per tile: exponents of K and V, four words of "value is NaN" bits
+
+template <int D>
+struct PtCfg {
+    static constexpr int G = D / 64;
+    static constexpr int IMG = D * kPtTile * 2;                    // one f16 image of a tile
+    static constexpr int OFF_K = IMG, OFF_V = 2 * IMG, OFF_P = 3 * IMG;
+    static constexpr int P_BYTES = kPtTile * kPtTile * 2;
+    static constexpr int OFF_BAR = OFF_P + P_BYTES;
+    // barriers, and room to align the base to 1 KB; never so little that two CTAs would share an SM (tensor memory holds one)
+    static constexpr int SMEM = OFF_BAR + 256 + 1024 > 118 * 1024 ? OFF_BAR + 256 + 1024 : 118 * 1024;
+    static constexpr int COL_S = D;                                // tensor memory: O, then two score buffers
+    static constexpr int COLS = 512;
+};
+
+// Tiles of a sequence that its rows see: the first one's index and their number.
+__device__ __forceinline__ void pt_range(const AttnArgs& a, const Kv4Seq& s, int& t0, int& n) {
+    const int first = max(s.len - s.q_len, 0);
+    t0 = a.window > 0 ? max(first - a.window + 1, 0) / kPtTile : 0;
+    n = s.q_len > 0 ? (s.len + kPtTile - 1) / kPtTile - t0 : 0;
+}
+
+// One CTA expands K or V of one tile of one head.  image: [(sequence, head, tile)][K, V][IMG bytes]; meta alike, kPtMeta ints.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_per_seq, uint8_t* image, int* meta, unsigned int* err) {
+    using C = PtCfg<D>;
+    constexpr int G = C::G;
+    extern __shared__ __align__(1024) uint8_t ex_sm[];
+    __shared__ uint8_t* blocks[8];
+    __shared__ float red[8];
+    __shared__ unsigned int nan_bits[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool is_v = blockIdx.x & 1;
+    const int ti = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
+    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    int tile0, n;
+    pt_range(a, s, tile0, n);
+    if (ti >= n || ti >= tiles_per_seq) return;
+    const int p0 = (tile0 + ti) * kPtTile;
+    if (tid < 8) blocks[tid] = p0 + tid * 16 < s.len ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
+    if (tid < 4) nan_bits[tid] = 0;
+    __syncthreads();
+    // the largest |value| a pair can stand for
+    float mx = 0.0f;
+    for (int i = tid; i < G * kPtTile; i += 256) {
+        const int t = i % kPtTile, g = i / kPtTile;
+        const uint8_t* blk = blocks[t >> 4];
+        if (!blk || p0 + t >= s.len) continue;
+        const uint32_t pw = *reinterpret_cast<const uint32_t*>(blk + (is_v ? 17 * D : 8 * D) + g * 64 + (t & 15) * 4);
+        const float sc = __uint_as_float(pw << 16), bi = __uint_as_float(pw & 0xFFFF0000u);
+        const float v = fmaxf(fabsf(bi), fabsf(fmaf(15.0f, sc, bi)));
+        if (v < INFINITY && fabsf(sc) < INFINITY) mx = fmaxf(mx, v);
+        else atomicOr(nan_bits + (t >> 5), 1u << (t & 31));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) red[warp] = mx;
+    __syncthreads();
+    mx = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, red[i]);
+    // scaled into [1, 2); an all-zero tile keeps a harmless exponent
+    const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 126);
+    const float down = pow2f(-e);
+    const size_t at = ((size_t)(b * a.cache.kv_heads + h) * tiles_per_seq + ti);
+    if (tid == 0) meta[at * kPtMeta + (is_v ? 1 : 0)] = e;
+    if (is_v && tid < 4) meta[at * kPtMeta + 2 + tid] = (int)nan_bits[tid];
+
+    if (!is_v) {
+        // a word = 8 elements of a position, f16 order 0 4 1 5 2 6 3 7 (the queries' too): one 16-byte chunk of the row
+        for (int i = tid; i < kPtTile * (D / 8); i += 256) {
+            const int c8 = i % (D / 8), t = i / (D / 8), g = c8 >> 3;
+            const uint8_t* blk = blocks[t >> 4];
+            uint32_t o[4] = {0, 0, 0, 0};
+            if (blk && p0 + t < s.len) {
+                constexpr int U = D >= 128 ? 2 : 1;
+                const int tt = t & 15, cc = (c8 >> 1) & 3, j = c8 & 1;
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + (g / U) * (512 * U) + ((tt & 1) * 8 + (tt >> 1)) * (32 * U) + cc * (8 * U) + (g % U) * 8 + j * 4);
+                const uint32_t pw = *reinterpret_cast<const uint32_t*>(blk + 8 * D + g * 64 + tt * 4);
+                const float sc = __uint_as_float(pw << 16);
+                const __half2 hs = __float2half2_rn(sc * down), hb = __float2half2_rn(fmaf(8.0f, sc, __uint_as_float(pw & 0xFFFF0000u)) * down);
+                uint32_t nb[4];
+                nibbles_h2(w, nb);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = h2_bits(__hfma2(bits_h2(nb[k]), hs, hb));
+            }
+            *reinterpret_cast<uint4*>(ex_sm + g * (kPtTile * 128) + umma::sw128_offset(t, c8 & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    } else {
+        // rows are elements, 8 positions to a 16-byte chunk in the order 0 2 1 3 4 6 5 7 (the weights' too)
+        for (int i = tid; i < (kPtTile / 8) * (D / 8); i += 256) {
+            const int ch = i % (kPtTile / 8), n8 = i / (kPtTile / 8), g = n8 >> 3;  // chunk of positions, 8 elements
+            const uint8_t* blk = blocks[ch >> 1];
+            uint32_t o[8][4];
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[d][k] = 0;
+            if (blk) {
+                const int t = (ch & 1) * 8;
+#pragma unroll
+                for (int qd = 0; qd < 2; ++qd) {
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(blk + 9 * D + g * 512 + (n8 & 7) * 64 + ((t >> 2) + qd) * 16);
+                    const uint4 p4 = *reinterpret_cast<const uint4*>(blk + 17 * D + g * 64 + (t + 4 * qd) * 4);
+                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w}, pw[4] = {p4.x, p4.y, p4.z, p4.w};
+                    float sc[4], bi[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float s0 = __uint_as_float(pw[k] << 16), b0 = __uint_as_float(pw[k] & 0xFFFF0000u);
+                        const bool in = p0 + ch * 8 + qd * 4 + k < s.len && fabsf(s0) < INFINITY && fabsf(b0) < INFINITY;  // NaN: marked above
+                        sc[k] = in ? s0 * down : 0.0f;
+                        bi[k] = in ? fmaf(8.0f, s0, b0) * down : 0.0f;
+                    }
+                    const __half2 s02 = __floats2half2_rn(sc[0], sc[2]), s13 = __floats2half2_rn(sc[1], sc[3]);
+                    const __half2 b02 = __floats2half2_rn(bi[0], bi[2]), b13 = __floats2half2_rn(bi[1], bi[3]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t nb[4];
+                        nibbles_h2(w[x], nb);
+                        o[2 * x][2 * qd] = h2_bits(__hfma2(bits_h2(nb[0]), s02, b02));
+                        o[2 * x + 1][2 * qd] = h2_bits(__hfma2(bits_h2(nb[1]), s02, b02));
+                        o[2 * x][2 * qd + 1] = h2_bits(__hfma2(bits_h2(nb[2]), s13, b13));
+                        o[2 * x + 1][2 * qd + 1] = h2_bits(__hfma2(bits_h2(nb[3]), s13, b13));
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                *reinterpret_cast<uint4*>(ex_sm + (ch >> 3) * (D * 128) + umma::sw128_offset(n8 * 8 + d, ch & 7)) = make_uint4(o[d][0], o[d][1], o[d][2], o[d][3]);
+        }
+    }
+    __syncthreads();
+    uint4* dst = reinterpret_cast<uint4*>(image + (at * 2 + (is_v ? 1 : 0)) * C::IMG);
+    for (int i = tid; i < C::IMG / 16; i += 256) dst[i] = reinterpret_cast<const uint4*>(ex_sm)[i];
+}
+
+// Instruction descriptor for kind::f16 with f16 A and B (format 0), f32 D; the other fields as in umma::make_idesc_bf16.
+__device__ __forceinline__ uint32_t make_idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]),
+        "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]),
+        "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_per_seq, const uint8_t* image, const int* meta, unsigned int* err) {
+    using C = PtCfg<D>;
+    extern __shared__ uint8_t pt_raw[];
+    uint8_t* sm = pt_raw + ((1024u - (smem_u32(pt_raw) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+    uint64_t *k_full = bars, *v_full = bars + 1, *k_free = bars + 2, *pv_done = bars + 3, *s_full = bars + 4 /* 2 */, *p_ready = bars + 6, *q_ready = bars + 7;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+    const int tid = threadIdx.x, warp = tid >> 5;
+
+    // which rows: units are counted in row tiles, the last rows of a sequence (which see most) first
+    const int h = blockIdx.x % a.cache.kv_heads;
+    long long at = blockIdx.x / a.cache.kv_heads;
+    int b = 0, rts = 0;
+    Kv4Seq s{0, 0, 0};
+    for (; b < a.seqs.n_seqs; ++b) {
+        s = kv4_seq(a.seqs, b, err);
+        rts = (int)(((int64_t)s.q_len * a.group + kPtTile - 1) / kPtTile);
+        if (at < rts) break;
+        at -= rts;
+    }
+    if (b >= a.seqs.n_seqs) return;
+    const int rt = rts - 1 - (int)at, rows_all = s.q_len * a.group, pos_base = s.len - s.q_len;
+    int seq_t0, seq_n;
+    pt_range(a, s, seq_t0, seq_n);
+    const int j_first = rt * kPtTile / a.group, j_last = min((rt * kPtTile + kPtTile - 1) / a.group, s.q_len - 1);
+    const int p_last = pos_base + j_last;  // may be negative: rows without a position
+    const int t_begin = a.window > 0 ? max(pos_base + j_first - a.window + 1, 0) / kPtTile : 0;
+    const int n_tiles = p_last >= 0 ? min(p_last / kPtTile + 1, seq_t0 + min(seq_n, tiles_per_seq)) - t_begin : 0;
+    const size_t img0 = (size_t)(b * a.cache.kv_heads + h) * tiles_per_seq + (t_begin - seq_t0);
+
+    if (tid == 0) {
+        mbar_init(k_full, 1);
+        mbar_init(v_full, 1);
+        mbar_init(k_free, 1);
+        mbar_init(pv_done, 1);
+        mbar_init(s_full, 1);
+        mbar_init(s_full + 1, 1);
+        mbar_init(p_ready, 128);
+        mbar_init(q_ready, 128);
+        mbar_fence_init();
+    }
+    if (warp == 5) umma::tmem_alloc(tmem_slot, C::COLS);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 4) {
+        // ── copies ──
+        if ((tid & 31) == 0) {
+            auto load = [&](int i, int v) {
+                uint64_t* bar = v ? v_full : k_full;
+                uint8_t* dst = sm + (v ? C::OFF_V : C::OFF_K);
+                const uint8_t* src = image + ((img0 + i) * 2 + v) * C::IMG;
+                mbar_expect_tx(bar, C::IMG);
+#pragma unroll
+                for (int p = 0; p < C::IMG; p += 16384) bulk_g2s(dst + p, src + p, C::IMG < 16384 ? C::IMG : 16384, bar);
+            };
+            if (n_tiles > 0) {
+                load(0, 0);
+                load(0, 1);
+            }
+            if (n_tiles > 1 && (ok = mbar_wait(k_free, 0))) load(1, 0);
+            for (int i = 0; i + 1 < n_tiles && ok; ++i) {
+                if (i + 2 < n_tiles) {
+                    if (!(ok = mbar_wait(k_free, (i + 1) & 1))) break;
+                    load(i + 2, 0);
+                }
+                if (!(ok = mbar_wait(pv_done, i & 1))) break;
+                load(i + 1, 1);
+            }
+            if (!ok) atomicExch(err, 1u);
+        }
+    } else if (warp == 5) {
+        // ── MMAs ──
+        if ((tid & 31) == 0 && n_tiles > 0) {
+            const uint32_t id_qk = make_idesc_f16(128, kPtTile), id_pv = make_idesc_f16(128, D);
+            auto qk = [&](int i) {
+                umma::fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k >> 2) * (kPtTile * 128) + (k & 3) * 32;
+                    umma::mma_bf16(tmem + C::COL_S + (i & 1) * kPtTile, umma::make_desc_sw128_kmajor(smem_u32(sm + off)),
+                                   umma::make_desc_sw128_kmajor(smem_u32(sm + C::OFF_K + off)), id_qk, k > 0);
+                }
+                umma::commit(s_full + (i & 1));
+                umma::commit(k_free);
+            };
+            ok = mbar_wait(q_ready, 0) && mbar_wait(k_full, 0);
+            if (ok) qk(0);
+            for (int i = 0; i < n_tiles && ok; ++i) {
+                if (i + 1 < n_tiles) {
+                    if (!(ok = mbar_wait(k_full, (i + 1) & 1))) break;
+                    qk(i + 1);
+                }
+                if (!(ok = mbar_wait(p_ready, i & 1) && mbar_wait(v_full, i & 1))) break;
+                umma::fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < kPtTile / 16; ++k)
+                    umma::mma_bf16(tmem, umma::make_desc_sw128_kmajor(smem_u32(sm + C::OFF_P + (k >> 2) * (kPtTile * 128) + (k & 3) * 32)),
+                                   umma::make_desc_sw128_kmajor(smem_u32(sm + C::OFF_V + (k >> 2) * (D * 128) + (k & 3) * 32)), id_pv, (i > 0 || k > 0));
+                umma::commit(pv_done);
+            }
+            if (!ok) atomicExch(err, 1u);
+        }
+    } else {
+        // ── a row per thread ──
+        const int row = tid, rr = rt * kPtTile + row;
+        const bool valid = rr < rows_all;
+        const int j = valid ? rr / a.group : 0, hq = h * a.group + (valid ? rr % a.group : 0);
+        const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (int64_t)(s.row0 + j) * a.qt + (int64_t)hq * a.qh;
+        const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 * warp of tensor memory (bits 16-31)
+        float f_row;
+        {
+            const bool vec = (((uintptr_t)a.q & 15) == 0) && ((a.qt | a.qh) & 7) == 0;
+            float mx = 0.0f;
+            for (int c = 0; c < D / 8; ++c) {
+                float v[8];
+                if (valid) ld_act8(qp + 8 * c, vec, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mx = valid ? fmaxf(mx, fabsf(v[k])) : mx;
+            }
+            // scaled by a power of two into [2^14, 2^15); a negative scale turns the queries' sign, a scale of 0 makes them 0
+            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -110), 127);
+            float up = pow2f(min(14 - e, 127));
+            if (a.scale_log2 < 0.0f) up = -up;
+            const float mag = fabsf(a.scale_log2);
+            if (mag == 0.0f) up = 0.0f;
+            f_row = (mag == 0.0f ? 1.0f : mag) * pow2f(max(e - 14, -126));
+            for (int c = 0; c < D / 8; ++c) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+                if (valid) ld_act8(qp + 8 * c, vec, v);
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = h2_bits(__floats2half2_rn(v[k] * up, v[k + 4] * up));
+                *reinterpret_cast<uint4*>(sm + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            umma::fence_smem_to_async();
+            mbar_arrive(q_ready);
+        }
+        const int see_hi = valid ? pos_base + j : 0x7FFFFFFF;
+        const int see_lo = valid && a.window > 0 ? see_hi - a.window + 1 : 0;
+        float m_ref = -INFINITY, l = 0.0f;
+        int e_k = 0, e_v = 0;
+        if (n_tiles > 0) {
+            e_k = meta[img0 * kPtMeta];
+            e_v = meta[img0 * kPtMeta + 1];
+        }
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            const int t0 = (t_begin + i) * kPtTile;
+            const int* mt = meta + (img0 + i) * kPtMeta;
+            const int ek = e_k, ev = e_v;
+            const uint32_t nb[4] = {(uint32_t)mt[2], (uint32_t)mt[3], (uint32_t)mt[4], (uint32_t)mt[5]};
+            if (i + 1 < n_tiles) {
+                e_k = mt[kPtMeta];
+                e_v = mt[kPtMeta + 1];
+            }
+            ok = mbar_wait(s_full + (i & 1), (i >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            umma::fence_after_sync();
+            float v[4][32];
+            const uint32_t sc = lane_base + C::COL_S + (i & 1) * kPtTile;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) umma::ld_32x32(sc + 32 * q, v[q]);
+            if (t0 + kPtTile - 1 > see_hi || t0 < see_lo) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const int t = t0 + 32 * q + k;
+                        if (t > see_hi || t < see_lo) v[q][k] = -INFINITY;
+                    }
+            }
+            float mx[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                mx[q] = v[q][0];
+#pragma unroll
+                for (int k = 1; k < 32; ++k) mx[q] = fmaxf(mx[q], v[q][k]);
+            }
+            // weights are exp2(S f + e_v - m): the tile's values are held divided by 2^e_v
+            const float f = fmaxf(f_row * pow2f(ek), 1.2e-38f);
+            const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, (float)ev);
+            const bool grow = top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY);
+            float fix = 1.0f;
+            if (grow) {
+                fix = exp2_approx(m_ref - top);  // 0 from -infinity
+                m_ref = top;
+                l *= fix;
+            }
+            if (i > 0) {
+                // the product before this one has read its weights, and O may be touched
+                ok = mbar_wait(pv_done, (i - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (__any_sync(0xffffffffu, grow)) {
+                    umma::fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        umma::ld_32x32(lane_base + c, o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] *= fix;
+                        tmem_st_32x32(lane_base + c, o);
+                    }
+                    umma::fence_before_sync();
+                }
+            }
+            const float off = (float)ev - (m_ref == -INFINITY ? 0.0f : m_ref);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < kPtTile / 8; ++c) {
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    w[k] = exp2_approx(fmaf(v[c >> 2][(c & 3) * 8 + k], f, off));
+                    sum[k & 3] += w[k];
+                }
+                *reinterpret_cast<uint4*>(sm + C::OFF_P + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) =
+                    make_uint4(h2_bits(__floats2half2_rn(w[0], w[2])), h2_bits(__floats2half2_rn(w[1], w[3])),
+                               h2_bits(__floats2half2_rn(w[4], w[6])), h2_bits(__floats2half2_rn(w[5], w[7])));
+            }
+            umma::fence_smem_to_async();
+            umma::fence_before_sync();
+            mbar_arrive(p_ready);
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(-ev), l);
+            if (nb[0] | nb[1] | nb[2] | nb[3]) {  // values that are NaN: held as 0; rows that see one become NaN
+                for (int t = 0; t < kPtTile; ++t)
+                    if ((nb[t >> 5] >> (t & 31) & 1u) && t0 + t <= see_hi && t0 + t >= see_lo) l = NAN;
+            }
+        }
+        if (ok && n_tiles > 0) {
+            ok = mbar_wait(pv_done, (n_tiles - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        umma::fence_after_sync();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D;
+        const __nv_bfloat16* gp = a.gate ? (const __nv_bfloat16*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh : nullptr;
+        const bool gvec = ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            float o[32];
+            if (n_tiles > 0) {
+                umma::ld_32x32(lane_base + c, o);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+            }
+            if (!valid || !ok) continue;
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+                float y[8], g[8];
+                if (gp) ld_act8(gp + c + k, gvec, g);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    y[x] = o[k + x] * inv;
+                    if (gp) y[x] /= 1.0f + expf(-g[x]);
+                }
+                st_act8(dst + c + k, true, y);
+            }
+        }
+        if (!ok && tid == 0) atomicExch(err, 1u);
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == 5) umma::tmem_dealloc(tmem, C::COLS);
+}
+
+// ─── host side ──────────────────────────────────────────────────────────────
+static int pt_tiles_per_seq(const AttnArgs& a) {
+    const int64_t all = ((int64_t)a.seqs.max_seq_len + kPtTile - 1) / kPtTile;
+    if (a.window <= 0) return (int)all;
+    const int64_t seen = ((int64_t)a.window + a.seqs.max_q_len + kPtTile - 1) / kPtTile + 1;
+    return (int)(seen < all ? seen : all);
+}
+template <int D>
+static size_t pt_image_bytes(const AttnArgs& a) {
+    return (size_t)a.seqs.n_seqs * a.cache.kv_heads * pt_tiles_per_seq(a) * 2 * PtCfg<D>::IMG;
+}
+
+// At least a full tile of rows per sequence, and images of at most 4 GB.
+template <int D>
+bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a) {
+    return (int64_t)a.seqs.max_q_len * a.group >= kPtTile && pt_image_bytes<D>(a) <= (size_t)4 << 30 && a.cache.kv_heads <= 65535 &&
+           a.seqs.n_seqs <= 65535;
+}
+
+template <int D>
+int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
+    using C = PtCfg<D>;
+    const int tiles = pt_tiles_per_seq(a);
+    const size_t image = pt_image_bytes<D>(a), meta = (size_t)a.seqs.n_seqs * a.cache.kv_heads * tiles * kPtMeta * 4;
+    int rc = kv4_reserve(e, image + meta);
+    if (rc) return rc;
+    uint8_t* img = reinterpret_cast<uint8_t*>(e->kv4.work);
+    int* mt = reinterpret_cast<int*>(img + image);
+    unsigned int* err = e->dec_sync + 2;
+    int& set = e->kv4.occupancy[48 + D / 64];
+    if (!set) {
+        MOE_CUDA(cudaFuncSetAttribute(kv4_expand_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::IMG));
+        MOE_CUDA(cudaFuncSetAttribute(kv4_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        set = 1;
+    }
+    const int64_t q_rows = (int64_t)a.seqs.max_q_len * a.group;
+    int64_t units = (int64_t)a.seqs.n_tokens * a.group / kPtTile + a.seqs.n_seqs, per = (q_rows + kPtTile - 1) / kPtTile * a.seqs.n_seqs;
+    units = (per < units ? per : units) * a.cache.kv_heads;
+    MOE_REQUIRE(units < 0x7FFFFFFF, "kv4_attention: too many rows for one call");
+    if (tiles > 0) {
+        kv4_expand_kernel<D><<<dim3(2 * tiles, a.cache.kv_heads, a.seqs.n_seqs), 256, C::IMG, e->stream>>>(a, tiles, img, mt, err);
+        e->launches++;
+    }
+    kv4_prompt_kernel<D><<<(unsigned)units, 192, C::SMEM, e->stream>>>(a, tiles, img, mt, err);
+    e->launches++;
+    MOE_CUDA(cudaGetLastError());
+    return MOE_OK;
+}
+
+template bool kv4_prompt_fits<64>(const moe_engine*, const AttnArgs&);
+template bool kv4_prompt_fits<128>(const moe_engine*, const AttnArgs&);
+template bool kv4_prompt_fits<256>(const moe_engine*, const AttnArgs&);
+template int launch_kv4_prompt<64>(moe_engine*, AttnArgs);
+template int launch_kv4_prompt<128>(moe_engine*, AttnArgs);
+template int launch_kv4_prompt<256>(moe_engine*, AttnArgs);
+
+}  // namespace moe
