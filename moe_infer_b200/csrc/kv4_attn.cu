@@ -2,13 +2,18 @@
 //
 //   o[j, h] = sum_t softmax_t(scale q[j, h] . k_t) v_t   over the positions t that row j sees.
 //
-// The nibbles go to the tensor cores as they are: n - 8 is exact in f16, so with k_t = s n + b (per 64 elements, group g)
+// The nibbles go to the tensor cores as they are: n - 8 (n - 7.5 for the values of f32 rows) is exact in f16, so with
+// k_t = s n + b (per 64 elements, group g)
 //   q . k_t = sum_g  s[t, g] (q_g . (n - 8)) + (b + 8 s)[t, g] sum(q_g)
-//   o_g     = sum_t (p_t s[t, g]) (n - 8)    + sum_t p_t (b + 8 s)[t, g]
-// which leaves one scale per score and group instead of one per element, and no rounding of keys or values.  Queries and
-// weights are f16 operands scaled by powers of two; for f32 rows they are split into a high and a low f16 term that share
-// an MMA as rows r and r + 8 (22 bits; the eight query heads of a KV head fill the tile), for bf16 rows one term is
-// exact (queries) or four bits finer than the result's type (weights).  Sums and the softmax are f32.
+//   o_g     = sum_t (w_t s[t, g]) (n - 8)    + sum_t w_t (b + 8 s)[t, g]
+// which leaves one scale per score and group instead of one per element, and no rounding of keys or values.  Keys and
+// values are the A operand of mma.m16n8k16 (16 positions, 16 elements), eight query rows the columns: the eight query
+// heads of a KV head fill it.  Queries and weights are f16 operands scaled by powers of two; for f32 rows they are split
+// into a high and a low f16 term (22 bits) that two MMAs add into the same sums, for bf16 rows one term is exact (queries)
+// or three bits finer than the result's type (weights).  Sums and the softmax are f32.
+//
+// Weights are w = exp2(x - ref), one reference per row: it moves only when a weight times its scale would leave f16's
+// range, then to 2^8 below that; a row's result does not depend on it otherwise.
 //
 // A work unit is (sequence, KV head, row tile): `rows` query rows of the heads that share a KV head against its positions,
 // 64 * TB at a time.  A producer warp brings the tiles' blocks in with bulk copies (one per 16 positions, so pages may end
@@ -24,33 +29,37 @@
 
 namespace moe {
 
-template <int D_, bool F32_, int MT_, int TB_, bool SPLIT_>
+template <int D_, bool F32_, int NT_, int TB_, bool SPLIT_>
 struct AttnCfg {
-    static constexpr int D = D_, MT = MT_, TB = TB_;
+    static constexpr int D = D_, NT = NT_, TB = TB_;
     static constexpr bool F32 = F32_, SPLIT = SPLIT_;
     static constexpr int G = D / 64;               // scale groups of a head
-    static constexpr int RH = F32 ? 1 : 2;         // query rows a lane holds per MMA tile
-    static constexpr int ROWS = 8 * RH * MT;       // query rows of a unit
+    static constexpr int ROWS = 8 * NT;            // query rows of a unit
     static constexpr int NB = 4 * TB;              // blocks of a tile
     static constexpr int TILE = NB * kKv4Block;    // positions of a tile
     static constexpr int TP = 4 / G;               // warps that share a group in the value pass
     static constexpr int PB = NB / TP;             // blocks a warp takes in the value pass
     static constexpr int BLK = kv4_block_bytes(D);
     static constexpr int STAGE = NB * BLK;
-    static constexpr int STAGES = MT >= 4 ? 2 : 3;
+    static constexpr int STAGES = 3;
     static constexpr int KS = D / 16;              // MMA steps over a head
+    static constexpr int QW = F32 ? 16 : 8;        // bytes of a lane's query operand per step
+    static constexpr int PS = 20;                  // floats from one row's weights of a block to the next (no bank conflicts)
     static constexpr int OFF_Q = STAGES * STAGE;
-    static constexpr int OFF_P = OFF_Q + KS * MT * 512;
-    static constexpr int P_BYTES = NB * ROWS * 64;                  // one buffer of weights
+    static constexpr int OFF_P = OFF_Q + KS * NT * 32 * QW;
+    static constexpr int P_BYTES = NB * ROWS * PS * 4;              // one buffer of weights
     static constexpr int RED_BYTES = (TP - 1) * ROWS * D * 4;       // partial sums of the value pass meet in the same place
     static constexpr int P_TOTAL = 2 * P_BYTES > RED_BYTES ? 2 * P_BYTES : RED_BYTES;
-    static constexpr int OFF_M = OFF_P + P_TOTAL;                   // [2][NB][ROWS] running maxima that go with the weights
-    static constexpr int OFF_QS = OFF_M + 2 * NB * ROWS * 4;        // [G][ROWS] sums of the queries' groups
+    static constexpr int OFF_M = OFF_P + P_TOTAL;                   // [2][4][ROWS] references the warps used for a tile
+    static constexpr int OFF_FL = OFF_M + 8 * ROWS * 4;             // [2][4] what the warps have to say about a tile
+    static constexpr int OFF_QS = OFF_FL + 32;                      // [G][ROWS] sums of the queries' groups
     static constexpr int OFF_RF = OFF_QS + G * ROWS * 4;            // [ROWS] factor that makes a score of the MMA's sum
-    static constexpr int OFF_ML = OFF_RF + ROWS * 4;                // [2][4][ROWS] maxima and sums of the warps
-    static constexpr int OFF_BAR = (OFF_ML + 8 * ROWS * 4 + 15) / 16 * 16;
+    static constexpr int OFF_L = OFF_RF + ROWS * 4;                 // [4][ROWS] sums of the warps' weights
+    static constexpr int OFF_BAR = (OFF_L + 4 * ROWS * 4 + 15) / 16 * 16;
     static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 64;
 };
+constexpr float kWeightTop = 14.0f, kWeightSet = 6.0f;  // log2 of weight * scale: at most, and where a new reference puts the largest
+constexpr unsigned kFlagMoved = 1u, kFlagNan = 2u;
 
 // A unit of work and the tiles of it that exist.
 struct AttnUnit {
@@ -140,13 +149,27 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// the same pairs as n - 7.5 (64 + n in steps of 1/16, so the half is exact).  For the values of f32 rows: their sum has no
+// drift then, and the tensor core's truncating sums stay relative to what they hold
+__device__ __forceinline__ void nibbles_mid_h2(uint32_t w, uint32_t (&o)[4]) {
+    const __half2 m = bits_h2(0xD478D478u);
+    o[0] = h2_bits(__hadd2(bits_h2((w << 4 & 0x00F000F0u) | 0x54005400u), m));
+    o[1] = h2_bits(__hadd2(bits_h2((w & 0x00F000F0u) | 0x54005400u), m));
+    o[2] = h2_bits(__hadd2(bits_h2((w >> 4 & 0x00F000F0u) | 0x54005400u), m));
+    o[3] = h2_bits(__hadd2(bits_h2((w >> 8 & 0x00F000F0u) | 0x54005400u), m));
+}
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <class C, typename T>
-__global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
+__global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2 ? 168 : 200) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long red[8];
-    constexpr int D = C::D, G = C::G, MT = C::MT, RH = C::RH, ROWS = C::ROWS, NB = C::NB, TILE = C::TILE;
+    constexpr int D = C::D, G = C::G, NT = C::NT, ROWS = C::ROWS, NB = C::NB, TILE = C::TILE, TB = C::TB, PB = C::PB, PS = C::PS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
     uint64_t* empty = full + C::STAGES;
@@ -252,15 +275,16 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
     }
 
     // ── the four computing warps ──
-    const int r = lane >> 2, c = lane & 3;
-    const int g_own = warp % G, tp = warp / G;  // value pass: group, part of the positions
+    const int r = lane >> 2, c = lane & 3;      // scores: positions 2 r, 2 r + 1 of a block, rows 2 c, 2 c + 1 of eight
+    const int g_own = warp % G, tp = warp / G;  // value pass: group, part of the positions; weights: row r, positions 4 c ..
     const T* qp = (const T*)a.q;
     const T* gatep = (const T*)a.gate;
     T* outp = (T*)a.out;
     float* q_sum = reinterpret_cast<float*>(sm + C::OFF_QS);
     float* row_f = reinterpret_cast<float*>(sm + C::OFF_RF);
-    float* m_buf = reinterpret_cast<float*>(sm + C::OFF_M);
-    float* ml = reinterpret_cast<float*>(sm + C::OFF_ML);
+    float* refs = reinterpret_cast<float*>(sm + C::OFF_M);
+    unsigned* flags = reinterpret_cast<unsigned*>(sm + C::OFF_FL);
+    float* sums = reinterpret_cast<float*>(sm + C::OFF_L);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -281,71 +305,70 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {  // lane: elements (i * 32 + lane)
                 x[i] = valid ? ld_act(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + i * 32 + lane) : 0.0f;
-                mx = max(mx, fabsf(x[i]));
+                mx = fmaxf(mx, fabsf(x[i]));
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            int e = (int)(__float_as_uint(mx) >> 23) - 127;  // mx in [2^e, 2^(e + 1))
-            e = max(e, -110);
-            const float up = pow2f(14 - e > 127 ? 127 : 14 - e);
+            mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+            const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -110);  // mx in [2^e, 2^(e + 1))
+            const float up = pow2f(min(14 - e, 127));
             if (lane == 0) row_f[row] = a.scale_log2 * pow2f(max(e - 14, -126));
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const float v = x[i] * up;
-                const __half hi = __float2half_rn(v);
-                const __half lo = __float2half_rn(v - __half2float(hi));
-                // sums over 64 elements: i even / odd halves of a group
-                float sum = C::F32 ? v : __half2float(hi);
+            for (int g = 0; g < G; ++g) {
+                float sum = 0.0f;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) {
-                    if (i & 1) q_sum[(i >> 1) * ROWS + row] += sum;
-                    else q_sum[(i >> 1) * ROWS + row] = sum;
+                for (int i = 0; i < 2; ++i) {
+                    const float v = x[2 * g + i] * up;
+                    const __half hi = __float2half_rn(v);
+                    sum += C::F32 ? v : __half2float(hi);
+                    // element d of the group -> (step, register, half) of the operand
+                    const int d = i * 32 + lane, cc = d >> 4, jj = (d >> 3) & 1, k8 = d & 7;
+                    const int ks = g * 4 + jj * 2 + ((k8 >> 1) & 1);
+                    uint8_t* dst = sm + C::OFF_Q + ((ks * NT + (row >> 3)) * 32 + (row & 7) * 4 + cc) * C::QW + (k8 & 1) * 4 + (k8 >> 2) * 2;
+                    *reinterpret_cast<__half*>(dst) = hi;
+                    if (C::F32) *reinterpret_cast<__half*>(dst + 8) = __float2half_rn(v - __half2float(hi));
                 }
-                // element d of the head -> (step, register, half) of the A operand
-                const int d = i * 32 + lane, g = d >> 6, cc = (d >> 4) & 3, jj = (d >> 3) & 1, k8 = d & 7;
-                const int ks = g * 4 + jj * 2 + ((k8 >> 1) & 1);
-                const int reg = (k8 & 1) * 2, half = k8 >> 2;  // elements (0,4): a0, (1,5): a2; (2,6), (3,7): next step
-                const int mt = row / (8 * RH), rin = row % (8 * RH);
-                uint8_t* dst = sm + C::OFF_Q + (ks * MT + mt) * 512 + ((rin & 7) * 4 + cc) * 16 + half * 2;
-                if (C::F32) {
-                    *reinterpret_cast<__half*>(dst + reg * 4) = hi;
-                    *reinterpret_cast<__half*>(dst + (reg + 1) * 4) = lo;
-                } else {
-                    *reinterpret_cast<__half*>(dst + (reg + (rin >> 3)) * 4) = hi;
-                }
+                sum = warp_sum(sum);
+                if (lane == 0) q_sum[g * ROWS + row] = sum;
             }
         }
         compute_barrier();
 
-        float m_run[MT][RH], l_run[MT][RH], rf[MT][RH];
-        int see_hi[MT][RH], see_lo[MT][RH];  // positions the row sees: see_lo <= t <= see_hi
+        // rows 2 c and 2 c + 1 of every eight
+        float ref[NT][2], l_run[NT][2], rf[NT][2];
+        int see_hi[NT][2], see_lo[NT][2];  // positions the row sees: see_lo <= t <= see_hi
         int all_hi = 0x7FFFFFFF, all_lo = -1;
-        float o[MT][8][4], o_bias[MT][RH], m_val[MT][RH];
-        int e_run = 0;                       // exponent field of the value scales' reference
+        float o[NT][4][4], o_bias[NT];     // elements 8 r + 2 x and + 1 of the group, rows 2 c and 2 c + 1; row r
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nt = 0; nt < NT; ++nt) {
+            o_bias[nt] = 0.0f;
 #pragma unroll
-            for (int h = 0; h < RH; ++h) {
-                m_run[mt][h] = m_val[mt][h] = -INFINITY;
-                l_run[mt][h] = o_bias[mt][h] = 0.0f;
-                const int row = mt * 8 * RH + h * 8 + r, rr = u.rt * ROWS + row;
-                rf[mt][h] = row_f[row];
+            for (int e = 0; e < 2; ++e) {
+                ref[nt][e] = -INFINITY;
+                l_run[nt][e] = 0.0f;
+                const int row = nt * 8 + 2 * c + e, rr = u.rt * ROWS + row;
+                rf[nt][e] = row_f[row];
                 // rows behind the last are computed unmasked and not written
-                see_hi[mt][h] = rr < rows_all ? pos_base + rr / a.group : 0x7FFFFFFF;
-                see_lo[mt][h] = a.window > 0 && rr < rows_all ? see_hi[mt][h] - a.window + 1 : 0;
-                all_hi = min(all_hi, see_hi[mt][h]);
-                all_lo = max(all_lo, see_lo[mt][h]);
+                see_hi[nt][e] = rr < rows_all ? pos_base + rr / a.group : 0x7FFFFFFF;
+                see_lo[nt][e] = a.window > 0 && rr < rows_all ? see_hi[nt][e] - a.window + 1 : 0;
+                all_hi = min(all_hi, see_hi[nt][e]);
+                all_lo = max(all_lo, see_lo[nt][e]);
             }
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) o[nt][x][i] = 0.0f;
         }
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) {
+        for (int s = 1; s < 4; s <<= 1) {
             all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, s));
             all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, s));
+        }
+        float qs_reg[NT == 1 ? G : 1][2];  // sums of the queries' groups, from shared memory where there are more rows
+        if constexpr (NT == 1) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                qs_reg[g][0] = q_sum[g * ROWS + 2 * c];
+                qs_reg[g][1] = q_sum[g * ROWS + 2 * c + 1];
+            }
         }
 
         int buf = 0;
@@ -355,22 +378,18 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
             if (!ok) *abort_flag = 1;
             const uint8_t* st = sm + stage * C::STAGE;
             // ── scores ──
-#pragma unroll 1
-            for (int tb = 0; tb < C::TB; ++tb) {
-                const int blk = warp * C::TB + tb;
-                const uint8_t* kb = st + blk * C::BLK;
-                const int pos0 = t0 + blk * kKv4Block + 4 * c;  // this lane's positions pos0 .. pos0 + 3
-                float s[MT][RH][4];
+            float s[TB][NT][4];  // (position 2 r, rows 2 c, 2 c + 1), (position 2 r + 1, the same rows)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+            for (int tb = 0; tb < TB; ++tb) {
+                const uint8_t* kb = st + (warp * TB + tb) * C::BLK;
 #pragma unroll
-                    for (int h = 0; h < RH; ++h)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[mt][h][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) s[tb][nt][i] = 0.0f;
                 constexpr int U = G >= 2 ? 2 : 1;
 #pragma unroll
                 for (int it = 0; it < G / U; ++it) {
-                    uint32_t kw[2][2 * U];  // key tile, word of (group, j)
+                    uint32_t kw[2][2 * U];  // position parity, word of (group, j)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if constexpr (U == 2) {
@@ -384,208 +403,250 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
 #pragma unroll
                     for (int uu = 0; uu < U; ++uu) {
                         const int g = it * U + uu;
-                        float acc[MT][2][4];
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) acc[mt][i][k] = 0.0f;
+                        float acc[NT][4];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             uint32_t nb[2][4];
                             nibbles_h2(kw[0][uu * 2 + j], nb[0]);
                             nibbles_h2(kw[1][uu * 2 + j], nb[1]);
 #pragma unroll
-                            for (int v = 0; v < 2; ++v)
+                            for (int v = 0; v < 2; ++v) {
+                                const uint4 ka = make_uint4(nb[0][2 * v], nb[1][2 * v], nb[0][2 * v + 1], nb[1][2 * v + 1]);
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    const uint4 af = *reinterpret_cast<const uint4*>(sm + C::OFF_Q + ((g * 4 + j * 2 + v) * MT + mt) * 512 + lane * 16);
-                                    mma_f16(acc[mt][0], af, nb[0][2 * v], nb[0][2 * v + 1]);
-                                    mma_f16(acc[mt][1], af, nb[1][2 * v], nb[1][2 * v + 1]);
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const uint8_t* qa = sm + C::OFF_Q + (((g * 4 + j * 2 + v) * NT + nt) * 32 + lane) * C::QW;
+                                    if constexpr (C::F32) {
+                                        const uint4 qf = *reinterpret_cast<const uint4*>(qa);
+                                        if (j == 0 && v == 0) mma_f16_zero(acc[nt], ka, qf.x, qf.y);
+                                        else mma_f16(acc[nt], ka, qf.x, qf.y);
+                                        mma_f16(acc[nt], ka, qf.z, qf.w);
+                                    } else {
+                                        const uint2 qf = *reinterpret_cast<const uint2*>(qa);
+                                        if (j == 0 && v == 0) mma_f16_zero(acc[nt], ka, qf.x, qf.y);
+                                        else mma_f16(acc[nt], ka, qf.x, qf.y);
+                                    }
                                 }
+                            }
                         }
-                        const uint4 pr = *reinterpret_cast<const uint4*>(kb + 8 * D + g * 64 + c * 16);
-                        const uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
+                        const uint2 pr = *reinterpret_cast<const uint2*>(kb + 8 * D + g * 64 + r * 8);
+                        const uint32_t pw[2] = {pr.x, pr.y};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {  // position pos0 + k: key tile k % 2, column 2 c + k / 2
+                        for (int k = 0; k < 2; ++k) {
                             const float sc = __uint_as_float(pw[k] << 16), bi = fmaf(8.0f, sc, __uint_as_float(pw[k] & 0xFFFF0000u));
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt)
+                            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int h = 0; h < RH; ++h) {
-                                    const float qs = q_sum[g * ROWS + mt * 8 * RH + h * 8 + r];
-                                    const float d = C::F32 ? acc[mt][k & 1][k >> 1] + acc[mt][k & 1][2 + (k >> 1)] : acc[mt][k & 1][2 * h + (k >> 1)];
-                                    s[mt][h][k] = fmaf(sc, d, fmaf(bi, qs, s[mt][h][k]));
+                                for (int e = 0; e < 2; ++e) {
+                                    const float qs = NT == 1 ? qs_reg[NT == 1 ? g : 0][e] : q_sum[g * ROWS + nt * 8 + 2 * c + e];
+                                    s[tb][nt][2 * k + e] = fmaf(sc, acc[nt][2 * k + e], fmaf(bi, qs, s[tb][nt][2 * k + e]));
                                 }
                         }
                     }
                 }
-                const bool whole = t0 + TILE - 1 <= all_hi && t0 >= all_lo;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int h = 0; h < RH; ++h) {
-                        const int row = mt * 8 * RH + h * 8 + r;
-                        float mx = -INFINITY;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float x = s[mt][h][k] * rf[mt][h];
-                            if (!whole && (pos0 + k > see_hi[mt][h] || pos0 + k < see_lo[mt][h])) x = -INFINITY;
-                            s[mt][h][k] = x;
-                            mx = fmaxf(mx, x);
-                        }
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float m_new = fmaxf(m_run[mt][h], mx);
-                        const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-                        float4 p;
-                        p.x = exp2_approx(s[mt][h][0] - m_ref);
-                        p.y = exp2_approx(s[mt][h][1] - m_ref);
-                        p.z = exp2_approx(s[mt][h][2] - m_ref);
-                        p.w = exp2_approx(s[mt][h][3] - m_ref);
-                        l_run[mt][h] = fmaf(l_run[mt][h], exp2_approx(m_run[mt][h] - m_ref), (p.x + p.y) + (p.z + p.w));
-                        m_run[mt][h] = m_new;
-                        *reinterpret_cast<float4*>(sm + C::OFF_P + buf * C::P_BYTES + (blk * ROWS + row) * 64 + c * 16) = p;
-                        if (c == 0) m_buf[(buf * NB + blk) * ROWS + row] = m_new;
-                    }
             }
+            // the largest scale of each block's values (NaN, as a bit pattern, above every number)
+            unsigned my_flags = 0;
+            float ev[TB];
+#pragma unroll
+            for (int tb = 0; tb < TB; ++tb) {
+                const int blk = warp * TB + tb;
+                const uint8_t* vp = st + blk * C::BLK + 17 * D;
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < (G + 1) / 2; ++i) {  // a lane's pairs: positions of its own, groups 2 i and 2 i + 1
+                    const int g = 2 * i + (lane >> 4), t = lane & 15;
+                    if (g < G) {
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + g * 64 + t * 4) << 16;
+                        if (t0 + blk * kKv4Block + t < u.len) m = max(m, x);
+                    }
+                }
+                m = __reduce_max_sync(0xffffffffu, m);
+                if (m >= 0x7F800000u) {
+                    my_flags |= kFlagNan;
+                    m = 0;
+#pragma unroll
+                    for (int i = 0; i < (G + 1) / 2; ++i) {
+                        const int g = 2 * i + (lane >> 4), t = lane & 15;
+                        if (g < G) {
+                            const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + g * 64 + t * 4) << 16;
+                            if (x < 0x7F800000u && t0 + blk * kKv4Block + t < u.len) m = max(m, x);
+                        }
+                    }
+                    m = __reduce_max_sync(0xffffffffu, m);
+                }
+                ev[tb] = (float)(max((int)(m >> 23) - 126, -100));  // scales below 2^ev
+            }
+            // weights
+            const bool whole = t0 + TILE - 1 <= all_hi && t0 >= all_lo;
+            float use[NT][2], sum[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int tb = 0; tb < TB; ++tb) {
+                        const int pos = t0 + (warp * TB + tb) * kKv4Block + 2 * r;
+                        float x0 = s[tb][nt][e] * rf[nt][e], x1 = s[tb][nt][2 + e] * rf[nt][e];
+                        if (!whole) {
+                            if (pos > see_hi[nt][e] || pos < see_lo[nt][e]) x0 = -INFINITY;
+                            if (pos + 1 > see_hi[nt][e] || pos + 1 < see_lo[nt][e]) x1 = -INFINITY;
+                        }
+                        s[tb][nt][e] = x0;
+                        s[tb][nt][2 + e] = x1;
+                        top = fmaxf(top, fmaxf(x0, x1) + ev[tb]);
+                    }
+                    use[nt][e] = top;
+                }
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) use[nt][e] = fmaxf(use[nt][e], __shfl_xor_sync(0xffffffffu, use[nt][e], k));
+            bool moved = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const bool mv = use[nt][e] > ref[nt][e] + kWeightTop;
+                    moved |= mv;
+                    use[nt][e] = mv ? use[nt][e] - kWeightSet : ref[nt][e];
+                    const float off = use[nt][e] == -INFINITY ? 0.0f : use[nt][e];
+                    sum[nt][e] = 0.0f;
+#pragma unroll
+                    for (int tb = 0; tb < TB; ++tb) {
+                        s[tb][nt][e] = exp2_approx(s[tb][nt][e] - off);
+                        s[tb][nt][2 + e] = exp2_approx(s[tb][nt][2 + e] - off);
+                        sum[nt][e] += s[tb][nt][e] + s[tb][nt][2 + e];
+                        *reinterpret_cast<float2*>(sm + C::OFF_P + buf * C::P_BYTES + (((warp * TB + tb) * ROWS + nt * 8 + 2 * c + e) * PS + 2 * r) * 4) =
+                            make_float2(s[tb][nt][e], s[tb][nt][2 + e]);
+                    }
+                }
+            if (__any_sync(0xffffffffu, moved)) my_flags |= kFlagMoved;
+            if (r == 0) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    *reinterpret_cast<float2*>(refs + (buf * 4 + warp) * ROWS + nt * 8 + 2 * c) = make_float2(use[nt][0], use[nt][1]);
+            }
+            if (lane == 0) flags[buf * 4 + warp] = my_flags;
             compute_barrier();
             if (*(volatile int*)abort_flag) ok = false;
             // ── values ──
-            // the largest scale this warp meets in the tile, positions past the sequence's end left out
+            const uint4 fl = *reinterpret_cast<const uint4*>(flags + buf * 4);
+            const unsigned any = fl.x | fl.y | fl.z | fl.w;
+            const bool weird = any & kFlagNan, reref = any & kFlagMoved;
+            float off_r[NT];  // the common reference of row r
+            if (reref) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float fix[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = nt * 8 + 2 * c + e;
+                        float m = ref[nt][e];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m = fmaxf(m, refs[(buf * 4 + i) * ROWS + row]);
+                        const float off = m == -INFINITY ? 0.0f : m;
+                        fix[e] = exp2_approx(ref[nt][e] - off);
+                        l_run[nt][e] *= fix[e];
+                        sum[nt][e] *= exp2_approx(use[nt][e] - off);
+                        ref[nt][e] = m;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        o[nt][x][0] *= fix[0];
+                        o[nt][x][1] *= fix[1];
+                        o[nt][x][2] *= fix[0];
+                        o[nt][x][3] *= fix[1];
+                    }
+                    // row r: its common reference and fix are held by lane r / 2 (rows 2 c, 2 c + 1)
+                    const float m0 = __shfl_sync(0xffffffffu, ref[nt][0], r >> 1), m1 = __shfl_sync(0xffffffffu, ref[nt][1], r >> 1);
+                    const float x0 = __shfl_sync(0xffffffffu, fix[0], r >> 1), x1 = __shfl_sync(0xffffffffu, fix[1], r >> 1);
+                    const float m = (r & 1) ? m1 : m0;
+                    off_r[nt] = m == -INFINITY ? 0.0f : m;
+                    o_bias[nt] *= (r & 1) ? x1 : x0;
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) l_run[nt][e] += sum[nt][e];
             const bool tail = t0 + TILE > u.len;
-            uint32_t e_max = 0;
+            float acc[C::F32 ? NT : 1][4][4];  // f32 rows: the tile's sums, added to the unit's with f32 rounding
 #pragma unroll
-            for (int pb = 0; pb < C::PB; ++pb) {
-                const int blk = tp * C::PB + pb;
-                const uint4 pr = *reinterpret_cast<const uint4*>(st + blk * C::BLK + 17 * D + g_own * 64 + c * 16);
-                const uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (!tail || t0 + blk * kKv4Block + 4 * c + k < u.len) e_max = max(e_max, (pw[k] >> 7) & 0xFFu);
-            }
-            e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, 1));
-            e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, 2));
-            // a group that was stored as NaN must not reach rows that do not see it (weight 0), nor set the reference
-            const bool weird = e_max == 0xFFu;
-            if (weird) {
-                e_max = 0;
-                for (int pb = 0; pb < C::PB; ++pb) {
-                    const int blk = tp * C::PB + pb;
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t pw = *reinterpret_cast<const uint32_t*>(st + blk * C::BLK + 17 * D + g_own * 64 + c * 16 + k * 4);
-                        const uint32_t ex = (pw >> 7) & 0xFFu;
-                        if (ex != 0xFFu && (!tail || t0 + blk * kKv4Block + 4 * c + k < u.len)) e_max = max(e_max, ex);
-                    }
-                }
-                e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, 1));
-                e_max = max(e_max, __shfl_xor_sync(0xffffffffu, e_max, 2));
-            }
-            if ((int)e_max > e_run) {
-                const int e_new = max((int)e_max, 20);
-                const float f = e_run == 0 ? 0.0f : pow2f(max(e_run - e_new, -126));
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[mt][n][i] *= f;
-                e_run = e_new;
-            }
-            const float s_up = pow2f(127 - max(e_run, 20) + 14);
-            float f_blk[MT][RH][C::PB];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < RH; ++h) {
-                    const int row = mt * 8 * RH + h * 8 + r;
-                    float m_new = m_val[mt][h];
-#pragma unroll
-                    for (int pb = 0; pb < C::PB; ++pb) {
-                        f_blk[mt][h][pb] = m_buf[(buf * NB + tp * C::PB + pb) * ROWS + row];
-                        m_new = fmaxf(m_new, f_blk[mt][h][pb]);
-                    }
-                    const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-#pragma unroll
-                    for (int pb = 0; pb < C::PB; ++pb) f_blk[mt][h][pb] = exp2_approx(f_blk[mt][h][pb] - m_ref);
-                    if (m_new != m_val[mt][h]) {
-                        const float f = exp2_approx(m_val[mt][h] - m_ref);
-                        o_bias[mt][h] *= f;
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            if (C::F32) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) o[mt][n][i] *= f;
-                            } else {
-                                o[mt][n][2 * h] *= f;
-                                o[mt][n][2 * h + 1] *= f;
-                            }
-                        }
-                        m_val[mt][h] = m_new;
-                    }
-                }
-#pragma unroll 1
-            for (int pb = 0; pb < C::PB; ++pb) {
-                const int blk = tp * C::PB + pb;
+            for (int pb = 0; pb < PB; ++pb) {
+                const int blk = tp * PB + pb;
                 const uint8_t* vb = st + blk * C::BLK + 9 * D;
                 const uint4 vw = *reinterpret_cast<const uint4*>(vb + g_own * 512 + lane * 16);
                 const uint4 pr = *reinterpret_cast<const uint4*>(vb + 8 * D + g_own * 64 + c * 16);
-                const uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
+                uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
+                if (tail) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (t0 + blk * kKv4Block + 4 * c + k >= u.len) pw[k] = 0;
+                }
                 float sc[4], bi[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const bool in = !tail || t0 + blk * kKv4Block + 4 * c + k < u.len;
-                    const float s0 = in ? __uint_as_float(pw[k] << 16) : 0.0f;
-                    bi[k] = in ? fmaf(8.0f, s0, __uint_as_float(pw[k] & 0xFFFF0000u)) : 0.0f;
-                    sc[k] = s0 * s_up;
+                    sc[k] = __uint_as_float(pw[k] << 16);
+                    bi[k] = fmaf(C::F32 ? 7.5f : 8.0f, sc[k], __uint_as_float(pw[k] & 0xFFFF0000u));
                 }
-                uint32_t nb[4][4];  // word x: {b0 of tile 2x, b0 of 2x + 1, b1 of 2x, b1 of 2x + 1}
-                nibbles_h2(vw.x, nb[0]);
-                nibbles_h2(vw.y, nb[1]);
-                nibbles_h2(vw.z, nb[2]);
-                nibbles_h2(vw.w, nb[3]);
+                uint32_t nb[4][4];  // word x: elements 8 r + 2 x, 8 r + 2 x + 1 of positions (0, 2), then of (1, 3)
+                if constexpr (C::F32) {
+                    nibbles_mid_h2(vw.x, nb[0]);
+                    nibbles_mid_h2(vw.y, nb[1]);
+                    nibbles_mid_h2(vw.z, nb[2]);
+                    nibbles_mid_h2(vw.w, nb[3]);
+                } else {
+                    nibbles_h2(vw.x, nb[0]);
+                    nibbles_h2(vw.y, nb[1]);
+                    nibbles_h2(vw.z, nb[2]);
+                    nibbles_h2(vw.w, nb[3]);
+                }
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t af[4];
-#pragma unroll
-                    for (int h = 0; h < RH; ++h) {
-                        const int row = mt * 8 * RH + h * 8 + r;
-                        float4 p = *reinterpret_cast<const float4*>(sm + C::OFF_P + buf * C::P_BYTES + (blk * ROWS + row) * 64 + c * 16);
-                        float f = f_blk[mt][h][0];  // f_blk[mt][h][pb] without indexing registers by a variable
-#pragma unroll
-                        for (int k = 1; k < C::PB; ++k) f = pb == k ? f_blk[mt][h][k] : f;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float4 p = *reinterpret_cast<const float4*>(sm + C::OFF_P + buf * C::P_BYTES + ((blk * ROWS + nt * 8 + r) * PS + 4 * c) * 4);
+                    if (reref) {
+                        const float f = exp2_approx(refs[(buf * 4 + blk / TB) * ROWS + nt * 8 + r] - off_r[nt]);
                         p.x *= f; p.y *= f; p.z *= f; p.w *= f;
-                        if (!weird) {
-                            o_bias[mt][h] += fmaf(p.x, bi[0], p.y * bi[1]) + fmaf(p.z, bi[2], p.w * bi[3]);
-                            p.x *= sc[0]; p.y *= sc[1]; p.z *= sc[2]; p.w *= sc[3];
-                        } else {
-                            o_bias[mt][h] += (p.x == 0.0f ? 0.0f : p.x * bi[0]) + (p.y == 0.0f ? 0.0f : p.y * bi[1]) +
-                                             (p.z == 0.0f ? 0.0f : p.z * bi[2]) + (p.w == 0.0f ? 0.0f : p.w * bi[3]);
-                            p.x = p.x == 0.0f ? 0.0f : p.x * sc[0];
-                            p.y = p.y == 0.0f ? 0.0f : p.y * sc[1];
-                            p.z = p.z == 0.0f ? 0.0f : p.z * sc[2];
-                            p.w = p.w == 0.0f ? 0.0f : p.w * sc[3];
-                        }
-                        const __half2 h02 = __floats2half2_rn(p.x, p.z), h13 = __floats2half2_rn(p.y, p.w);
-                        if (C::F32) {
-                            const float2 b02 = __half22float2(h02), b13 = __half22float2(h13);
-                            af[0] = h2_bits(h02);
-                            af[2] = h2_bits(h13);
-                            af[1] = h2_bits(__floats2half2_rn(p.x - b02.x, p.z - b02.y));
-                            af[3] = h2_bits(__floats2half2_rn(p.y - b13.x, p.w - b13.y));
-                        } else {
-                            af[h] = h2_bits(h02);
-                            af[2 + h] = h2_bits(h13);
-                        }
                     }
-                    const uint4 av = make_uint4(af[0], af[1], af[2], af[3]);
+                    if (!weird) {
+                        o_bias[nt] = fmaf(p.x, bi[0], fmaf(p.y, bi[1], fmaf(p.z, bi[2], fmaf(p.w, bi[3], o_bias[nt]))));
+                        p.x *= sc[0]; p.y *= sc[1]; p.z *= sc[2]; p.w *= sc[3];
+                    } else {  // a group that was stored as NaN must not reach rows that do not see it (weight 0)
+                        o_bias[nt] += (p.x == 0.0f ? 0.0f : p.x * bi[0]) + (p.y == 0.0f ? 0.0f : p.y * bi[1]) +
+                                      (p.z == 0.0f ? 0.0f : p.z * bi[2]) + (p.w == 0.0f ? 0.0f : p.w * bi[3]);
+                        p.x = p.x == 0.0f ? 0.0f : p.x * sc[0];
+                        p.y = p.y == 0.0f ? 0.0f : p.y * sc[1];
+                        p.z = p.z == 0.0f ? 0.0f : p.z * sc[2];
+                        p.w = p.w == 0.0f ? 0.0f : p.w * sc[3];
+                    }
+                    const __half2 h02 = __floats2half2_rn(p.x, p.z), h13 = __floats2half2_rn(p.y, p.w);
+                    const uint32_t b0 = h2_bits(h02), b1 = h2_bits(h13);
+                    if constexpr (C::F32) {
+                        const float2 f02 = __half22float2(h02), f13 = __half22float2(h13);
+                        const uint32_t l0 = h2_bits(__floats2half2_rn(p.x - f02.x, p.z - f02.y)), l1 = h2_bits(__floats2half2_rn(p.y - f13.x, p.w - f13.y));
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        mma_f16(o[mt][2 * x], av, nb[x][0], nb[x][2]);
-                        mma_f16(o[mt][2 * x + 1], av, nb[x][1], nb[x][3]);
+                        for (int x = 0; x < 4; ++x) {
+                            const uint4 va = make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]);
+                            if (pb == 0) mma_f16_zero(acc[nt][x], va, b0, b1);
+                            else mma_f16(acc[nt][x], va, b0, b1);
+                            mma_f16(acc[nt][x], va, l0, l1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) mma_f16(o[nt][x], make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]), b0, b1);
                     }
                 }
+            }
+            if constexpr (C::F32) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[nt][x][i] += acc[nt][x][i];
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + stage);
@@ -597,106 +658,82 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
         }
         if (!ok) break;
 
-        // ── the unit's end: maxima and sums of the warps, sums of the value pass ──
+        // ── the unit's end: sums of the warps' weights, sums of the value pass ──
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int h = 0; h < RH; ++h) {
-                const int row = mt * 8 * RH + h * 8 + r;
-                float l = l_run[mt][h], ob = o_bias[mt][h];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                ob += __shfl_xor_sync(0xffffffffu, ob, 1);
-                ob += __shfl_xor_sync(0xffffffffu, ob, 2);
-                o_bias[mt][h] = ob;
-                if (c == 0) {
-                    ml[warp * ROWS + row] = m_run[mt][h];
-                    ml[(4 + warp) * ROWS + row] = l;
-                }
+            for (int e = 0; e < 2; ++e) {
+                float l = l_run[nt][e];
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+                if (r == 0) sums[warp * ROWS + nt * 8 + 2 * c + e] = l;
             }
+            float ob = o_bias[nt];
+            ob += __shfl_xor_sync(0xffffffffu, ob, 1);
+            ob += __shfl_xor_sync(0xffffffffu, ob, 2);
+            const float b0 = __shfl_sync(0xffffffffu, ob, 8 * c), b1 = __shfl_sync(0xffffffffu, ob, 8 * c + 4);  // of rows 2 c, 2 c + 1
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                o[nt][x][0] += b0;
+                o[nt][x][1] += b1;
+                o[nt][x][2] += b0;
+                o[nt][x][3] += b1;
+            }
+        }
         compute_barrier();
         const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles <= w_end;
-        const float unscale_a = pow2f(max(min(max(e_run, 20) - 127 - 14, 127), -126));
         float* slot = nullptr;
         if (C::SPLIT && !whole_unit) slot = a.part + (size_t)(2 * blockIdx.x + (w_at <= w_begin ? 0 : 1)) * ROWS * (D + 2);
         float* red_o = reinterpret_cast<float*>(sm + C::OFF_P);
+        const int d0 = 64 * g_own + 8 * r;
+        if (C::TP > 1) {
+            if (tp > 0) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < RH; ++h) {
-                const int row = mt * 8 * RH + h * 8 + r;
-                float m = -INFINITY, l = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) m = fmaxf(m, ml[i * ROWS + row]);
-                const float m_ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) l = fmaf(ml[(4 + i) * ROWS + row], exp2_approx(ml[i * ROWS + row] - m_ref), l);
-                const float f = exp2_approx(m_val[mt][h] - m_ref);
-                const float fo = f * unscale_a, fb = f * o_bias[mt][h];
-                // 16 elements of the row: 64 g + 16 c + (0..7) in column 0 of the MMA tiles, + 8 in column 1
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const float x0 = C::F32 ? o[mt][n][0] + o[mt][n][2] : o[mt][n][2 * h];
-                    const float x1 = C::F32 ? o[mt][n][1] + o[mt][n][3] : o[mt][n][2 * h + 1];
-                    o[mt][n][C::F32 ? 0 : 2 * h] = fmaf(x0, fo, fb);
-                    o[mt][n][C::F32 ? 1 : 2 * h + 1] = fmaf(x1, fo, fb);
-                }
-                l_run[mt][h] = l;
-                m_run[mt][h] = m;
-                if (C::TP > 1 && tp > 0) {
-                    float* d = red_o + ((size_t)(tp - 1) * ROWS + row) * D + 64 * g_own + 16 * c;
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        d[n] = o[mt][n][C::F32 ? 0 : 2 * h];
-                        d[8 + n] = o[mt][n][C::F32 ? 1 : 2 * h + 1];
+                    for (int e = 0; e < 2; ++e) {
+                        float4* d = reinterpret_cast<float4*>(red_o + ((size_t)(tp - 1) * ROWS + nt * 8 + 2 * c + e) * D + d0);
+                        d[0] = make_float4(o[nt][0][e], o[nt][0][2 + e], o[nt][1][e], o[nt][1][2 + e]);
+                        d[1] = make_float4(o[nt][2][e], o[nt][2][2 + e], o[nt][3][e], o[nt][3][2 + e]);
                     }
-                }
             }
-        if (C::TP > 1) compute_barrier();
+            compute_barrier();
+        }
         if (tp == 0) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int h = 0; h < RH; ++h) {
-                    const int row = mt * 8 * RH + h * 8 + r, rr = u.rt * ROWS + row;
-                    float y[16];
+                for (int e = 0; e < 2; ++e) {
+                    const int row = nt * 8 + 2 * c + e, rr = u.rt * ROWS + row;
+                    float y[8];
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        y[n] = o[mt][n][C::F32 ? 0 : 2 * h];
-                        y[8 + n] = o[mt][n][C::F32 ? 1 : 2 * h + 1];
+                    for (int x = 0; x < 4; ++x) {
+                        y[2 * x] = o[nt][x][e];
+                        y[2 * x + 1] = o[nt][x][2 + e];
                     }
-                    if (C::TP > 1) {
 #pragma unroll
-                        for (int t = 0; t < C::TP - 1; ++t) {
-                            const float* d = red_o + ((size_t)t * ROWS + row) * D + 64 * g_own + 16 * c;
+                    for (int t = 0; t < C::TP - 1; ++t) {
+                        const float* d = red_o + ((size_t)t * ROWS + row) * D + d0;
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) y[n] += d[n];
-                        }
+                        for (int n = 0; n < 8; ++n) y[n] += d[n];
                     }
-                    const int d0 = 64 * g_own + 16 * c;
+                    const float l = (sums[row] + sums[ROWS + row]) + (sums[2 * ROWS + row] + sums[3 * ROWS + row]);
                     if (slot) {
-                        float4* dst = reinterpret_cast<float4*>(slot + (size_t)row * D + d0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                        if (g_own == 0 && c == 0) {
-                            slot[(size_t)ROWS * D + row] = m_run[mt][h];
-                            slot[(size_t)ROWS * (D + 1) + row] = l_run[mt][h];
+                        st_act8(slot + (size_t)row * D + d0, true, y);
+                        if (g_own == 0 && r == 0) {
+                            slot[(size_t)ROWS * D + row] = ref[nt][e];
+                            slot[(size_t)ROWS * (D + 1) + row] = l;
                         }
                     } else if (rr < rows_all) {
                         const int j = rr / a.group, hq = u.h * a.group + rr % a.group;
-                        const float inv = l_run[mt][h] == 0.0f ? 0.0f : 1.0f / l_run[mt][h];
-                        T* dst = outp + ((int64_t)(u.row0 + j) * a.heads + hq) * D + d0;
+                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                         const T* gp = gatep ? gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)hq * a.gh + d0 : nullptr;
 #pragma unroll
-                        for (int n = 0; n < 16; ++n) {
+                        for (int n = 0; n < 8; ++n) {
                             y[n] *= inv;
                             if (gp) y[n] /= 1.0f + expf(-ld_act(gp + n));
                         }
-                        float y0[8], y1[8];
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) { y0[n] = y[n]; y1[n] = y[8 + n]; }
-                        st_act8(dst, true, y0);
-                        st_act8(dst + 8, true, y1);
+                        st_act8(outp + ((int64_t)(u.row0 + j) * a.heads + hq) * D + d0, true, y);
                     }
                 }
         }
@@ -704,91 +741,173 @@ __global__ void __launch_bounds__(160) kv4_attn_kernel(AttnArgs a, unsigned int*
     }
 }
 
-// Joins the partial results of units that were split over CTAs: one CTA per row of such a unit.
+// Joins the partial results of units that were split over CTAs.  grid: x = units (or, where there are more of those, the
+// borders between CTAs: a border splits at most one unit, and a unit is joined by the first border inside it), y = pieces of
+// a unit's rows x elements.  The plan is made before the wait: the batch's arrays were there before the attention kernel.
 template <class C, typename T>
-__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, unsigned int* err) {
-    pdl_wait();
-    constexpr int D = C::D, ROWS = C::ROWS, COLS = D / 4, PARTS = 256 / COLS;
-    __shared__ long long red[8];
-    __shared__ float4 sums[256];
-    __shared__ float ls[256];
-    // grid: x = row of the tile, y = row tile, z = (sequence, KV head)
-    const int row = blockIdx.x, rt = blockIdx.y, b = blockIdx.z / a.cache.kv_heads, h = blockIdx.z % a.cache.kv_heads;
-    const Kv4Seq s = kv4_seq(a.seqs, b, err);
-    const int rr = rt * ROWS + row;
-    if (rr >= s.q_len * a.group) return;
-    int rts, lo, tiles;
-    attn_seq_tiles<C>(a, s, rts, lo, tiles);
-    // tiles before this unit: those of the sequences before b, then of the units before this one
-    const int tid = threadIdx.x;
-    long long mine = 0, before = 0, total = 0;
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, int row_tiles, int by_border, unsigned int* err) {
+    constexpr int D = C::D, ROWS = C::ROWS;
+    __shared__ long long red[8], found[4];
+    __shared__ float4 acc_s[256];
+    __shared__ float f_s[256], l_s[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto cost = [&](int b, int& rts, int& tiles) -> long long {
+        int lo;
+        const Kv4Seq s = kv4_seq(a.seqs, b, err);
+        attn_seq_tiles<C>(a, s, rts, lo, tiles);
+        return (long long)rts * tiles * a.cache.kv_heads;
+    };
+    // total of all tiles, and of those of sequences before `b_unit`
+    const int b_unit = by_border ? 0 : blockIdx.x / (row_tiles * a.cache.kv_heads);
+    long long mine = 0, mine_before = 0;
     for (int i = tid; i < a.seqs.n_seqs; i += 256) {
-        const Kv4Seq si = kv4_seq(a.seqs, i, err);
-        int r2, l2, t2;
-        attn_seq_tiles<C>(a, si, r2, l2, t2);
-        const long long cst = (long long)r2 * t2 * a.cache.kv_heads;
+        int r2, t2;
+        const long long cst = cost(i, r2, t2);
         mine += cst;
-        if (i < b) before += cst;
+        if (i < b_unit) mine_before += cst;
     }
+    auto block_sum = [&](long long v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if ((tid & 31) == 0) red[tid >> 5] = mine;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) total += red[w];
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = before;
-    __syncthreads();
-    before = 0;
-    for (int w = 0; w < 8; ++w) before += red[w];
-    const long long at = before + (long long)(h * rts + rt) * tiles, n = min((long long)splits, total);
-    const int i0 = (int)(((at + 1) * n - 1) / total), i1 = (int)(((at + tiles) * n - 1) / total);
-    if (i0 == i1) return;  // the unit was written whole
-    // slot of CTA i's part of this unit: its first unit has the even one
-    auto slot_of = [&](int i) { return (size_t)(2 * i + (i > i0 || total * i / n >= at ? 0 : 1)) * ROWS * (D + 2); };
-    const int col = tid % COLS, part = tid / COLS;
-    float m = -INFINITY;
-    for (int i = i0 + part; i <= i1; i += PARTS) m = fmaxf(m, a.part[slot_of(i) + (size_t)ROWS * D + row]);
-    ls[tid] = m;
-    __syncthreads();
-    m = -INFINITY;
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if (lane == 0) red[warp] = v;
+        __syncthreads();
+        long long t = 0;
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) m = fmaxf(m, ls[p * COLS]);
-    __syncthreads();
-    const float m_ref = m == -INFINITY ? 0.0f : m;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = i0 + part; i <= i1; i += PARTS) {
-        const float* sp = a.part + slot_of(i);
-        const float f = exp2_approx(sp[(size_t)ROWS * D + row] - m_ref);
-        const float4 v = reinterpret_cast<const float4*>(sp + (size_t)row * D)[col];
-        l = fmaf(sp[(size_t)ROWS * (D + 1) + row], f, l);
-        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-    }
-    sums[tid] = acc;
-    ls[tid] = l;
-    __syncthreads();
-    if (part != 0) return;
+        for (int i = 0; i < 8; ++i) t += red[i];
+        return t;
+    };
+    const long long total = block_sum(mine), n = min((long long)splits, total);
+    int b = b_unit, h = 0, rt = 0, tiles = 0;
+    long long at = 0;
+    bool work = total > 0;
+    if (!by_border) {
+        int rts;
+        at = block_sum(mine_before);
+        cost(b, rts, tiles);
+        const int in = blockIdx.x % (row_tiles * a.cache.kv_heads);
+        h = in / row_tiles;
+        rt = in - h * row_tiles;
+        work = work && rt < rts;
+        at += (long long)(h * rts + rt) * tiles;
+    } else {
+        const long long border = blockIdx.x + 1;
+        work = work && border < n;
+        const long long x = work ? total * border / n : 0;
+        if (work) {  // the sequence that holds tile x: chunks of 256 sequences, prefix sums by one thread each
+            long long carry = 0;
+            for (int b0 = 0; b0 < a.seqs.n_seqs; b0 += 256) {
+                int r2 = 0, t2 = 0;
+                const long long cst = b0 + tid < a.seqs.n_seqs ? cost(b0 + tid, r2, t2) : 0;
+                long long inc = cst;
 #pragma unroll
-    for (int p = 1; p < PARTS; ++p) {
-        const float4 v = sums[p * COLS + col];
-        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-        l += ls[p * COLS + col];
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int j = rr / a.group, hq = h * a.group + rr % a.group;
-    float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    if (a.gate) {
-        const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + 4 * col;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                __syncthreads();
+                if (lane == 31) red[warp] = inc;
+                __syncthreads();
+                long long before = carry, sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] /= 1.0f + expf(-ld_act(gp + i));
+                for (int i = 0; i < 8; ++i) {
+                    if (i < warp) before += red[i];
+                    sum += red[i];
+                }
+                const long long lo = before + inc - cst;
+                if (x >= lo && x < lo + cst) {
+                    const int unit = (int)((x - lo) / t2);
+                    found[0] = b0 + tid;
+                    found[1] = unit;
+                    found[2] = lo + (long long)unit * t2;
+                }
+                carry += sum;
+                if (x < carry) break;
+            }
+            __syncthreads();
+            b = (int)found[0];
+            int rts;
+            cost(b, rts, tiles);
+            h = (int)found[1] / rts;
+            rt = (int)found[1] - h * rts;
+            at = found[2];
+            work = at < x;  // a border between units splits none
+        }
     }
-    T* dst = (T*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D + 4 * col;
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    int i0 = 0, i1 = 0;
+    if (work) {
+        i0 = (int)(((at + 1) * n - 1) / total);
+        i1 = (int)(((at + tiles) * n - 1) / total);
+        work = i0 < i1 && (!by_border || i0 == (int)blockIdx.x);
+    }
+    pdl_wait();
+    if (!work) return;
+    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const int rows_all = s.q_len * a.group;
+    const bool first_odd = total * i0 / n < at;  // CTA i0 began before this unit: its part is in the odd slot
+    auto slot_of = [&](int i) { return a.part + (size_t)(2 * i + (i == i0 && first_odd ? 1 : 0)) * ROWS * (D + 2); };
+    // a piece: one row, 64 elements: 16 columns of four x 16 CTAs at a time
+    for (int piece = blockIdx.y; piece < ROWS * (D / 64); piece += gridDim.y) {
+        const int row = piece / (D / 64), d0 = piece % (D / 64) * 64, rr = rt * ROWS + row;
+        if (rr >= rows_all) break;
+        const int col = tid & 15, part = tid >> 4;
+        float m = -INFINITY;
+        for (int i = i0 + tid; i <= i1; i += 256) m = fmaxf(m, slot_of(i)[(size_t)ROWS * D + row]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        __syncthreads();
+        if (lane == 0) l_s[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, l_s[i]);
+        const float off = m == -INFINITY ? 0.0f : m;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+        for (int c0 = i0; c0 <= i1; c0 += 256) {
+            __syncthreads();
+            if (c0 + tid <= i1) {
+                const float* sp = slot_of(c0 + tid);
+                const float f = exp2_approx(sp[(size_t)ROWS * D + row] - off);
+                f_s[tid] = f;
+                l = fmaf(sp[(size_t)ROWS * (D + 1) + row], f, l);
+            }
+            __syncthreads();
+            const int here = min(256, i1 - c0 + 1);
+#pragma unroll 8
+            for (int k = part; k < here; k += 16) {
+                const float4 v = reinterpret_cast<const float4*>(slot_of(c0 + k) + (size_t)row * D + d0)[col];
+                const float f = f_s[k];
+                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+            }
+        }
+        l = warp_sum(l);
+        __syncthreads();
+        acc_s[tid] = acc;
+        if (lane == 0) l_s[warp] = l;
+        __syncthreads();
+        if (part == 0) {
+            l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) l += l_s[i];
+#pragma unroll
+            for (int p = 1; p < 16; ++p) {
+                const float4 v = acc_s[p * 16 + col];
+                acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int j = rr / a.group, hq = h * a.group + rr % a.group;
+            float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            if (a.gate) {
+                const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + d0 + 4 * col;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] /= 1.0f + expf(-ld_act(gp + i));
+            }
+            T* dst = (T*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D + d0 + 4 * col;
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+            else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        }
+        __syncthreads();
+    }
 }
 
 // ─── host side ──────────────────────────────────────────────────────────────
@@ -834,21 +953,27 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
         int rc = kv4_reserve(e, (size_t)grid * 2 * C::ROWS * (C::D + 2) * 4);
         if (rc) return rc;
         a.part = e->kv4.work;
-        MOE_REQUIRE((int64_t)a.seqs.n_seqs * a.cache.kv_heads <= 65535 && row_tiles <= 65535, "kv4_attention: too many sequences for one call");
         MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)grid), dim3(160), C::SMEM, e->stream, a, err));
-        MOE_CUDA(launch_kernel(true, kv4_attn_join_kernel<C, T>, dim3(C::ROWS, (unsigned)row_tiles, (unsigned)(a.seqs.n_seqs * a.cache.kv_heads)),
-                               dim3(256), 0, e->stream, a, (int)grid, err));
-        e->launches += 2;
+        e->launches++;
+        if (grid == 1) return MOE_OK;  // nothing can be split
+        const int64_t all = (int64_t)a.seqs.n_seqs * a.cache.kv_heads * row_tiles;
+        const bool by_border = all > grid - 1;
+        const int64_t x = by_border ? grid - 1 : all;
+        int64_t y = 4 * e->sm_count / x;  // about four CTAs per SM
+        y = y < 1 ? 1 : y > C::ROWS * (C::D / 64) ? C::ROWS * (C::D / 64) : y;
+        MOE_CUDA(launch_kernel(true, kv4_attn_join_kernel<C, T>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, e->stream, a, (int)grid,
+                               (int)row_tiles, by_border ? 1 : 0, err));
+        e->launches++;
         return MOE_OK;
     }
 }
 
-// Rows of the tile: as few MMA tiles as hold a sequence's rows, up to four.  Units of their own (no splitting) once they
-// fill the GPU twice over.
+// Rows of the tile: as few columns of eight as hold a sequence's rows, up to four.  Units of their own (no splitting) once
+// they fill the GPU twice over.
 template <int D, typename T>
 static int launch_attn(moe_engine* e, const AttnArgs& a) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int R1 = F32 ? 8 : 16, V0 = (D == 64 ? 0 : D == 128 ? 8 : 16) + (F32 ? 4 : 0);
+    constexpr int V0 = (D == 64 ? 0 : D == 128 ? 8 : 16) + (F32 ? 4 : 0);
     const int64_t q_rows = (int64_t)a.seqs.max_q_len * a.group, n = a.seqs.n_seqs;
     auto units = [&](int rows) {  // at most: whole tiles of all rows, and one that is not full for every sequence
         const int64_t per_seq = (q_rows + rows - 1) / rows;
@@ -858,11 +983,12 @@ static int launch_attn(moe_engine* e, const AttnArgs& a) {
     constexpr int TB = 4 / (D / 64);
     if constexpr (!F32) {
         if (kv4_prompt_fits<D>(e, a)) return launch_kv4_prompt<D>(e, a);
+    } else {
+        if (q_rows > 16 && units(32) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(32));
     }
-    if (q_rows > 2 * R1 && units(4 * R1) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(4 * R1));
-    if (q_rows > 2 * R1) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(4 * R1));
-    if (q_rows > R1) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(2 * R1));
-    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(R1));
+    if (q_rows > 16) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(32));
+    if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16));
+    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8));
 }
 
 int check_kv4(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b);
