@@ -2,7 +2,7 @@
 //
 //   o[j, h] = sum_t softmax_t(scale q[j, h] . k_t) v_t   over the positions t that row j sees.
 //
-// The nibbles go to the tensor cores as they are: n - 8 (n - 7.5 for the values of f32 rows) is exact in f16, so with
+// The nibbles go to the tensor cores as they are: n - 8 (or 7) is exact in f16, so with
 // k_t = s n + b (per 64 elements, group g)
 //   q . k_t = sum_g  s[t, g] (q_g . (n - 8)) + (b + 8 s)[t, g] sum(q_g)
 //   o_g     = sum_t (w_t s[t, g]) (n - 8)    + sum_t w_t (b + 8 s)[t, g]
@@ -24,6 +24,8 @@
 // sequences of any lengths balance; units that cross CTAs leave partial sums that a second kernel joins.  Many rows
 // (prompts): one CTA per unit over the positions its rows see, nothing to join.
 #include <math.h>
+
+#include <type_traits>
 
 #include "kv4_attn.cuh"
 
@@ -59,7 +61,7 @@ struct AttnCfg {
     static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 64;
 };
 constexpr float kWeightTop = 14.0f, kWeightSet = 6.0f;  // log2 of weight * scale: at most, and where a new reference puts the largest
-constexpr unsigned kFlagMoved = 1u, kFlagNan = 2u;
+constexpr unsigned kFlagMoved = 1u, kFlagNan = 2u, kFlagTail = 4u;
 
 // A unit of work and the tiles of it that exist.
 struct AttnUnit {
@@ -153,15 +155,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
-}
-// the same pairs as n - 7.5 (64 + n in steps of 1/16, so the half is exact).  For the values of f32 rows: their sum has no
-// drift then, and the tensor core's truncating sums stay relative to what they hold
-__device__ __forceinline__ void nibbles_mid_h2(uint32_t w, uint32_t (&o)[4]) {
-    const __half2 m = bits_h2(0xD478D478u);
-    o[0] = h2_bits(__hadd2(bits_h2((w << 4 & 0x00F000F0u) | 0x54005400u), m));
-    o[1] = h2_bits(__hadd2(bits_h2((w & 0x00F000F0u) | 0x54005400u), m));
-    o[2] = h2_bits(__hadd2(bits_h2((w >> 4 & 0x00F000F0u) | 0x54005400u), m));
-    o[3] = h2_bits(__hadd2(bits_h2((w >> 8 & 0x00F000F0u) | 0x54005400u), m));
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -445,33 +438,28 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                 }
             }
             // the largest scale of each block's values (NaN, as a bit pattern, above every number)
-            unsigned my_flags = 0;
+            const bool tail = t0 + TILE > u.len;
+            unsigned my_flags = tail ? kFlagTail : 0u;
             float ev[TB];
 #pragma unroll
             for (int tb = 0; tb < TB; ++tb) {
-                const int blk = warp * TB + tb;
-                const uint8_t* vp = st + blk * C::BLK + 17 * D;
-                uint32_t m = 0;
+                const int blk = warp * TB + tb, t = lane & 15;
+                const uint8_t* vp = st + blk * C::BLK + 17 * D + t * 4;
+                const bool in = !tail || t0 + blk * kKv4Block + t < u.len;
+                // a lane's pairs: of one position, every other group
+                uint32_t x[(G + 1) / 2], m = 0;
 #pragma unroll
-                for (int i = 0; i < (G + 1) / 2; ++i) {  // a lane's pairs: positions of its own, groups 2 i and 2 i + 1
-                    const int g = 2 * i + (lane >> 4), t = lane & 15;
-                    if (g < G) {
-                        const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + g * 64 + t * 4) << 16;
-                        if (t0 + blk * kKv4Block + t < u.len) m = max(m, x);
-                    }
+                for (int i = 0; i < (G + 1) / 2; ++i) {
+                    x[i] = *reinterpret_cast<const uint32_t*>(vp + (G == 1 ? 0 : 2 * i + (lane >> 4)) * 64) << 16;
+                    if (!in) x[i] = 0;
+                    m = max(m, x[i]);
                 }
                 m = __reduce_max_sync(0xffffffffu, m);
                 if (m >= 0x7F800000u) {
                     my_flags |= kFlagNan;
                     m = 0;
 #pragma unroll
-                    for (int i = 0; i < (G + 1) / 2; ++i) {
-                        const int g = 2 * i + (lane >> 4), t = lane & 15;
-                        if (g < G) {
-                            const uint32_t x = *reinterpret_cast<const uint32_t*>(vp + g * 64 + t * 4) << 16;
-                            if (x < 0x7F800000u && t0 + blk * kKv4Block + t < u.len) m = max(m, x);
-                        }
-                    }
+                    for (int i = 0; i < (G + 1) / 2; ++i) m = max(m, x[i] < 0x7F800000u ? x[i] : 0u);
                     m = __reduce_max_sync(0xffffffffu, m);
                 }
                 ev[tb] = (float)(max((int)(m >> 23) - 126, -100));  // scales below 2^ev
@@ -480,23 +468,29 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             const bool whole = t0 + TILE - 1 <= all_hi && t0 >= all_lo;
             float use[NT][2], sum[NT][2];
 #pragma unroll
+            for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[tb][nt][i] *= rf[nt][i & 1];
+            if (!whole) {
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int pos = t0 + (warp * TB + tb) * kKv4Block + 2 * r + (i >> 1);
+                            if (pos > see_hi[nt][i & 1] || pos < see_lo[nt][i & 1]) s[tb][nt][i] = -INFINITY;
+                        }
+            }
+#pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = -INFINITY;
+                    use[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]) + ev[0];
 #pragma unroll
-                    for (int tb = 0; tb < TB; ++tb) {
-                        const int pos = t0 + (warp * TB + tb) * kKv4Block + 2 * r;
-                        float x0 = s[tb][nt][e] * rf[nt][e], x1 = s[tb][nt][2 + e] * rf[nt][e];
-                        if (!whole) {
-                            if (pos > see_hi[nt][e] || pos < see_lo[nt][e]) x0 = -INFINITY;
-                            if (pos + 1 > see_hi[nt][e] || pos + 1 < see_lo[nt][e]) x1 = -INFINITY;
-                        }
-                        s[tb][nt][e] = x0;
-                        s[tb][nt][2 + e] = x1;
-                        top = fmaxf(top, fmaxf(x0, x1) + ev[tb]);
-                    }
-                    use[nt][e] = top;
+                    for (int tb = 1; tb < TB; ++tb) use[nt][e] = fmaxf(use[nt][e], fmaxf(s[tb][nt][e], s[tb][nt][2 + e]) + ev[tb]);
                 }
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1)
@@ -535,9 +529,8 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             // ── values ──
             const uint4 fl = *reinterpret_cast<const uint4*>(flags + buf * 4);
             const unsigned any = fl.x | fl.y | fl.z | fl.w;
-            const bool weird = any & kFlagNan, reref = any & kFlagMoved;
-            float off_r[NT];  // the common reference of row r
-            if (reref) {
+            if (any & kFlagMoved) {
+                // rare: the rows' references become the largest of the warps'; every warp corrects the weights it wrote
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float fix[2];
@@ -547,11 +540,15 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                         float m = ref[nt][e];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) m = fmaxf(m, refs[(buf * 4 + i) * ROWS + row]);
-                        const float off = m == -INFINITY ? 0.0f : m;
+                        const float off = m == -INFINITY ? 0.0f : m, f = exp2_approx(use[nt][e] - off);
                         fix[e] = exp2_approx(ref[nt][e] - off);
                         l_run[nt][e] *= fix[e];
-                        sum[nt][e] *= exp2_approx(use[nt][e] - off);
+                        sum[nt][e] *= f;
                         ref[nt][e] = m;
+#pragma unroll
+                        for (int tb = 0; tb < TB; ++tb)
+                            *reinterpret_cast<float2*>(sm + C::OFF_P + buf * C::P_BYTES + (((warp * TB + tb) * ROWS + row) * PS + 2 * r) * 4) =
+                                make_float2(s[tb][nt][e] * f, s[tb][nt][2 + e] * f);
                     }
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -560,28 +557,27 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                         o[nt][x][2] *= fix[0];
                         o[nt][x][3] *= fix[1];
                     }
-                    // row r: its common reference and fix are held by lane r / 2 (rows 2 c, 2 c + 1)
-                    const float m0 = __shfl_sync(0xffffffffu, ref[nt][0], r >> 1), m1 = __shfl_sync(0xffffffffu, ref[nt][1], r >> 1);
+                    // row r: its correction is held by lane r / 2 (rows 2 c, 2 c + 1)
                     const float x0 = __shfl_sync(0xffffffffu, fix[0], r >> 1), x1 = __shfl_sync(0xffffffffu, fix[1], r >> 1);
-                    const float m = (r & 1) ? m1 : m0;
-                    off_r[nt] = m == -INFINITY ? 0.0f : m;
                     o_bias[nt] *= (r & 1) ? x1 : x0;
                 }
+                compute_barrier();
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) l_run[nt][e] += sum[nt][e];
-            const bool tail = t0 + TILE > u.len;
             float acc[C::F32 ? NT : 1][4][4];  // f32 rows: the tile's sums, added to the unit's with f32 rounding
-#pragma unroll
-            for (int pb = 0; pb < PB; ++pb) {
+            // mid: n - 8 and n - 7 in turn, so that the sums of the nibbles, whose middle is 7.5, have no drift: the tensor core's
+            // truncating sums then stay relative to what they hold (f32 rows over 250,001 positions: 9e-7 off, 1.5e-5 with n - 8 alone)
+            auto block_of_values = [&](int pb, auto slow, auto first, auto mid) {
+                constexpr int kMid = decltype(mid)::value;
                 const int blk = tp * PB + pb;
                 const uint8_t* vb = st + blk * C::BLK + 9 * D;
                 const uint4 vw = *reinterpret_cast<const uint4*>(vb + g_own * 512 + lane * 16);
                 const uint4 pr = *reinterpret_cast<const uint4*>(vb + 8 * D + g_own * 64 + c * 16);
                 uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
-                if (tail) {
+                if constexpr (decltype(slow)::value) {  // positions past the sequence's end
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (t0 + blk * kKv4Block + 4 * c + k >= u.len) pw[k] = 0;
@@ -590,28 +586,17 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     sc[k] = __uint_as_float(pw[k] << 16);
-                    bi[k] = fmaf(C::F32 ? 7.5f : 8.0f, sc[k], __uint_as_float(pw[k] & 0xFFFF0000u));
+                    bi[k] = fmaf((float)kMid, sc[k], __uint_as_float(pw[k] & 0xFFFF0000u));
                 }
                 uint32_t nb[4][4];  // word x: elements 8 r + 2 x, 8 r + 2 x + 1 of positions (0, 2), then of (1, 3)
-                if constexpr (C::F32) {
-                    nibbles_mid_h2(vw.x, nb[0]);
-                    nibbles_mid_h2(vw.y, nb[1]);
-                    nibbles_mid_h2(vw.z, nb[2]);
-                    nibbles_mid_h2(vw.w, nb[3]);
-                } else {
-                    nibbles_h2(vw.x, nb[0]);
-                    nibbles_h2(vw.y, nb[1]);
-                    nibbles_h2(vw.z, nb[2]);
-                    nibbles_h2(vw.w, nb[3]);
-                }
+                nibbles_h2<kMid>(vw.x, nb[0]);
+                nibbles_h2<kMid>(vw.y, nb[1]);
+                nibbles_h2<kMid>(vw.z, nb[2]);
+                nibbles_h2<kMid>(vw.w, nb[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float4 p = *reinterpret_cast<const float4*>(sm + C::OFF_P + buf * C::P_BYTES + ((blk * ROWS + nt * 8 + r) * PS + 4 * c) * 4);
-                    if (reref) {
-                        const float f = exp2_approx(refs[(buf * 4 + blk / TB) * ROWS + nt * 8 + r] - off_r[nt]);
-                        p.x *= f; p.y *= f; p.z *= f; p.w *= f;
-                    }
-                    if (!weird) {
+                    if constexpr (!decltype(slow)::value) {
                         o_bias[nt] = fmaf(p.x, bi[0], fmaf(p.y, bi[1], fmaf(p.z, bi[2], fmaf(p.w, bi[3], o_bias[nt]))));
                         p.x *= sc[0]; p.y *= sc[1]; p.z *= sc[2]; p.w *= sc[3];
                     } else {  // a group that was stored as NaN must not reach rows that do not see it (weight 0)
@@ -630,7 +615,7 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             const uint4 va = make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]);
-                            if (pb == 0) mma_f16_zero(acc[nt][x], va, b0, b1);
+                            if constexpr (decltype(first)::value) mma_f16_zero(acc[nt][x], va, b0, b1);
                             else mma_f16(acc[nt][x], va, b0, b1);
                             mma_f16(acc[nt][x], va, l0, l1);
                         }
@@ -639,6 +624,22 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                         for (int x = 0; x < 4; ++x) mma_f16(o[nt][x], make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]), b0, b1);
                     }
                 }
+            };
+            using Yes = std::true_type;
+            using No = std::false_type;
+            using M8 = std::integral_constant<int, 8>;
+            using M7 = std::integral_constant<int, 7>;
+            if ((any & (kFlagNan | kFlagTail)) == 0) {
+                block_of_values(0, No{}, Yes{}, M8{});
+                if constexpr (PB > 1) block_of_values(1, No{}, No{}, M7{});
+                if constexpr (PB > 2) {
+                    block_of_values(2, No{}, No{}, M8{});
+                    block_of_values(3, No{}, No{}, M7{});
+                }
+            } else {
+                block_of_values(0, Yes{}, Yes{}, M8{});
+#pragma unroll 1
+                for (int pb = 1; pb < PB; ++pb) block_of_values(pb, Yes{}, No{}, M7{});
             }
             if constexpr (C::F32) {
 #pragma unroll
