@@ -43,7 +43,7 @@ struct AttnCfg {
     static constexpr int PB = NB / TP;             // blocks a warp takes in the value pass
     static constexpr int BLK = kv4_block_bytes(D);
     static constexpr int STAGE = NB * BLK;
-    static constexpr int STAGES = 3;
+    static constexpr int STAGES = NT == 1 ? 2 : 3;
     static constexpr int KS = D / 16;              // MMA steps over a head
     static constexpr int QW = F32 ? 16 : 8;        // bytes of a lane's query operand per step
     static constexpr int PS = 20;                  // floats from one row's weights of a block to the next (no bank conflicts)
@@ -70,6 +70,10 @@ struct AttnUnit {
     int t_lo, n_tiles;   // first position (multiple of the tile) and tiles
 };
 
+// What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
+// CTA that got many short sequences would finish last (lengths 100 to 16,000: 107 us without, @@ us with).
+constexpr int kUnitCost = 3;
+
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
 template <class C>
 __device__ __forceinline__ void attn_seq_tiles(const AttnArgs& a, const Kv4Seq& s, int& rts, int& lo, int& tiles) {
@@ -94,7 +98,7 @@ __device__ AttnPlan attn_scan(const AttnArgs& a, int nthreads, long long (&red)[
         const Kv4Seq s = kv4_seq(a.seqs, b, err);
         int rts, lo, tiles;
         attn_seq_tiles<C>(a, s, rts, lo, tiles);
-        return (long long)rts * tiles * a.cache.kv_heads;
+        return (long long)rts * (tiles + kUnitCost) * a.cache.kv_heads;
     };
     long long mine = 0;
     for (int b = tid; b < a.seqs.n_seqs; b += nthreads) mine += cost(b);
@@ -147,12 +151,12 @@ __device__ AttnPlan attn_scan(const AttnArgs& a, int nthreads, long long (&red)[
 
 // ─── small device pieces ────────────────────────────────────────────────────
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
@@ -192,10 +196,10 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             attn_seq_tiles<C>(a, s, rts, u.t_lo, u.n_tiles);
             u.b = p.b; u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len;
             const long long in = w_begin - p.prefix;
-            const int unit = (int)(in / u.n_tiles);
+            const int unit = (int)(in / (u.n_tiles + kUnitCost));
             u.h = unit / rts;
             u.rt = unit - u.h * rts;
-            w_at = p.prefix + (long long)unit * u.n_tiles;  // first tile of the unit
+            w_at = p.prefix + (long long)unit * (u.n_tiles + kUnitCost);  // where the unit begins: kUnitCost steps, then its tiles
         } else {
             // one unit per CTA, the units of a sequence's last rows (the longest) first; units are counted in row tiles
             const int h = blockIdx.x % a.cache.kv_heads;
@@ -216,14 +220,14 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             const int p0 = s.len - s.q_len + j0, p1 = s.len - s.q_len + j1;
             u.t_lo = a.window > 0 ? max(p0 - a.window + 1, 0) / TILE * TILE : 0;
             u.n_tiles = max((p1 + 1 - u.t_lo + TILE - 1) / TILE, 1);
-            w_begin = 0; w_end = u.n_tiles; w_at = 0;
+            w_begin = 0; w_end = u.n_tiles + kUnitCost; w_at = 0;
         }
     }
     __syncthreads();
 
     // steps to the unit behind u
     auto next_unit = [&](AttnUnit& n, long long& at) {
-        at += n.n_tiles;
+        at += n.n_tiles + kUnitCost;
         int rts, lo, tiles;
         Kv4Seq s{n.row0, n.q_len, n.len};
         attn_seq_tiles<C>(a, s, rts, lo, tiles);
@@ -246,22 +250,26 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (long long w = w_begin; w < w_end && ok; ++w) {
-            if (w >= at + n.n_tiles) next_unit(n, at);
-            const int pos = n.t_lo + (int)(w - at) * TILE + lane * kKv4Block;
-            const uint8_t* src = nullptr;
-            if (lane < NB && pos < n.len) src = kv4_block(a.cache, a.seqs, n.b, n.h, pos, C::BLK, err);
-            ok = mbar_wait(empty + stage, phase ^ 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const unsigned have = __ballot_sync(0xffffffffu, src != nullptr);
-            if (lane == 0) mbar_expect_tx(full + stage, __popc(have) * C::BLK);
-            __syncwarp();
-            if (src) bulk_g2s(sm + stage * C::STAGE + lane * C::BLK, src, C::BLK, full + stage);
-            if (++stage == C::STAGES) {
-                stage = 0;
-                phase ^= 1;
+        for (;;) {
+            const int t_first = (int)max(w_begin - at - kUnitCost, 0ll), t_stop = (int)min(w_end - at - kUnitCost, (long long)n.n_tiles);
+            for (int t = t_first; t < t_stop && ok; ++t) {
+                const int pos = n.t_lo + t * TILE + lane * kKv4Block;
+                const uint8_t* src = nullptr;
+                if (lane < NB && pos < n.len) src = kv4_block(a.cache, a.seqs, n.b, n.h, pos, C::BLK, err);
+                ok = mbar_wait(empty + stage, phase ^ 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const unsigned have = __ballot_sync(0xffffffffu, src != nullptr);
+                if (lane == 0) mbar_expect_tx(full + stage, __popc(have) * C::BLK);
+                __syncwarp();
+                if (src) bulk_g2s(sm + stage * C::STAGE + lane * C::BLK, src, C::BLK, full + stage);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
             }
+            if (!ok || at + n.n_tiles + kUnitCost >= w_end) break;
+            next_unit(n, at);
         }
         if (!ok && lane == 0) atomicExch(err, 1u);
         return;
@@ -281,25 +289,30 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (long long w = w_begin; w < w_end && ok;) {
-        if (w >= w_at + u.n_tiles) next_unit(u, w_at);
-        const long long w_stop = min(w_end, w_at + u.n_tiles);
+    for (bool more = true; more && ok;) {
+        const int t_first = (int)max(w_begin - w_at - kUnitCost, 0ll), t_stop = (int)min(w_end - w_at - kUnitCost, (long long)u.n_tiles);
         const int rows_all = u.q_len * a.group;
         const int pos_base = u.len - u.q_len;
 
         // queries of the unit as MMA operands: a warp takes a row at a time; scaled by a power of two so that the largest
         // element lies in [2^14, 2^15)
-        for (int row = warp; row < ROWS; row += 4) {
-            const int rr = u.rt * ROWS + row;
+        float xq[ROWS / 4][D / 32];  // all of a warp's rows are requested before the first is worked on
+#pragma unroll
+        for (int i = 0; i < ROWS / 4; ++i) {
+            const int rr = u.rt * ROWS + warp + 4 * i;
             const bool valid = rr < rows_all;
             const int j = valid ? rr / a.group : 0, hq = u.h * a.group + (valid ? rr % a.group : 0);
-            float x[D / 32];
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)  // lane: elements (k * 32 + lane)
+                xq[i][k] = valid ? ld_act(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + k * 32 + lane) : 0.0f;
+        }
+#pragma unroll
+        for (int ri = 0; ri < ROWS / 4; ++ri) {
+            const int row = warp + 4 * ri;
+            float (&x)[D / 32] = xq[ri];
             float mx = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {  // lane: elements (i * 32 + lane)
-                x[i] = valid ? ld_act(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + i * 32 + lane) : 0.0f;
-                mx = fmaxf(mx, fabsf(x[i]));
-            }
+            for (int i = 0; i < D / 32; ++i) mx = fmaxf(mx, fabsf(x[i]));
             mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
             const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -110);  // mx in [2^e, 2^(e + 1))
             const float up = pow2f(min(14 - e, 127));
@@ -365,8 +378,8 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         }
 
         int buf = 0;
-        for (; w < w_stop; ++w, buf ^= 1) {
-            const int t0 = u.t_lo + (int)(w - w_at) * TILE;
+        for (int ti = t_first; ti < t_stop; ++ti, buf ^= 1) {
+            const int t0 = u.t_lo + ti * TILE;
             ok = mbar_wait(full + stage, phase);
             if (!ok) *abort_flag = 1;
             const uint8_t* st = sm + stage * C::STAGE;
@@ -682,7 +695,7 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             }
         }
         compute_barrier();
-        const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles <= w_end;
+        const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles + kUnitCost <= w_end;
         float* slot = nullptr;
         if (C::SPLIT && !whole_unit) slot = a.part + (size_t)(2 * blockIdx.x + (w_at <= w_begin ? 0 : 1)) * ROWS * (D + 2);
         float* red_o = reinterpret_cast<float*>(sm + C::OFF_P);
@@ -739,6 +752,8 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                 }
         }
         compute_barrier();  // the weights' place and the row tables are free again
+        more = w_at + u.n_tiles + kUnitCost < w_end;
+        if (more) next_unit(u, w_at);
     }
 }
 
@@ -756,6 +771,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
         int lo;
         const Kv4Seq s = kv4_seq(a.seqs, b, err);
         attn_seq_tiles<C>(a, s, rts, lo, tiles);
+        tiles += kUnitCost;
         return (long long)rts * tiles * a.cache.kv_heads;
     };
     // total of all tiles, and of those of sequences before `b_unit`
@@ -948,7 +964,7 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
     } else {
         // no more CTAs than tiles there can be
         const int64_t row_tiles = ((int64_t)a.seqs.max_q_len * a.group + C::ROWS - 1) / C::ROWS;
-        const int64_t most = units * ((a.seqs.max_seq_len + C::TILE - 1) / C::TILE + 1);
+        const int64_t most = units * ((a.seqs.max_seq_len + C::TILE - 1) / C::TILE + 1 + kUnitCost);
         int64_t grid = (int64_t)e->sm_count * occ;
         if (grid > most) grid = most;
         int rc = kv4_reserve(e, (size_t)grid * 2 * C::ROWS * (C::D + 2) * 4);
