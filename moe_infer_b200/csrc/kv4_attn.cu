@@ -16,8 +16,8 @@
 // range, then to 2^8 below that; a row's result does not depend on it otherwise.
 //
 // A work unit is (sequence, KV head, row tile): `rows` query rows of the heads that share a KV head against its positions,
-// 64 * TB at a time.  A producer warp brings the tiles' blocks in with bulk copies (one per 16 positions, so pages may end
-// anywhere), four warps compute: in the score pass each warp owns a quarter of the tile's positions and keeps a running
+// 64 * TB at a time.  The tiles' blocks come in by bulk copies (one per 16 positions, so pages may end anywhere).  Four warps:
+// in the score pass each owns a quarter of the tile's positions and keeps a running
 // maximum and sum of its own, in the value pass it owns a group of 64 elements (and, for heads of less than four groups, a
 // part of the positions); the weights cross in shared memory, one barrier per tile.
 // Few rows (decode, verification): the tiles of all units are dealt evenly to as many CTAs as fit the GPU, in one line, so
@@ -58,7 +58,7 @@ struct AttnCfg {
     static constexpr int OFF_RF = OFF_QS + G * ROWS * 4;            // [ROWS] factor that makes a score of the MMA's sum
     static constexpr int OFF_L = OFF_RF + ROWS * 4;                 // [4][ROWS] sums of the warps' weights
     static constexpr int OFF_BAR = (OFF_L + 4 * ROWS * 4 + 15) / 16 * 16;
-    static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 64;
+    static constexpr int SMEM = OFF_BAR + STAGES * 8 + 16;
 };
 constexpr float kWeightTop = 14.0f, kWeightSet = 6.0f;  // log2 of weight * scale: at most, and where a new reference puts the largest
 constexpr unsigned kFlagMoved = 1u, kFlagNan = 2u, kFlagTail = 4u;
@@ -73,6 +73,12 @@ struct AttnUnit {
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (lengths 100 to 16,000: 107 us without, @@ us with).
 constexpr int kUnitCost = 3;
+
+struct AttnWalk {
+    AttnUnit n;
+    long long at;
+    int t, t_stop, more;
+};
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
 template <class C>
@@ -163,19 +169,16 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <class C, typename T>
-__global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2 ? 168 : 200) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
+__global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2 ? 168 : 255) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long red[8];
+    __shared__ AttnWalk walk;
     constexpr int D = C::D, G = C::G, NT = C::NT, ROWS = C::ROWS, NB = C::NB, TILE = C::TILE, TB = C::TB, PB = C::PB, PS = C::PS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
-    uint64_t* empty = full + C::STAGES;
-    int* abort_flag = reinterpret_cast<int*>(empty + C::STAGES);
+    int* abort_flag = reinterpret_cast<int*>(full + C::STAGES);
     if (tid == 0) {
-        for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(full + i, 1);
-            mbar_init(empty + i, 4);
-        }
+        for (int i = 0; i < C::STAGES; ++i) mbar_init(full + i, 1);
         mbar_fence_init();
         *abort_flag = 0;
     }
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     {
         AttnPlan p;
         if constexpr (C::SPLIT) {
-            p = attn_scan<C>(a, 160, red, err);
+            p = attn_scan<C>(a, 128, red, err);
             w_begin = p.begin;
             w_end = p.end;
             if (w_begin >= w_end) return;
@@ -243,39 +246,75 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         attn_seq_tiles<C>(a, s, rts, n.t_lo, n.n_tiles);
     };
 
-    if (warp == 4) {
-        // ── producer ──
-        AttnUnit n = u;
-        long long at = w_at;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (;;) {
-            const int t_first = (int)max(w_begin - at - kUnitCost, 0ll), t_stop = (int)min(w_end - at - kUnitCost, (long long)n.n_tiles);
-            for (int t = t_first; t < t_stop && ok; ++t) {
-                const int pos = n.t_lo + t * TILE + lane * kKv4Block;
-                const uint8_t* src = nullptr;
-                if (lane < NB && pos < n.len) src = kv4_block(a.cache, a.seqs, n.b, n.h, pos, C::BLK, err);
-                ok = mbar_wait(empty + stage, phase ^ 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const unsigned have = __ballot_sync(0xffffffffu, src != nullptr);
-                if (lane == 0) mbar_expect_tx(full + stage, __popc(have) * C::BLK);
-                __syncwarp();
-                if (src) bulk_g2s(sm + stage * C::STAGE + lane * C::BLK, src, C::BLK, full + stage);
-                if (++stage == C::STAGES) {
-                    stage = 0;
-                    phase ^= 1;
+    // The first warp also brings the tiles in, STAGES - 1 ahead: a tile's place is free once all warps have met at the barrier
+    // of the tile after it.  Its walk over the CTA's tiles lies in shared memory; the pages of the next tile to copy are
+    // looked up one tile before, so that the table's latency is not waited for.
+    int nx_page = -1, nx_block = 0;  // lane: page and block of its 16 positions in that tile; -1: none
+    auto look_up = [&]() {           // advances to the next tile (walk.t of walk.n) and looks its pages up
+        while (walk.more && walk.t >= walk.t_stop) {
+            __syncwarp();
+            if (lane == 0) {
+                AttnUnit n = walk.n;
+                long long at = walk.at;
+                walk.more = at + n.n_tiles + kUnitCost < w_end;
+                if (walk.more) {
+                    next_unit(n, at);
+                    walk.n = n;
+                    walk.at = at;
+                    walk.t = 0;
+                    walk.t_stop = (int)min(w_end - at - kUnitCost, (long long)n.n_tiles);
                 }
             }
-            if (!ok || at + n.n_tiles + kUnitCost >= w_end) break;
-            next_unit(n, at);
+            __syncwarp();
         }
-        if (!ok && lane == 0) atomicExch(err, 1u);
-        return;
+        nx_page = -1;
+        if (walk.more && lane < NB) {
+            const int pos = walk.n.t_lo + walk.t * TILE + lane * kKv4Block;
+            if (pos < walk.n.len) {
+                const int pg = pos / a.cache.page_size;
+                nx_block = (pos - pg * a.cache.page_size) / kKv4Block;
+                nx_page = pg < a.seqs.max_pages ? a.seqs.page_table[(size_t)walk.n.b * a.seqs.max_pages + pg] : -2;
+                if (nx_page == -1) nx_page = -2;
+            }
+        }
+    };
+    auto bring = [&](int st) {
+        if (!walk.more) return;
+        bool copy = nx_page != -1;
+        if (copy && (nx_page < 0 || nx_page >= a.cache.num_pages)) {
+            atomicExch(err, kErrKv4Page);
+            copy = false;
+        }
+        const unsigned have = __ballot_sync(0xffffffffu, copy);
+        if (lane == 0) mbar_expect_tx(full + st, __popc(have) * C::BLK);
+        __syncwarp();
+        if (copy) {
+            const int blocks = a.cache.page_size / kKv4Block;
+            bulk_g2s(sm + st * C::STAGE + lane * C::BLK,
+                     a.cache.pages + (((size_t)nx_page * a.cache.kv_heads + walk.n.h) * blocks + nx_block) * C::BLK, C::BLK, full + st);
+        }
+        __syncwarp();
+        if (lane == 0) ++walk.t;
+        __syncwarp();
+        look_up();
+    };
+    int stage = 0, st_in = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            walk.n = u;
+            walk.at = w_at;
+            walk.more = 1;
+            walk.t = (int)max(w_begin - w_at - kUnitCost, 0ll);
+            walk.t_stop = (int)min(w_end - w_at - kUnitCost, (long long)u.n_tiles);
+        }
+        __syncwarp();
+        look_up();
+#pragma unroll
+        for (; st_in < C::STAGES - 1; ++st_in) bring(st_in);
     }
 
-    // ── the four computing warps ──
     const int r = lane >> 2, c = lane & 3;      // scores: positions 2 r, 2 r + 1 of a block, rows 2 c, 2 c + 1 of eight
     const int g_own = warp % G, tp = warp / G;  // value pass: group, part of the positions; weights: row r, positions 4 c ..
     const T* qp = (const T*)a.q;
@@ -286,9 +325,6 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     float* refs = reinterpret_cast<float*>(sm + C::OFF_M);
     unsigned* flags = reinterpret_cast<unsigned*>(sm + C::OFF_FL);
     float* sums = reinterpret_cast<float*>(sm + C::OFF_L);
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
     for (bool more = true; more && ok;) {
         const int t_first = (int)max(w_begin - w_at - kUnitCost, 0ll), t_stop = (int)min(w_end - w_at - kUnitCost, (long long)u.n_tiles);
         const int rows_all = u.q_len * a.group;
@@ -539,6 +575,10 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             if (lane == 0) flags[buf * 4 + warp] = my_flags;
             compute_barrier();
             if (*(volatile int*)abort_flag) ok = false;
+            if (warp == 0 && ok) {
+                bring(st_in);
+                st_in = st_in + 1 == C::STAGES ? 0 : st_in + 1;
+            }
             // ── values ──
             const uint4 fl = *reinterpret_cast<const uint4*>(flags + buf * 4);
             const unsigned any = fl.x | fl.y | fl.z | fl.w;
@@ -662,8 +702,6 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[nt][x][i] += acc[nt][x][i];
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + stage);
             if (++stage == C::STAGES) {
                 stage = 0;
                 phase ^= 1;
@@ -755,17 +793,24 @@ __global__ void __launch_bounds__(160) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         more = w_at + u.n_tiles + kUnitCost < w_end;
         if (more) next_unit(u, w_at);
     }
+    if (!ok) {  // a copy did not arrive within the limit: reported; the others in flight are waited for (again with a limit)
+        if (lane == 0) atomicExch(err, 1u);
+        for (int k = 1; k < C::STAGES && warp == 0; ++k) mbar_wait(full + (stage + k) % C::STAGES, stage + k >= C::STAGES ? phase ^ 1 : phase);
+        compute_barrier();
+    }
 }
 
 // Joins the partial results of units that were split over CTAs.  grid: x = units (or, where there are more of those, the
 // borders between CTAs: a border splits at most one unit, and a unit is joined by the first border inside it), y = pieces of
-// a unit's rows x elements.  The plan is made before the wait: the batch's arrays were there before the attention kernel.
+// a unit's rows x elements: 256 / parts float4 each, `parts` threads of the CTA sharing an element's partial sums (few parts
+// where a unit has few partial results).  The plan is made before the wait: the batch's arrays were there before the
+// attention kernel.
 template <class C, typename T>
-__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, int row_tiles, int by_border, unsigned int* err) {
+__global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, int row_tiles, int by_border, int parts, unsigned int* err) {
     constexpr int D = C::D, ROWS = C::ROWS;
     __shared__ long long red[8], found[4];
     __shared__ float4 acc_s[256];
-    __shared__ float f_s[256], l_s[8];
+    __shared__ float m_s[256];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto cost = [&](int b, int& rts, int& tiles) -> long long {
         int lo;
@@ -863,68 +908,53 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     const int rows_all = s.q_len * a.group;
     const bool first_odd = total * i0 / n < at;  // CTA i0 began before this unit: its part is in the odd slot
     auto slot_of = [&](int i) { return a.part + (size_t)(2 * i + (i == i0 && first_odd ? 1 : 0)) * ROWS * (D + 2); };
-    // a piece: one row, 64 elements: 16 columns of four x 16 CTAs at a time
-    for (int piece = blockIdx.y; piece < ROWS * (D / 64); piece += gridDim.y) {
-        const int row = piece / (D / 64), d0 = piece % (D / 64) * 64, rr = rt * ROWS + row;
-        if (rr >= rows_all) break;
-        const int col = tid & 15, part = tid >> 4;
-        float m = -INFINITY;
-        for (int i = i0 + tid; i <= i1; i += 256) m = fmaxf(m, slot_of(i)[(size_t)ROWS * D + row]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int per = 256 / parts, e = tid % per, part = tid / per, idx = blockIdx.y * per + e;
+    const int row = idx / (D / 4), col = idx % (D / 4), rr = rt * ROWS + row;
+    const bool live = row < ROWS && rr < rows_all;
+    float m = -INFINITY;
+    if (live)
+        for (int i = i0 + part; i <= i1; i += parts) m = fmaxf(m, slot_of(i)[(size_t)ROWS * D + row]);
+    if (parts > 1) {
+        m_s[tid] = m;
         __syncthreads();
-        if (lane == 0) l_s[warp] = m;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, l_s[i]);
-        const float off = m == -INFINITY ? 0.0f : m;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-        for (int c0 = i0; c0 <= i1; c0 += 256) {
-            __syncthreads();
-            if (c0 + tid <= i1) {
-                const float* sp = slot_of(c0 + tid);
-                const float f = exp2_approx(sp[(size_t)ROWS * D + row] - off);
-                f_s[tid] = f;
-                l = fmaf(sp[(size_t)ROWS * (D + 1) + row], f, l);
-            }
-            __syncthreads();
-            const int here = min(256, i1 - c0 + 1);
-#pragma unroll 8
-            for (int k = part; k < here; k += 16) {
-                const float4 v = reinterpret_cast<const float4*>(slot_of(c0 + k) + (size_t)row * D + d0)[col];
-                const float f = f_s[k];
-                acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-            }
-        }
-        l = warp_sum(l);
-        __syncthreads();
-        acc_s[tid] = acc;
-        if (lane == 0) l_s[warp] = l;
-        __syncthreads();
-        if (part == 0) {
-            l = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) l += l_s[i];
-#pragma unroll
-            for (int p = 1; p < 16; ++p) {
-                const float4 v = acc_s[p * 16 + col];
-                acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-            }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int j = rr / a.group, hq = h * a.group + rr % a.group;
-            float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-            if (a.gate) {
-                const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + d0 + 4 * col;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] /= 1.0f + expf(-ld_act(gp + i));
-            }
-            T* dst = (T*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D + d0 + 4 * col;
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-            else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-        }
+        for (int p = 0; p < parts; ++p) m = fmaxf(m, m_s[p * per + e]);
         __syncthreads();
     }
+    const float off = m == -INFINITY ? 0.0f : m;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+    if (live) {
+#pragma unroll 4
+        for (int i = i0 + part; i <= i1; i += parts) {
+            const float* sp = slot_of(i);
+            const float f = exp2_approx(sp[(size_t)ROWS * D + row] - off);
+            const float4 v = reinterpret_cast<const float4*>(sp + (size_t)row * D)[col];
+            l = fmaf(sp[(size_t)ROWS * (D + 1) + row], f, l);
+            acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+        }
+    }
+    if (parts > 1) {
+        acc_s[tid] = acc;
+        m_s[tid] = l;
+        __syncthreads();
+        for (int p = 1; p < parts && part == 0; ++p) {
+            const float4 v = acc_s[p * per + e];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            l += m_s[p * per + e];
+        }
+    }
+    if (!live || part != 0) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int j = rr / a.group, hq = h * a.group + rr % a.group;
+    float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    if (a.gate) {
+        const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + 4 * col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] /= 1.0f + expf(-ld_act(gp + i));
+    }
+    T* dst = (T*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D + 4 * col;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
 }
 
 // ─── host side ──────────────────────────────────────────────────────────────
@@ -951,14 +981,14 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
     if (occ == 0) {
         MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         int n = 0;
-        MOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 160, C::SMEM));
+        MOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 128, C::SMEM));
         MOE_REQUIRE(n > 0, "kv4_attention: the kernel does not fit this device");
         occ = n;
     }
     unsigned int* err = e->dec_sync + 2;
     if constexpr (!C::SPLIT) {
         MOE_REQUIRE(units < 0x7FFFFFFF, "kv4_attention: too many rows for one call");
-        MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)units), dim3(160), C::SMEM, e->stream, a, err));
+        MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)units), dim3(128), C::SMEM, e->stream, a, err));
         e->launches++;
         return MOE_OK;
     } else {
@@ -970,16 +1000,16 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
         int rc = kv4_reserve(e, (size_t)grid * 2 * C::ROWS * (C::D + 2) * 4);
         if (rc) return rc;
         a.part = e->kv4.work;
-        MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)grid), dim3(160), C::SMEM, e->stream, a, err));
+        MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)grid), dim3(128), C::SMEM, e->stream, a, err));
         e->launches++;
         if (grid == 1) return MOE_OK;  // nothing can be split
         const int64_t all = (int64_t)a.seqs.n_seqs * a.cache.kv_heads * row_tiles;
         const bool by_border = all > grid - 1;
         const int64_t x = by_border ? grid - 1 : all;
-        int64_t y = 4 * e->sm_count / x;  // about four CTAs per SM
-        y = y < 1 ? 1 : y > C::ROWS * (C::D / 64) ? C::ROWS * (C::D / 64) : y;
-        MOE_CUDA(launch_kernel(true, kv4_attn_join_kernel<C, T>, dim3((unsigned)x, (unsigned)y), dim3(256), 0, e->stream, a, (int)grid,
-                               (int)row_tiles, by_border ? 1 : 0, err));
+        int parts = 1;  // about four partial results to a thread
+        while (parts < 64 && all * parts * 8 <= grid) parts *= 2;
+        MOE_CUDA(launch_kernel(true, kv4_attn_join_kernel<C, T>, dim3((unsigned)x, (unsigned)((C::ROWS * (C::D / 4) * parts + 255) / 256)), dim3(256), 0,
+                               e->stream, a, (int)grid, (int)row_tiles, by_border ? 1 : 0, parts, err));
         e->launches++;
         return MOE_OK;
     }
