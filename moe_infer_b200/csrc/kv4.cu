@@ -2,10 +2,12 @@
 //
 // Append: key (rotated on the way) and value rows -> nibbles and (scale, bias) pairs, bit for bit the codec of pack.cu:
 //   scale = (max - min) / 15, nibble = trunc((x - min) * (1 / scale) + 0.5), scale and bias = min stored in bf16.
-// Memory bound (f32, head 256: 2 KB read, 288 B written per position and head).  A sub-warp of D / 8 lanes takes one quad
-// (four positions that share words of V) of one head's keys or values; a lane holds eight elements of the four positions,
-// so a group's minimum and maximum are three shuffles, the rotation partner is a second (cached) load or sits in the same
-// lane, a lane's eight nibbles are one word of K, and the four positions' bytes of V meet in the lane that stores them.
+// Memory bound (f32, head 256: 2 KB read, 288 B written per position and head).  A CTA takes 16 positions of a sequence (one
+// block of the cache) and a head, so what it has to know first (sequence, page) is one chain of loads, and the rows are
+// requested before the page is known.  A sub-warp of D / 8 lanes takes one quad (four positions that share words of V) of
+// the keys or values; a lane holds eight elements of the four positions, so a group's minimum and maximum are three
+// shuffles, the rotation partner is a second (cached) load or sits in the same lane, a lane's eight nibbles are one word of
+// K, and the four positions' bytes of V meet in the lane that stores them.
 #include "kv4.cuh"
 
 namespace moe {
@@ -17,9 +19,9 @@ struct Kv4AppendArgs {
     int64_t kt, kh, vt, vh;
     const float* table;        // null: no rotation
     int64_t n_positions;
-    int rotary, interleaved, quads;
+    int rotary, interleaved;
     const int32_t* rope_positions;
-    int vec_k, vec_v, vec_partner;
+    int vec_k, vec_v, vec_partner, vec_table;
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) {
@@ -33,34 +35,59 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Quantises the eight elements a lane holds of its group of 64 (eight consecutive lanes): nibbles as one word, element i in
-// bits 4 i; the group's pair, equal in the eight lanes.
-__device__ __forceinline__ uint32_t kv4_quant8(const float (&x)[8], uint32_t& pair) {
-    float mn = x[0], mx = x[0];
+// Quantises four positions' groups of 64, eight elements each in the lanes 8 k .. 8 k + 7: nibbles as one word per position,
+// element i in bits 4 i.  Lane 8 k + i (and + 4) does the two divisions of position i and returns its (scale, bias) pair.
+__device__ __forceinline__ uint32_t kv4_quant(const float (&x)[4][8], uint32_t (&word)[4]) {
+    const int lane = threadIdx.x & 31;
+    float mn[4], mx[4];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        mn = min_nan(mn, x[i]);
-        mx = max_nan(mx, x[i]);
+    for (int i = 0; i < 4; ++i) {
+        mn[i] = mx[i] = x[i][0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) {
+            mn[i] = min_nan(mn[i], x[i][k]);
+            mx[i] = max_nan(mx[i], x[i][k]);
+        }
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    if (mx == mn) mx = __fadd_rn(mn, 1.0f);
-    const float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
-    const float inv = __fdiv_rn(1.0f, scale);
-    uint32_t word = 0;
+    for (int o = 1; o < 8; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float t = __fadd_rn(__fmul_rn(__fsub_rn(x[i], mn), inv), 0.5f);
-        word |= min(__float2uint_rz(t), 15u) << (4 * i);
-    }
-    pair = (uint32_t)f32_to_bf16_ref(scale) | (uint32_t)f32_to_bf16_ref(mn) << 16;
+        for (int i = 0; i < 4; ++i) {
+            mn[i] = min_nan(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+            mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+        }
+    const float lo = (lane & 2) ? ((lane & 1) ? mn[3] : mn[2]) : ((lane & 1) ? mn[1] : mn[0]);
+    float hi = (lane & 2) ? ((lane & 1) ? mx[3] : mx[2]) : ((lane & 1) ? mx[1] : mx[0]);
+    if (hi == lo) hi = __fadd_rn(lo, 1.0f);
+    const float scale = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    float inv = __fdiv_rn(1.0f, scale);
+    uint32_t pair = (uint32_t)f32_to_bf16_ref(scale) | (uint32_t)f32_to_bf16_ref(lo) << 16;
     // not finite, or too large for its pair to be: both halves NaN (the attention kernel looks at the scale alone)
-    const bool ok = fabsf(mn) < INFINITY && fabsf(scale) < INFINITY && (pair & 0x7F80u) != 0x7F80u && (pair & 0x7F800000u) != 0x7F800000u;
-    if (!ok) pair = 0x7FC07FC0u;
-    return ok ? word : 0u;
+    if (!(fabsf(lo) < INFINITY && fabsf(scale) < INFINITY && (pair & 0x7F80u) != 0x7F80u && (pair & 0x7F800000u) != 0x7F800000u)) {
+        pair = 0x7FC07FC0u;
+        inv = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = __shfl_sync(0xffffffffu, inv, (lane & 24) + i);
+        word[i] = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float t = __fadd_rn(__fmul_rn(__fsub_rn(x[i][k], mn[i]), f), 0.5f);
+            word[i] = min(__float2uint_rz(t), 15u) * (1u << (4 * k)) + word[i];
+        }
+    }
+    return pair;
+}
+
+// bytes b of four words to word b of four: out[b] = byte b of in[0], in[1], in[2], in[3]
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __byte_perm(in[0], in[1], 0x5140), b = __byte_perm(in[2], in[3], 0x5140);
+    const uint32_t c = __byte_perm(in[0], in[1], 0x7362), d = __byte_perm(in[2], in[3], 0x7362);
+    out[0] = __byte_perm(a, b, 0x5410);
+    out[1] = __byte_perm(a, b, 0x7632);
+    out[2] = __byte_perm(c, d, 0x5410);
+    out[3] = __byte_perm(c, d, 0x7632);
 }
 
 // Byte offset inside a block's K nibbles of the word that holds elements 8 l .. 8 l + 7 of position t.
@@ -72,25 +99,19 @@ __device__ __forceinline__ int kv4_k_offset(int l, int t) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsigned int* err) {
-    constexpr int LPT = D / 8, SUB = 32 / LPT;
-    const int lane = threadIdx.x & 31, sub = lane / LPT, l = lane % LPT;
-    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * SUB + sub;
-    const int per_quad = 2 * a.cache.kv_heads;
-    const int64_t bq = item / per_quad;
-    const int r = (int)(item - bq * per_quad);
-    const bool is_v = r >= a.cache.kv_heads;
-    const int h = is_v ? r - a.cache.kv_heads : r;
-    const int64_t b64 = bq / a.quads;
-    Kv4Seq s{0, 0, 0};
-    if (b64 < a.seqs.n_seqs) s = kv4_seq(a.seqs, (int)b64, err);
-    const int b = (int)b64;
+__global__ void __launch_bounds__(D, 1024 / D) kv4_append_kernel(Kv4AppendArgs a, unsigned int* err) {
+    constexpr int LPT = D / 8;
+    const int l = threadIdx.x % LPT, sub = threadIdx.x / LPT;        // eight sub-warps: four quads of keys, then of values
+    const bool is_v = sub >= 4;
+    const int h = blockIdx.x, b = blockIdx.z;
+    const Kv4Seq s = kv4_seq(a.seqs, b, err);
     const int first = max(s.len - s.q_len, 0);                       // first position this call writes
-    const int q0 = (first & ~3) + 4 * (int)(bq - b64 * a.quads);     // this quad's first position
+    const int p0 = (first & ~15) + 16 * (int)blockIdx.y;             // the CTA's positions
+    if (p0 >= s.len || s.len <= first) return;
+    const int q0 = p0 + 4 * (sub & 3);                               // this quad's first position
     const int row_of = s.row0 + s.q_len - s.len;                     // row = row_of + position
-    uint8_t* blk = nullptr;
-    if (q0 < s.len && s.len > first) blk = kv4_block(a.cache, a.seqs, b, h, q0, kv4_block_bytes(D), err);
-    const int lo = blk ? max(first - q0, 0) : 4, hi = blk ? min(s.len - q0, 4) : 0;
+    const int lo = max(first - q0, 0), hi = min(s.len - q0, 4);
+    uint8_t* const blk = kv4_block(a.cache, a.seqs, b, h, p0, kv4_block_bytes(D), err);
 
     float x[4][8];
 #pragma unroll
@@ -110,11 +131,16 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsign
         const float* cs = a.table + pos * a.rotary;
         const int half = a.rotary >> 1;
         if (a.interleaved) {
+            float ct[4], st[4];
+            if (a.vec_table) {  // rotary a multiple of 8: the lane's four pairs are all there and contiguous
+                *reinterpret_cast<float4*>(ct) = *reinterpret_cast<const float4*>(cs + 4 * l);
+                *reinterpret_cast<float4*>(st) = *reinterpret_cast<const float4*>(cs + half + 4 * l);
+            }
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
                 const int p = (8 * l + k) >> 1;
                 if (8 * l + k >= a.rotary) break;
-                const float c = cs[p], sn = cs[half + p], u = x[i][k], w = x[i][k + 1];
+                const float c = a.vec_table ? ct[k >> 1] : cs[p], sn = a.vec_table ? st[k >> 1] : cs[half + p], u = x[i][k], w = x[i][k + 1];
                 x[i][k] = __fsub_rn(__fmul_rn(u, c), __fmul_rn(w, sn));
                 x[i][k + 1] = __fadd_rn(__fmul_rn(u, sn), __fmul_rn(w, c));
             }
@@ -141,10 +167,9 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsign
             }
         }
     }
-    uint32_t word[4], pair[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) word[i] = kv4_quant8(x[i], pair[i]);
-    if (hi <= lo) return;
+    uint32_t word[4];
+    const uint32_t pair = kv4_quant(x, word);
+    if (!blk || hi <= lo) return;
 
     const int t0 = q0 % kKv4Block;  // 0, 4, 8 or 12
     uint8_t* nib = blk + (is_v ? 9 * D : 0);
@@ -156,13 +181,8 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsign
         // bytes of the four positions, elements (2x, 2x + 1): word x of the lane's 16
         uint8_t* dst = nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16;
         uint32_t w[4];
-#pragma unroll
-        for (int x4 = 0; x4 < 4; ++x4) {
-            w[x4] = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[x4] |= (word[i] >> (8 * x4) & 0xFFu) << (8 * i);
-        }
-        if (lo == 0 && hi == 4) {
+        transpose_bytes(word, w);
+        if (lo <= 0 && hi == 4) {
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
@@ -172,37 +192,22 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendArgs a, unsign
                     if (i >= lo && i < hi) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
         }
     }
-    if ((l & 7) == 0) {
-        uint32_t* pd = reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0;
-        if (lo == 0 && hi == 4) {
-            *reinterpret_cast<uint4*>(pd) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i >= lo && i < hi) pd[i] = pair[i];
-        }
-    }
+    const int mine = l & 7;
+    if (mine >= lo && mine < hi) *(reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0 + mine) = pair;
 }
 
 // The way back: same mapping, values = nibble * scale + bias (the product is exact, so one rounding).
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4View cache, Kv4Seqs seqs, int quads, T* k_out, T* v_out, int vec, unsigned int* err) {
-    constexpr int LPT = D / 8, SUB = 32 / LPT;
-    const int lane = threadIdx.x & 31, sub = lane / LPT, l = lane % LPT;
-    const int64_t item = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * SUB + sub;
-    const int per_quad = 2 * cache.kv_heads;
-    const int64_t bq = item / per_quad;
-    const int r = (int)(item - bq * per_quad);
-    const bool is_v = r >= cache.kv_heads;
-    const int h = is_v ? r - cache.kv_heads : r;
-    const int64_t b64 = bq / quads;
-    if (b64 >= seqs.n_seqs) return;
-    const int b = (int)b64;
+__global__ void __launch_bounds__(D) kv4_gather_kernel(Kv4View cache, Kv4Seqs seqs, T* k_out, T* v_out, int vec, unsigned int* err) {
+    constexpr int LPT = D / 8;
+    const int l = threadIdx.x % LPT, sub = threadIdx.x / LPT;
+    const bool is_v = sub >= 4;
+    const int h = blockIdx.x, b = blockIdx.z;
     const Kv4Seq s = kv4_seq(seqs, b, err);
-    // positions of the rows, those without one (negative) among them: quads are aligned to the position, also below zero
+    // positions of the rows, those without one (negative) among them: aligned to the block, also below zero
     const int first = s.len - s.q_len;
-    const int q0 = (first & ~3) + 4 * (int)(bq - b64 * quads);
-    if (q0 >= s.len) return;
+    const int q0 = (first & ~15) + 16 * (int)blockIdx.y + 4 * (sub & 3);
+    if (q0 >= s.len || q0 + 3 < first) return;
     T* out = is_v ? v_out : k_out;
     const uint8_t* blk = q0 >= 0 ? kv4_block(cache, seqs, b, h, q0, kv4_block_bytes(D), err) : nullptr;
     uint32_t word[4] = {}, pair[4] = {};
@@ -215,10 +220,7 @@ __global__ void __launch_bounds__(128) kv4_gather_kernel(Kv4View cache, Kv4Seqs 
         } else {
             const uint4 q = *reinterpret_cast<const uint4*>(nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16);
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int x4 = 0; x4 < 4; ++x4) word[i] |= (w[x4] >> (8 * i) & 0xFFu) << (8 * x4);
+            transpose_bytes(w, word);
         }
         const uint4 p = *reinterpret_cast<const uint4*>(nib + 8 * D + ((l >> 3) * 16 + t0) * 4);
         pair[0] = p.x; pair[1] = p.y; pair[2] = p.z; pair[3] = p.w;
@@ -255,14 +257,10 @@ Kv4Seqs kv4_seqs(const moe_kv4_batch_t* b) {
     return Kv4Seqs{b->q_start, b->seq_lens, b->page_table, b->n_seqs, b->n_tokens, b->max_pages, b->max_seq_len, b->max_q_len};
 }
 
-// blocks of four warps that cover every (sequence, quad, head, key or value)
-static int64_t quad_blocks(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b, int quads) {
-    const int64_t per_block = 4 * (256 / c->head_dim);
-    return ((int64_t)b->n_seqs * quads * 2 * c->num_kv_heads + per_block - 1) / per_block;
-}
-static int quads_of(const moe_kv4_batch_t* b) {  // q rows touch at most this many aligned quads of positions
-    const int q = b->max_q_len < b->n_tokens ? b->max_q_len : b->n_tokens;
-    return (int)(((int64_t)q + 2) / 4 + 1);
+// q rows touch at most this many blocks of 16 positions
+static int64_t blocks_of(const moe_kv4_batch_t* b) {
+    const int64_t q = b->max_q_len < b->n_tokens ? b->max_q_len : b->n_tokens;
+    return (q + 14) / 16 + 1;
 }
 
 }  // namespace moe
@@ -310,14 +308,14 @@ int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
         a.interleaved = rope->interleaved;
     }
     a.rope_positions = rope_positions_dev;
-    a.quads = quads_of(batch);
     a.vec_k = ((uintptr_t)k_dev & 15) == 0 && (k_token_stride | k_head_stride) % vec == 0;
     a.vec_v = ((uintptr_t)v_dev & 15) == 0 && (v_token_stride | v_head_stride) % vec == 0;
+    a.vec_table = a.rotary % 8 == 0 && ((uintptr_t)a.table & 15) == 0;
     a.vec_partner = a.vec_k && a.rotary % 16 == 0 && ((uintptr_t)a.table & 15) == 0;
-    const int64_t blocks = quad_blocks(cache, batch, a.quads);
-    MOE_REQUIRE(blocks < 0x7FFFFFFF, "kv4_append: too many rows for one call");
+    MOE_REQUIRE(blocks_of(batch) <= 65535 && batch->n_seqs <= 65535, "kv4_append: too many rows or sequences for one call");
     unsigned int* err = e->dec_sync + 2;
-    auto run = [&](auto kernel) { kernel<<<(unsigned)blocks, 128, 0, e->stream>>>(a, err); };
+    const dim3 grid(cache->num_kv_heads, (unsigned)blocks_of(batch), batch->n_seqs);
+    auto run = [&](auto kernel) { kernel<<<grid, cache->head_dim, 0, e->stream>>>(a, err); };
     const bool f32 = dtype == MOE_DT_F32;
     switch (cache->head_dim) {
         case 64: f32 ? run(kv4_append_kernel<float, 64>) : run(kv4_append_kernel<__nv_bfloat16, 64>); break;
@@ -341,14 +339,13 @@ int moe_kv4_gather_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
     MOE_REQUIRE((((uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & amask) == 0, "kv4_gather: misaligned pointer");
     DeviceScope scope(e->device);
     MOE_CUDA(scope.status);
-    const int quads = quads_of(batch);
-    const int64_t blocks = quad_blocks(cache, batch, quads);
-    MOE_REQUIRE(blocks < 0x7FFFFFFF, "kv4_gather: too many rows for one call");
+    MOE_REQUIRE(blocks_of(batch) <= 65535 && batch->n_seqs <= 65535, "kv4_gather: too many rows or sequences for one call");
+    const dim3 grid(cache->num_kv_heads, (unsigned)blocks_of(batch), batch->n_seqs);
     const int vec = (((uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & 15) == 0;
     unsigned int* err = e->dec_sync + 2;
     auto run = [&](auto kernel, auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        kernel<<<(unsigned)blocks, 128, 0, e->stream>>>(kv4_view(cache), kv4_seqs(batch), quads, (T*)k_out_dev, (T*)v_out_dev, vec, err);
+        kernel<<<grid, cache->head_dim, 0, e->stream>>>(kv4_view(cache), kv4_seqs(batch), (T*)k_out_dev, (T*)v_out_dev, vec, err);
     };
     const bool f32 = dtype == MOE_DT_F32;
     float* f = nullptr;

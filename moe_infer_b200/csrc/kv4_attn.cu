@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     constexpr int D = C::D, ROWS = C::ROWS;
     __shared__ long long red[8], found[4];
     __shared__ float4 acc_s[256];
-    __shared__ float m_s[256];
+    __shared__ float m_s[256], l_s[256];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto cost = [&](int b, int& rts, int& tiles) -> long long {
         int lo;
@@ -911,37 +911,44 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     const int per = 256 / parts, e = tid % per, part = tid / per, idx = blockIdx.y * per + e;
     const int row = idx / (D / 4), col = idx % (D / 4), rr = rt * ROWS + row;
     const bool live = row < ROWS && rr < rows_all;
-    float m = -INFINITY;
-    if (live)
-        for (int i = i0 + part; i <= i1; i += parts) m = fmaxf(m, slot_of(i)[(size_t)ROWS * D + row]);
-    if (parts > 1) {
-        m_s[tid] = m;
-        __syncthreads();
-        for (int p = 0; p < parts; ++p) m = fmaxf(m, m_s[p * per + e]);
-        __syncthreads();
-    }
-    const float off = m == -INFINITY ? 0.0f : m;
+    // running reference, sum of weights and sums of values; four partial results requested at a time
+    float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
+    auto add = [&](float m2, float l2, const float4& v) {
+        const float m_new = fmaxf(m, m2), off = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = exp2_approx(m - off), f2 = exp2_approx(m2 - off);
+        l = fmaf(l2, f2, l * f);
+        acc.x = fmaf(v.x, f2, acc.x * f); acc.y = fmaf(v.y, f2, acc.y * f);
+        acc.z = fmaf(v.z, f2, acc.z * f); acc.w = fmaf(v.w, f2, acc.w * f);
+        m = m_new;
+    };
     if (live) {
-#pragma unroll 4
-        for (int i = i0 + part; i <= i1; i += parts) {
-            const float* sp = slot_of(i);
-            const float f = exp2_approx(sp[(size_t)ROWS * D + row] - off);
-            const float4 v = reinterpret_cast<const float4*>(sp + (size_t)row * D)[col];
-            l = fmaf(sp[(size_t)ROWS * (D + 1) + row], f, l);
-            acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+        for (int i = i0 + part; i <= i1; i += 4 * parts) {
+            float m4[4], l4[4];
+            float4 v4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                m4[k] = -INFINITY;
+                l4[k] = 0.0f;
+                v4[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i + k * parts <= i1) {
+                    const float* sp = slot_of(i + k * parts);
+                    m4[k] = sp[(size_t)ROWS * D + row];
+                    l4[k] = sp[(size_t)ROWS * (D + 1) + row];
+                    v4[k] = reinterpret_cast<const float4*>(sp + (size_t)row * D)[col];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add(m4[k], l4[k], v4[k]);
         }
     }
-    if (parts > 1) {
+    for (int p = parts; p > 1; p >>= 1) {  // the threads of an element in pairs
         acc_s[tid] = acc;
-        m_s[tid] = l;
+        m_s[tid] = m;
+        l_s[tid] = l;
         __syncthreads();
-        for (int p = 1; p < parts && part == 0; ++p) {
-            const float4 v = acc_s[p * per + e];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-            l += m_s[p * per + e];
-        }
+        if (part < p / 2) add(m_s[tid + p / 2 * per], l_s[tid + p / 2 * per], acc_s[tid + p / 2 * per]);
+        __syncthreads();
     }
     if (!live || part != 0) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1006,8 +1013,8 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
         const int64_t all = (int64_t)a.seqs.n_seqs * a.cache.kv_heads * row_tiles;
         const bool by_border = all > grid - 1;
         const int64_t x = by_border ? grid - 1 : all;
-        int parts = 1;  // about four partial results to a thread
-        while (parts < 64 && all * parts * 8 <= grid) parts *= 2;
+        int parts = 1;  // two to eight partial results to a thread
+        while (parts < 64 && all * parts * 4 <= grid) parts *= 2;
         MOE_CUDA(launch_kernel(true, kv4_attn_join_kernel<C, T>, dim3((unsigned)x, (unsigned)((C::ROWS * (C::D / 4) * parts + 255) / 256)), dim3(256), 0,
                                e->stream, a, (int)grid, (int)row_tiles, by_border ? 1 : 0, parts, err));
         e->launches++;
