@@ -6,7 +6,7 @@
 // bulk copies.  f16 values of a tile are scaled by a power of two of its own, so any range of values keeps 11 bits.
 //
 // Attention kernel: a CTA owns 128 rows (of the query heads that share a KV head) and walks its positions.  One thread
-// copies, one issues MMAs, four warps hold a row per thread:
+// copies, one issues MMAs, eight warps hold a row per pair of threads (half a tile's positions, then half of O, each):
 //   S = Q K^T (128 x 128, two buffers in tensor memory)  ->  w = exp2(S f - m)  ->  f16 P in shared memory  ->  O += P V
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 (the weights of a row
 // share one reference, so the result does not depend on when).  QK of the next tile runs under the softmax of this one.
@@ -26,9 +26,10 @@ struct PtCfg {
     static constexpr int IMG = D * kPtTile * 2;                    // one f16 image of a tile
     static constexpr int OFF_K = IMG, OFF_V = 2 * IMG, OFF_P = 3 * IMG;
     static constexpr int P_BYTES = kPtTile * kPtTile * 2;
-    static constexpr int OFF_BAR = OFF_P + P_BYTES;
-    // barriers, and room to align the base to 1 KB; never so little that two CTAs would share an SM (tensor memory holds one)
-    static constexpr int SMEM = OFF_BAR + 256 + 1024 > 118 * 1024 ? OFF_BAR + 256 + 1024 : 118 * 1024;
+    static constexpr int OFF_TOP = OFF_P + P_BYTES;                // [2][2][128] f32: maxima of a row's two threads
+    static constexpr int OFF_BAR = OFF_TOP + 2048;
+    // never so little that two CTAs would share an SM (tensor memory holds one)
+    static constexpr int SMEM = OFF_BAR + 128 > 118 * 1024 ? OFF_BAR + 128 : 118 * 1024;
     static constexpr int COL_S = D;                                // tensor memory: O, then two score buffers
     static constexpr int COLS = 512;
 };
@@ -170,10 +171,13 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const float (&v)[3
 }
 
 template <int D>
-__global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_per_seq, const uint8_t* image, const int* meta, unsigned int* err) {
+__global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_per_seq, const uint8_t* image, const int* meta, unsigned int* err) {
     using C = PtCfg<D>;
-    extern __shared__ uint8_t pt_raw[];
-    uint8_t* sm = pt_raw + ((1024u - (smem_u32(pt_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t sm[];  // all of the CTA's shared memory: no static part moves it off its alignment
+    if (smem_u32(sm) & 1023u) {
+        if (threadIdx.x == 0) atomicExch(err, 2u);
+        return;
+    }
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
     uint64_t *k_full = bars, *v_full = bars + 1, *k_free = bars + 2, *pv_done = bars + 3, *s_full = bars + 4 /* 2 */, *p_ready = bars + 6, *q_ready = bars + 7;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
@@ -207,18 +211,18 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
         mbar_init(pv_done, 1);
         mbar_init(s_full, 1);
         mbar_init(s_full + 1, 1);
-        mbar_init(p_ready, 128);
-        mbar_init(q_ready, 128);
+        mbar_init(p_ready, 256);
+        mbar_init(q_ready, 256);
         mbar_fence_init();
     }
-    if (warp == 5) umma::tmem_alloc(tmem_slot, C::COLS);
+    if (warp == 9) umma::tmem_alloc(tmem_slot, C::COLS);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
 
-    if (warp == 4) {
+    if (warp == 8) {
         // ── copies ──
         if ((tid & 31) == 0) {
             auto load = [&](int i, int v) {
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
             }
             if (!ok) atomicExch(err, 1u);
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         // ── MMAs ──
         if ((tid & 31) == 0 && n_tiles > 0) {
             const uint32_t id_qk = make_idesc_f16(128, kPtTile), id_pv = make_idesc_f16(128, D);
@@ -277,12 +281,13 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
             if (!ok) atomicExch(err, 1u);
         }
     } else {
-        // ── a row per thread ──
-        const int row = tid, rr = rt * kPtTile + row;
+        // ── two threads per row: positions 64 half .. 64 half + 63 of a tile, elements half * D / 2 .. of O ──
+        const int row = tid & 127, half = tid >> 7, rr = rt * kPtTile + row;
         const bool valid = rr < rows_all;
         const int j = valid ? rr / a.group : 0, hq = h * a.group + (valid ? rr % a.group : 0);
         const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (int64_t)(s.row0 + j) * a.qt + (int64_t)hq * a.qh;
-        const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 * warp of tensor memory (bits 16-31)
+        const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 * (warp % 4) of tensor memory (bits 16-31)
+        float* tops = reinterpret_cast<float*>(sm + C::OFF_TOP);         // [2 tiles][2 halves][128 rows]
         float f_row;
         {
             const bool vec = (((uintptr_t)a.q & 15) == 0) && ((a.qt | a.qh) & 7) == 0;
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
             const float mag = fabsf(a.scale_log2);
             if (mag == 0.0f) up = 0.0f;
             f_row = (mag == 0.0f ? 1.0f : mag) * pow2f(max(e - 14, -126));
-            for (int c = 0; c < D / 8; ++c) {
+            for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = 0.0f;
@@ -321,42 +326,49 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
             e_k = meta[img0 * kPtMeta];
             e_v = meta[img0 * kPtMeta + 1];
         }
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const int t0 = (t_begin + i) * kPtTile;
+        for (int i = 0; i < n_tiles; ++i) {
+            const int t0 = (t_begin + i) * kPtTile + 64 * half;  // this thread's positions
             const int* mt = meta + (img0 + i) * kPtMeta;
             const int ek = e_k, ev = e_v;
-            const uint32_t nb[4] = {(uint32_t)mt[2], (uint32_t)mt[3], (uint32_t)mt[4], (uint32_t)mt[5]};
+            const uint32_t nb[2] = {(uint32_t)mt[2 + 2 * half], (uint32_t)mt[3 + 2 * half]};
             if (i + 1 < n_tiles) {
                 e_k = mt[kPtMeta];
                 e_v = mt[kPtMeta + 1];
             }
-            ok = mbar_wait(s_full + (i & 1), (i >> 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            ok = mbar_wait(s_full + (i & 1), (i >> 1) & 1) && ok;
             umma::fence_after_sync();
-            float v[4][32];
-            const uint32_t sc = lane_base + C::COL_S + (i & 1) * kPtTile;
+            float v[2][32];
+            const uint32_t sc = lane_base + C::COL_S + (i & 1) * kPtTile + 64 * half;
+            umma::ld_32x32(sc, v[0]);
+            umma::ld_32x32(sc + 32, v[1]);
+            if (t0 + 63 > see_hi || t0 < see_lo) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) umma::ld_32x32(sc + 32 * q, v[q]);
-            if (t0 + kPtTile - 1 > see_hi || t0 < see_lo) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
                         const int t = t0 + 32 * q + k;
                         if (t > see_hi || t < see_lo) v[q][k] = -INFINITY;
                     }
             }
-            float mx[4];
+            float mx[4] = {v[0][0], v[0][1], v[1][0], v[1][1]};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                mx[q] = v[q][0];
-#pragma unroll
-                for (int k = 1; k < 32; ++k) mx[q] = fmaxf(mx[q], v[q][k]);
+            for (int k = 2; k < 32; k += 2) {
+                mx[0] = fmaxf(mx[0], v[0][k]);
+                mx[1] = fmaxf(mx[1], v[0][k + 1]);
+                mx[2] = fmaxf(mx[2], v[1][k]);
+                mx[3] = fmaxf(mx[3], v[1][k + 1]);
             }
             // weights are exp2(S f + e_v - m): the tile's values are held divided by 2^e_v
             const float f = fmaxf(f_row * pow2f(ek), 1.2e-38f);
-            const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, (float)ev);
+            float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, (float)ev);
+            tops[((i & 1) * 2 + half) * 128 + row] = ok ? top : NAN;  // a wait that gave up reaches the row's other thread
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float other = tops[((i & 1) * 2 + (half ^ 1)) * 128 + row];
+            if (__any_sync(0xffffffffu, !ok || other != other)) {
+                ok = false;
+                break;
+            }
+            top = fmaxf(top, other);
             const bool grow = top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY);
             float fix = 1.0f;
             if (grow) {
@@ -364,58 +376,61 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 m_ref = top;
                 l *= fix;
             }
+            const float off = (float)ev - (m_ref == -INFINITY ? 0.0f : m_ref);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[k] = exp2_approx(fmaf(v[c >> 2][(c & 3) * 8 + k], f, off));
+                    sum[k & 3] += x[k];
+                }
+                w[4 * c] = h2_bits(__floats2half2_rn(x[0], x[2]));
+                w[4 * c + 1] = h2_bits(__floats2half2_rn(x[1], x[3]));
+                w[4 * c + 2] = h2_bits(__floats2half2_rn(x[4], x[6]));
+                w[4 * c + 3] = h2_bits(__floats2half2_rn(x[5], x[7]));
+            }
             if (i > 0) {
                 // the product before this one has read its weights, and O may be touched
                 ok = mbar_wait(pv_done, (i - 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
                 if (__any_sync(0xffffffffu, grow)) {
                     umma::fence_after_sync();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
+                    for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
                         float o[32];
                         umma::ld_32x32(lane_base + c, o);
 #pragma unroll
                         for (int k = 0; k < 32; ++k) o[k] *= fix;
                         tmem_st_32x32(lane_base + c, o);
                     }
-                    umma::fence_before_sync();
                 }
             }
-            const float off = (float)ev - (m_ref == -INFINITY ? 0.0f : m_ref);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int c = 0; c < kPtTile / 8; ++c) {
-                float w[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    w[k] = exp2_approx(fmaf(v[c >> 2][(c & 3) * 8 + k], f, off));
-                    sum[k & 3] += w[k];
-                }
-                *reinterpret_cast<uint4*>(sm + C::OFF_P + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) =
-                    make_uint4(h2_bits(__floats2half2_rn(w[0], w[2])), h2_bits(__floats2half2_rn(w[1], w[3])),
-                               h2_bits(__floats2half2_rn(w[4], w[6])), h2_bits(__floats2half2_rn(w[5], w[7])));
-            }
+            for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(sm + C::OFF_P + half * (kPtTile * 128) + umma::sw128_offset(row, c)) =
+                    make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             umma::fence_smem_to_async();
             umma::fence_before_sync();
             mbar_arrive(p_ready);
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(-ev), l);
-            if (nb[0] | nb[1] | nb[2] | nb[3]) {  // values that are NaN: held as 0; rows that see one become NaN
-                for (int t = 0; t < kPtTile; ++t)
+            if (nb[0] | nb[1]) {  // values that are NaN: held as 0; rows that see one become NaN
+                for (int t = 0; t < 64; ++t)
                     if ((nb[t >> 5] >> (t & 31) & 1u) && t0 + t <= see_hi && t0 + t >= see_lo) l = NAN;
             }
         }
-        if (ok && n_tiles > 0) {
-            ok = mbar_wait(pv_done, (n_tiles - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-        }
+        if (ok && n_tiles > 0) ok = mbar_wait(pv_done, (n_tiles - 1) & 1);
         umma::fence_after_sync();
+        tops[half * 128 + row] = l;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        l += tops[(half ^ 1) * 128 + row];
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D;
         const __nv_bfloat16* gp = a.gate ? (const __nv_bfloat16*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh : nullptr;
         const bool gvec = ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             float o[32];
             if (n_tiles > 0) {
                 umma::ld_32x32(lane_base + c, o);
@@ -440,7 +455,7 @@ __global__ void __launch_bounds__(192) kv4_prompt_kernel(AttnArgs a, int tiles_p
     }
     umma::fence_before_sync();
     __syncthreads();
-    if (warp == 5) umma::tmem_dealloc(tmem, C::COLS);
+    if (warp == 9) umma::tmem_dealloc(tmem, C::COLS);
 }
 
 // ─── host side ──────────────────────────────────────────────────────────────
@@ -486,7 +501,7 @@ int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
         kv4_expand_kernel<D><<<dim3(2 * tiles, a.cache.kv_heads, a.seqs.n_seqs), 256, C::IMG, e->stream>>>(a, tiles, img, mt, err);
         e->launches++;
     }
-    kv4_prompt_kernel<D><<<(unsigned)units, 192, C::SMEM, e->stream>>>(a, tiles, img, mt, err);
+    kv4_prompt_kernel<D><<<(unsigned)units, 320, C::SMEM, e->stream>>>(a, tiles, img, mt, err);
     e->launches++;
     MOE_CUDA(cudaGetLastError());
     return MOE_OK;
