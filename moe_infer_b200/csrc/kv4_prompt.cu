@@ -291,13 +291,32 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         float f_row;
         {
             const bool vec = (((uintptr_t)a.q & 15) == 0) && ((a.qt | a.qh) & 7) == 0;
-            float mx = 0.0f;
-            for (int c = 0; c < D / 8; ++c) {
-                float v[8];
-                if (valid) ld_act8(qp + 8 * c, vec, v);
+            // half a row per thread, all of it requested at once
+            uint4 raw[D / 16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) mx = valid ? fmaxf(mx, fabsf(v[k])) : mx;
+            for (int c = 0; c < D / 16; ++c) raw[c] = make_uint4(0, 0, 0, 0);
+            const __nv_bfloat16* src = qp + half * (D / 2);
+            if (valid && vec) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) raw[c] = reinterpret_cast<const uint4*>(src)[c];
+            } else if (valid) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + 8 * c;
+                    raw[c] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+                }
             }
+            float mx = 0.0f;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xFFFF0000u))));
+            }
+            tops[half * 128 + row] = mx;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            mx = fmaxf(mx, tops[(half ^ 1) * 128 + row]);
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // the place is used for the tiles' maxima next
             // scaled by a power of two into [2^14, 2^15); a negative scale turns the queries' sign, a scale of 0 makes them 0
             const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -110), 127);
             float up = pow2f(min(14 - e, 127));
@@ -305,15 +324,19 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             const float mag = fabsf(a.scale_log2);
             if (mag == 0.0f) up = 0.0f;
             f_row = (mag == 0.0f ? 1.0f : mag) * pow2f(max(e - 14, -126));
-            for (int c = half * (D / 16); c < (half + 1) * (D / 16); ++c) {
+#pragma unroll
+            for (int cc = 0; cc < D / 16; ++cc) {
+                const int c = half * (D / 16) + cc;
+                const uint32_t w[4] = {raw[cc].x, raw[cc].y, raw[cc].z, raw[cc].w};
                 float v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-                if (valid) ld_act8(qp + 8 * c, vec, v);
-                uint32_t o[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = h2_bits(__floats2half2_rn(v[k] * up, v[k + 4] * up));
-                *reinterpret_cast<uint4*>(sm + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+                for (int k = 0; k < 4; ++k) {
+                    v[2 * k] = __uint_as_float(w[k] << 16) * up;
+                    v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * up;
+                }
+                *reinterpret_cast<uint4*>(sm + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) =
+                    make_uint4(h2_bits(__floats2half2_rn(v[0], v[4])), h2_bits(__floats2half2_rn(v[1], v[5])), h2_bits(__floats2half2_rn(v[2], v[6])),
+                               h2_bits(__floats2half2_rn(v[3], v[7])));
             }
             umma::fence_smem_to_async();
             mbar_arrive(q_ready);
@@ -431,6 +454,12 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         const bool gvec = ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0;
 #pragma unroll 1
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+            uint4 graw[4];
+            const bool gfast = gp && gvec && valid;
+            if (gfast) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) graw[k] = reinterpret_cast<const uint4*>(gp + c)[k];
+            }
             float o[32];
             if (n_tiles > 0) {
                 umma::ld_32x32(lane_base + c, o);
@@ -440,14 +469,23 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             }
             if (!valid || !ok) continue;
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-                float y[8], g[8];
-                if (gp) ld_act8(gp + c + k, gvec, g);
+            for (int k = 0; k < 32; ++k) o[k] *= inv;
+            if (gfast) {
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    y[x] = o[k + x] * inv;
-                    if (gp) y[x] /= 1.0f + expf(-g[x]);
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t w[4] = {graw[k >> 2].x, graw[k >> 2].y, graw[k >> 2].z, graw[k >> 2].w};
+                    o[2 * k] = __fdividef(o[2 * k], 1.0f + __expf(-__uint_as_float(w[k & 3] << 16)));
+                    o[2 * k + 1] = __fdividef(o[2 * k + 1], 1.0f + __expf(-__uint_as_float(w[k & 3] & 0xFFFF0000u)));
                 }
+            } else if (gp) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] /= 1.0f + expf(-ld_act(gp + c + k));
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+                float y[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) y[x] = o[k + x];
                 st_act8(dst + c + k, true, y);
             }
         }
