@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         for (int i = 0; i < ROWS / 4; ++i) {
             const int rr = u.rt * ROWS + warp + 4 * i;
             const bool valid = rr < rows_all;
-            const int j = valid ? rr / a.group : 0, hq = u.h * a.group + (valid ? rr % a.group : 0);
+            const int j = valid ? over_group(rr, a.by_group) : 0, hq = u.h * a.group + (valid ? rr - j * a.group : 0);
 #pragma unroll
             for (int k = 0; k < D / 32; ++k)  // lane: elements (k * 32 + lane)
                 xq[i][k] = valid ? ld_act(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + k * 32 + lane) : 0.0f;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                 const int row = nt * 8 + 2 * c + e, rr = u.rt * ROWS + row;
                 rf[nt][e] = row_f[row];
                 // rows behind the last are computed unmasked and not written
-                see_hi[nt][e] = rr < rows_all ? pos_base + rr / a.group : 0x7FFFFFFF;
+                see_hi[nt][e] = rr < rows_all ? pos_base + over_group(rr, a.by_group) : 0x7FFFFFFF;
                 see_lo[nt][e] = a.window > 0 && rr < rows_all ? see_hi[nt][e] - a.window + 1 : 0;
                 all_hi = min(all_hi, see_hi[nt][e]);
                 all_lo = max(all_lo, see_lo[nt][e]);
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                             slot[(size_t)ROWS * (D + 1) + row] = l;
                         }
                     } else if (rr < rows_all) {
-                        const int j = rr / a.group, hq = u.h * a.group + rr % a.group;
+                        const int j = over_group(rr, a.by_group), hq = u.h * a.group + rr - j * a.group;
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                         const T* gp = gatep ? gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)hq * a.gh + d0 : nullptr;
 #pragma unroll
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     }
     if (!live || part != 0) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int j = rr / a.group, hq = h * a.group + rr % a.group;
+    const int j = over_group(rr, a.by_group), hq = h * a.group + rr - j * a.group;
     float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     if (a.gate) {
         const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + 4 * col;
@@ -1080,6 +1080,7 @@ extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cac
     a.qt = q_token_stride; a.qh = q_head_stride; a.gt = gate_token_stride; a.gh = gate_head_stride;
     a.heads = num_heads;
     a.group = num_heads / cache->num_kv_heads;
+    a.by_group = make_group_div((uint32_t)a.group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.window = window;
     const bool f32 = dtype == MOE_DT_F32;

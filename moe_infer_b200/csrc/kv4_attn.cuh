@@ -4,6 +4,18 @@
 
 namespace moe {
 
+// Division of a number below 2^31 by a run-time constant without a divide: (umulhi(n, mul) + n) >> shift with
+// shift = ceil(log2 d) and mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund-Montgomery).
+struct GroupDiv {
+    uint32_t mul, shift, d;
+};
+inline GroupDiv make_group_div(uint32_t d) {
+    GroupDiv g{0, 0, d};
+    while ((1ull << g.shift) < d) ++g.shift;
+    g.mul = (uint32_t)((((1ull << g.shift) - d) << 32) / d) + 1u;
+    return g;
+}
+
 struct AttnArgs {
     Kv4View cache;
     Kv4Seqs seqs;
@@ -12,6 +24,7 @@ struct AttnArgs {
     void* out;
     int64_t qt, qh, gt, gh;  // element strides
     int heads, group;        // query heads; query heads per KV head
+    GroupDiv by_group;
     float scale_log2;        // scale * log2(e)
     int window;              // 0: none
     float* part;             // work area of the call
@@ -25,6 +38,7 @@ template <int D>
 int launch_kv4_prompt(moe_engine* e, AttnArgs a);
 
 #ifdef __CUDACC__
+__device__ __forceinline__ int over_group(int n, const GroupDiv& g) { return (int)((__umulhi((uint32_t)n, g.mul) + (uint32_t)n) >> g.shift); }
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // without ftz the compiler adds three instructions for results below 2^-126

@@ -284,71 +284,68 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         // ── two threads per row: positions 64 half .. 64 half + 63 of a tile, elements half * D / 2 .. of O ──
         const int row = tid & 127, half = tid >> 7, rr = rt * kPtTile + row;
         const bool valid = rr < rows_all;
-        const int j = valid ? rr / a.group : 0, hq = h * a.group + (valid ? rr % a.group : 0);
-        const __nv_bfloat16* qp = (const __nv_bfloat16*)a.q + (int64_t)(s.row0 + j) * a.qt + (int64_t)hq * a.qh;
         const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // lanes 32 * (warp % 4) of tensor memory (bits 16-31)
         float* tops = reinterpret_cast<float*>(sm + C::OFF_TOP);         // [2 tiles][2 halves][128 rows]
-        float f_row;
+        // rows whole, 16 bytes a lane: D / 8 lanes to a row, so 256 / D rows to a warp's load, and 16 rows to a warp
+        constexpr int LPR = D / 8, RPL = 32 / LPR, NL = 16 / RPL;
+        const int lane = tid & 31, sub = lane / LPR, lc = lane % LPR;
+        auto row_of = [&](int i) { return warp * 16 + i * RPL + sub; };
+        auto load_rows = [&](const uint16_t* base, int64_t ts, int64_t hs, bool vec, uint4 (&raw)[NL]) {
+            base += (int64_t)s.row0 * ts + (int64_t)(h * a.group) * hs + 8 * lc;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int rw = min(rt * kPtTile + row_of(i), rows_all - 1);  // rows behind the last: a copy, not written
+                const int jj = over_group(rw, a.by_group);
+                const uint16_t* e = base + jj * ts + (rw - jj * a.group) * hs;
+                if (vec) raw[i] = *reinterpret_cast<const uint4*>(e);
+                else raw[i] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+            }
+        };
+        int e_k = 0, e_v = 0;
+        if (n_tiles > 0) {
+            e_k = meta[img0 * kPtMeta];
+            e_v = meta[img0 * kPtMeta + 1];
+        }
         {
             const bool vec = (((uintptr_t)a.q & 15) == 0) && ((a.qt | a.qh) & 7) == 0;
-            // half a row per thread, all of it requested at once
-            uint4 raw[D / 16];
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) raw[c] = make_uint4(0, 0, 0, 0);
-            const __nv_bfloat16* src = qp + half * (D / 2);
-            if (valid && vec) {
-#pragma unroll
-                for (int c = 0; c < D / 16; ++c) raw[c] = reinterpret_cast<const uint4*>(src)[c];
-            } else if (valid) {
-#pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
-                    const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + 8 * c;
-                    raw[c] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-                }
-            }
-            float mx = 0.0f;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xFFFF0000u))));
-            }
-            tops[half * 128 + row] = mx;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            mx = fmaxf(mx, tops[(half ^ 1) * 128 + row]);
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // the place is used for the tiles' maxima next
-            // scaled by a power of two into [2^14, 2^15); a negative scale turns the queries' sign, a scale of 0 makes them 0
-            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -110), 127);
-            float up = pow2f(min(14 - e, 127));
-            if (a.scale_log2 < 0.0f) up = -up;
+            uint4 raw[NL];
+            load_rows((const uint16_t*)a.q, a.qt, a.qh, vec, raw);
             const float mag = fabsf(a.scale_log2);
-            if (mag == 0.0f) up = 0.0f;
-            f_row = (mag == 0.0f ? 1.0f : mag) * pow2f(max(e - 14, -126));
 #pragma unroll
-            for (int cc = 0; cc < D / 16; ++cc) {
-                const int c = half * (D / 16) + cc;
-                const uint32_t w[4] = {raw[cc].x, raw[cc].y, raw[cc].z, raw[cc].w};
+            for (int i = 0; i < NL; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                uint32_t mb = 0;  // the largest magnitude, as bf16 bits
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mb = max(mb, max(w[k] & 0x7FFFu, (w[k] >> 16) & 0x7FFFu));
+#pragma unroll
+                for (int o = 1; o < LPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                // scaled by a power of two into [2^14, 2^15); a negative scale turns the queries' sign, a scale of 0 makes them 0
+                const int e = min(max((int)(mb >> 7) - 127, -110), 127);
+                float up = pow2f(min(14 - e, 127));
+                if (a.scale_log2 < 0.0f) up = -up;
+                if (mag == 0.0f) up = 0.0f;
+                const int rw = row_of(i);
+                if (lc == 0) tops[rw] = (mag == 0.0f ? 1.0f : mag) * pow2f(max(e - 14, -126));
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     v[2 * k] = __uint_as_float(w[k] << 16) * up;
                     v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * up;
                 }
-                *reinterpret_cast<uint4*>(sm + (c >> 3) * (kPtTile * 128) + umma::sw128_offset(row, c & 7)) =
+                *reinterpret_cast<uint4*>(sm + (lc >> 3) * (kPtTile * 128) + umma::sw128_offset(rw, lc & 7)) =
                     make_uint4(h2_bits(__floats2half2_rn(v[0], v[4])), h2_bits(__floats2half2_rn(v[1], v[5])), h2_bits(__floats2half2_rn(v[2], v[6])),
                                h2_bits(__floats2half2_rn(v[3], v[7])));
             }
             umma::fence_smem_to_async();
             mbar_arrive(q_ready);
         }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float f_row = tops[row];
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the place is used for the tiles' maxima next
+        const int j = valid ? over_group(rr, a.by_group) : 0;
         const int see_hi = valid ? pos_base + j : 0x7FFFFFFF;
         const int see_lo = valid && a.window > 0 ? see_hi - a.window + 1 : 0;
         float m_ref = -INFINITY, l = 0.0f;
-        int e_k = 0, e_v = 0;
-        if (n_tiles > 0) {
-            e_k = meta[img0 * kPtMeta];
-            e_v = meta[img0 * kPtMeta + 1];
-        }
         for (int i = 0; i < n_tiles; ++i) {
             const int t0 = (t_begin + i) * kPtTile + 64 * half;  // this thread's positions
             const int* mt = meta + (img0 + i) * kPtMeta;
@@ -443,23 +440,21 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                     if ((nb[t >> 5] >> (t & 31) & 1u) && t0 + t <= see_hi && t0 + t >= see_lo) l = NAN;
             }
         }
+        // the gates of the rows this warp will write, all requested before the last product is waited for
+        uint4 graw[NL];
+        if (a.gate) {
+            load_rows((const uint16_t*)a.gate, a.gt, a.gh, ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0, graw);
+        }
         if (ok && n_tiles > 0) ok = mbar_wait(pv_done, (n_tiles - 1) & 1);
         umma::fence_after_sync();
         tops[half * 128 + row] = l;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         l += tops[(half ^ 1) * 128 + row];
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        __nv_bfloat16* dst = (__nv_bfloat16*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D;
-        const __nv_bfloat16* gp = a.gate ? (const __nv_bfloat16*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh : nullptr;
-        const bool gvec = ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0;
+        // through shared memory (where K and V were: every product has been waited for), so that rows are written whole
+        float* stage = reinterpret_cast<float*>(sm + C::OFF_K);
 #pragma unroll 1
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-            uint4 graw[4];
-            const bool gfast = gp && gvec && valid;
-            if (gfast) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) graw[k] = reinterpret_cast<const uint4*>(gp + c)[k];
-            }
             float o[32];
             if (n_tiles > 0) {
                 umma::ld_32x32(lane_base + c, o);
@@ -467,26 +462,30 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
 #pragma unroll
                 for (int k = 0; k < 32; ++k) o[k] = 0.0f;
             }
-            if (!valid || !ok) continue;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] *= inv;
-            if (gfast) {
+            for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<float4*>(stage + row * D + (((c >> 2) + k) ^ (row & 7)) * 4) =
+                    make_float4(o[4 * k] * inv, o[4 * k + 1] * inv, o[4 * k + 2] * inv, o[4 * k + 3] * inv);
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ok) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const uint32_t w[4] = {graw[k >> 2].x, graw[k >> 2].y, graw[k >> 2].z, graw[k >> 2].w};
-                    o[2 * k] = __fdividef(o[2 * k], 1.0f + __expf(-__uint_as_float(w[k & 3] << 16)));
-                    o[2 * k + 1] = __fdividef(o[2 * k + 1], 1.0f + __expf(-__uint_as_float(w[k & 3] & 0xFFFF0000u)));
+            for (int i = 0; i < NL; ++i) {
+                const int rw = row_of(i), rr2 = rt * kPtTile + rw;
+                if (rr2 >= rows_all) continue;
+                const int jj = over_group(rr2, a.by_group);
+                const float4 y0 = *reinterpret_cast<const float4*>(stage + rw * D + ((2 * lc) ^ (rw & 7)) * 4);
+                const float4 y1 = *reinterpret_cast<const float4*>(stage + rw * D + ((2 * lc + 1) ^ (rw & 7)) * 4);
+                float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+                if (a.gate) {
+                    const uint32_t w[4] = {graw[i].x, graw[i].y, graw[i].z, graw[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        y[2 * k] = __fdividef(y[2 * k], 1.0f + __expf(-__uint_as_float(w[k] << 16)));
+                        y[2 * k + 1] = __fdividef(y[2 * k + 1], 1.0f + __expf(-__uint_as_float(w[k] & 0xFFFF0000u)));
+                    }
                 }
-            } else if (gp) {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] /= 1.0f + expf(-ld_act(gp + c + k));
-            }
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-                float y[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) y[x] = o[k + x];
-                st_act8(dst + c + k, true, y);
+                st_act8((__nv_bfloat16*)a.out + ((int64_t)(s.row0 + jj) * a.heads + h * a.group + rr2 - jj * a.group) * D + 8 * lc, true, y);
             }
         }
         if (!ok && tid == 0) atomicExch(err, 1u);
