@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     // The first warp also brings the tiles in, STAGES - 1 ahead: a tile's place is free once all warps have met at the barrier
     // of the tile after it.  Its walk over the CTA's tiles lies in shared memory; the pages of the next tile to copy are
     // looked up one tile before, so that the table's latency is not waited for.
-    int nx_page = -1, nx_block = 0;  // lane: page and block of its 16 positions in that tile; -1: none
+    int nx_page = 0, nx_block = -1;  // lane: page and block of its 16 positions in that tile; block -1: none
     auto look_up = [&]() {           // advances to the next tile (walk.t of walk.n) and looks its pages up
         while (walk.more && walk.t >= walk.t_stop) {
             __syncwarp();
@@ -267,20 +267,20 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             }
             __syncwarp();
         }
-        nx_page = -1;
+        nx_block = -1;
         if (walk.more && lane < NB) {
             const int pos = walk.n.t_lo + walk.t * TILE + lane * kKv4Block;
             if (pos < walk.n.len) {
                 const int pg = pos / a.cache.page_size;
                 nx_block = (pos - pg * a.cache.page_size) / kKv4Block;
-                nx_page = pg < a.seqs.max_pages ? a.seqs.page_table[(size_t)walk.n.b * a.seqs.max_pages + pg] : -2;
-                if (nx_page == -1) nx_page = -2;
+                nx_page = -1;
+                if (pg < a.seqs.max_pages) nx_page = a.seqs.page_table[(size_t)walk.n.b * a.seqs.max_pages + pg];  // used in bring()
             }
         }
     };
     auto bring = [&](int st) {
         if (!walk.more) return;
-        bool copy = nx_page != -1;
+        bool copy = nx_block >= 0;
         if (copy && (nx_page < 0 || nx_page >= a.cache.num_pages)) {
             atomicExch(err, kErrKv4Page);
             copy = false;
@@ -332,44 +332,54 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
 
         // queries of the unit as MMA operands: a warp takes a row at a time; scaled by a power of two so that the largest
         // element lies in [2^14, 2^15)
-        float xq[ROWS / 4][D / 32];  // all of a warp's rows are requested before the first is worked on
+        // a lane takes eight elements of a row, D / 8 lanes a row; all of a warp's rows are requested before the first is used
+        constexpr int LPR = D / 8, RPL = 32 / LPR, NL = ROWS / 4 / RPL > 0 ? ROWS / 4 / RPL : 1;
+        const int sub = lane / LPR, lc = lane % LPR;
+        if (warp * NL * RPL < ROWS) {  // fewer rows than the four warps' lanes can take: the first warps do it
+            float xq[NL][8];
 #pragma unroll
-        for (int i = 0; i < ROWS / 4; ++i) {
-            const int rr = u.rt * ROWS + warp + 4 * i;
-            const bool valid = rr < rows_all;
-            const int j = valid ? over_group(rr, a.by_group) : 0, hq = u.h * a.group + (valid ? rr - j * a.group : 0);
+            for (int i = 0; i < NL; ++i) {
+                const int rr = u.rt * ROWS + (warp * NL + i) * RPL + sub;
+                const bool valid = rr < rows_all;
+                const int j = valid ? over_group(rr, a.by_group) : 0, hq = u.h * a.group + (valid ? rr - j * a.group : 0);
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k)  // lane: elements (k * 32 + lane)
-                xq[i][k] = valid ? ld_act(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + k * 32 + lane) : 0.0f;
-        }
+                for (int k = 0; k < 8; ++k) xq[i][k] = 0.0f;
+                if (valid) ld_act8(qp + (int64_t)(u.row0 + j) * a.qt + (int64_t)hq * a.qh + 8 * lc, a.vec_q, xq[i]);
+            }
 #pragma unroll
-        for (int ri = 0; ri < ROWS / 4; ++ri) {
-            const int row = warp + 4 * ri;
-            float (&x)[D / 32] = xq[ri];
-            float mx = 0.0f;
+            for (int i = 0; i < NL; ++i) {
+                const int row = (warp * NL + i) * RPL + sub;
+                float (&x)[8] = xq[i];
+                float mx = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) mx = fmaxf(mx, fabsf(x[i]));
-            mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-            const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -110);  // mx in [2^e, 2^(e + 1))
-            const float up = pow2f(min(14 - e, 127));
-            if (lane == 0) row_f[row] = a.scale_log2 * pow2f(max(e - 14, -126));
+                for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(x[k]));
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
+                for (int k = 1; k < LPR; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+                const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -110);  // mx in [2^e, 2^(e + 1))
+                const float up = pow2f(min(14 - e, 127));
+                // elements (0, 4), (1, 5) of the eight are a step's operand, (2, 6), (3, 7) the next one's
+                uint32_t hi[4], lo[4];
                 float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float v = x[2 * g + i] * up;
-                    const __half hi = __float2half_rn(v);
-                    sum += C::F32 ? v : __half2float(hi);
-                    // element d of the group -> (step, register, half) of the operand
-                    const int d = i * 32 + lane, cc = d >> 4, jj = (d >> 3) & 1, k8 = d & 7;
-                    const int ks = g * 4 + jj * 2 + ((k8 >> 1) & 1);
-                    uint8_t* dst = sm + C::OFF_Q + ((ks * NT + (row >> 3)) * 32 + (row & 7) * 4 + cc) * C::QW + (k8 & 1) * 4 + (k8 >> 2) * 2;
-                    *reinterpret_cast<__half*>(dst) = hi;
-                    if (C::F32) *reinterpret_cast<__half*>(dst + 8) = __float2half_rn(v - __half2float(hi));
+                for (int k = 0; k < 4; ++k) {
+                    const float v0 = x[k] * up, v1 = x[k + 4] * up;
+                    const __half2 h = __floats2half2_rn(v0, v1);
+                    const float2 f = __half22float2(h);
+                    hi[k] = h2_bits(h);
+                    lo[k] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
+                    sum += C::F32 ? v0 + v1 : f.x + f.y;
                 }
-                sum = warp_sum(sum);
-                if (lane == 0) q_sum[g * ROWS + row] = sum;
+#pragma unroll
+                for (int k = 1; k < 8; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);  // over the group of 64
+                const int g = lc >> 3, cc = (lc >> 1) & 3, jj = lc & 1;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    uint8_t* dst = sm + C::OFF_Q + (((g * 4 + jj * 2 + v) * NT + (row >> 3)) * 32 + (row & 7) * 4 + cc) * C::QW;
+                    if constexpr (C::F32) *reinterpret_cast<uint4*>(dst) = make_uint4(hi[2 * v], hi[2 * v + 1], lo[2 * v], lo[2 * v + 1]);
+                    else *reinterpret_cast<uint2*>(dst) = make_uint2(hi[2 * v], hi[2 * v + 1]);
+                }
+                if ((lc & 7) == 0) q_sum[g * ROWS + row] = sum;
+                if (lc == 0) row_f[row] = a.scale_log2 * pow2f(max(e - 14, -126));
             }
         }
         compute_barrier();
@@ -753,10 +763,22 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         }
         if (tp == 0) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                // the gates of both rows are requested before either is used
+                int64_t at_out[2];
+                bool live[2];
+                float gt[2][8];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int row = nt * 8 + 2 * c + e, rr = u.rt * ROWS + row;
+                    const int rr = u.rt * ROWS + nt * 8 + 2 * c + e;
+                    live[e] = rr < rows_all;
+                    const int j = live[e] ? over_group(rr, a.by_group) : 0, hq = u.h * a.group + (live[e] ? rr - j * a.group : 0);
+                    at_out[e] = ((int64_t)(u.row0 + j) * a.heads + hq) * D + d0;
+                    if (gatep && !slot && live[e]) ld_act8(gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)hq * a.gh + d0, a.vec_gate, gt[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = nt * 8 + 2 * c + e;
                     float y[8];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -776,18 +798,17 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                             slot[(size_t)ROWS * D + row] = ref[nt][e];
                             slot[(size_t)ROWS * (D + 1) + row] = l;
                         }
-                    } else if (rr < rows_all) {
-                        const int j = over_group(rr, a.by_group), hq = u.h * a.group + rr - j * a.group;
+                    } else if (live[e]) {
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                        const T* gp = gatep ? gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)hq * a.gh + d0 : nullptr;
 #pragma unroll
                         for (int n = 0; n < 8; ++n) {
                             y[n] *= inv;
-                            if (gp) y[n] /= 1.0f + expf(-ld_act(gp + n));
+                            if (gatep) y[n] = gated(y[n], gt[e][n]);
                         }
-                        st_act8(outp + ((int64_t)(u.row0 + j) * a.heads + hq) * D + d0, true, y);
+                        st_act8(outp + at_out[e], true, y);
                     }
                 }
+            }
         }
         compute_barrier();  // the weights' place and the row tables are free again
         more = w_at + u.n_tiles + kUnitCost < w_end;
@@ -1083,6 +1104,9 @@ extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cac
     a.by_group = make_group_div((uint32_t)a.group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.window = window;
+    const int vec = dtype == MOE_DT_F32 ? 4 : 8;
+    a.vec_q = ((uintptr_t)q_dev & 15) == 0 && (q_token_stride | q_head_stride) % vec == 0;
+    a.vec_gate = ((uintptr_t)gate_dev & 15) == 0 && (gate_token_stride | gate_head_stride) % vec == 0;
     const bool f32 = dtype == MOE_DT_F32;
     switch (cache->head_dim) {
         case 64: return f32 ? launch_attn<64, float>(e, a) : launch_attn<64, __nv_bfloat16>(e, a);

@@ -23,6 +23,7 @@ struct AttnArgs {
     const void* gate;        // null: none
     void* out;
     int64_t qt, qh, gt, gh;  // element strides
+    int vec_q, vec_gate;     // rows readable 16 bytes at a time
     int heads, group;        // query heads; query heads per KV head
     GroupDiv by_group;
     float scale_log2;        // scale * log2(e)
@@ -44,6 +45,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // without ftz the compiler adds three instructions for results below 2^-126
     return r;
 }
+// y * sigmoid(g); the quotient is within two roundings, and 0 where 1 + exp(-g) passes 2^126
+__device__ __forceinline__ float gated(float y, float g) { return __fdividef(y, 1.0f + __expf(-g)); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 // (a & m) | c as one instruction (written out: with two constants the compiler makes two of it)

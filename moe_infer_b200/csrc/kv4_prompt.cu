@@ -307,9 +307,8 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             e_v = meta[img0 * kPtMeta + 1];
         }
         {
-            const bool vec = (((uintptr_t)a.q & 15) == 0) && ((a.qt | a.qh) & 7) == 0;
             uint4 raw[NL];
-            load_rows((const uint16_t*)a.q, a.qt, a.qh, vec, raw);
+            load_rows((const uint16_t*)a.q, a.qt, a.qh, a.vec_q, raw);
             const float mag = fabsf(a.scale_log2);
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         // the gates of the rows this warp will write, all requested before the last product is waited for
         uint4 graw[NL];
         if (a.gate) {
-            load_rows((const uint16_t*)a.gate, a.gt, a.gh, ((uintptr_t)a.gate & 15) == 0 && ((a.gt | a.gh) & 7) == 0, graw);
+            load_rows((const uint16_t*)a.gate, a.gt, a.gh, a.vec_gate, graw);
         }
         if (ok && n_tiles > 0) ok = mbar_wait(pv_done, (n_tiles - 1) & 1);
         umma::fence_after_sync();
@@ -481,8 +480,8 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                     const uint32_t w[4] = {graw[i].x, graw[i].y, graw[i].z, graw[i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        y[2 * k] = __fdividef(y[2 * k], 1.0f + __expf(-__uint_as_float(w[k] << 16)));
-                        y[2 * k + 1] = __fdividef(y[2 * k + 1], 1.0f + __expf(-__uint_as_float(w[k] & 0xFFFF0000u)));
+                        y[2 * k] = gated(y[2 * k], __uint_as_float(w[k] << 16));
+                        y[2 * k + 1] = gated(y[2 * k + 1], __uint_as_float(w[k] & 0xFFFF0000u));
                     }
                 }
                 st_act8((__nv_bfloat16*)a.out + ((int64_t)(s.row0 + jj) * a.heads + h * a.group + rr2 - jj * a.group) * D + 8 * lc, true, y);
