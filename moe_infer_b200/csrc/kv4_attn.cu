@@ -43,7 +43,7 @@ struct AttnCfg {
     static constexpr int PB = NB / TP;             // blocks a warp takes in the value pass
     static constexpr int BLK = kv4_block_bytes(D);
     static constexpr int STAGE = NB * BLK;
-    static constexpr int STAGES = NT == 1 ? 2 : 3;
+    static constexpr int STAGES = 2;
     static constexpr int KS = D / 16;              // MMA steps over a head
     static constexpr int QW = F32 ? 16 : 8;        // bytes of a lane's query operand per step
     static constexpr int PS = 20;                  // floats from one row's weights of a block to the next (no bank conflicts)
@@ -73,12 +73,6 @@ struct AttnUnit {
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (lengths 100 to 16,000: 107 us without, @@ us with).
 constexpr int kUnitCost = 3;
-
-struct AttnWalk {
-    AttnUnit n;
-    long long at;
-    int t, t_stop, more;
-};
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
 template <class C>
@@ -172,7 +166,6 @@ template <class C, typename T>
 __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2 ? 168 : 255) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long red[8];
-    __shared__ AttnWalk walk;
     constexpr int D = C::D, G = C::G, NT = C::NT, ROWS = C::ROWS, NB = C::NB, TILE = C::TILE, TB = C::TB, PB = C::PB, PS = C::PS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
@@ -246,73 +239,58 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         attn_seq_tiles<C>(a, s, rts, n.t_lo, n.n_tiles);
     };
 
-    // The first warp also brings the tiles in, STAGES - 1 ahead: a tile's place is free once all warps have met at the barrier
-    // of the tile after it.  Its walk over the CTA's tiles lies in shared memory; the pages of the next tile to copy are
-    // looked up one tile before, so that the table's latency is not waited for.
-    int nx_page = 0, nx_block = -1;  // lane: page and block of its 16 positions in that tile; block -1: none
-    auto look_up = [&]() {           // advances to the next tile (walk.t of walk.n) and looks its pages up
-        while (walk.more && walk.t >= walk.t_stop) {
-            __syncwarp();
-            if (lane == 0) {
-                AttnUnit n = walk.n;
-                long long at = walk.at;
-                walk.more = at + n.n_tiles + kUnitCost < w_end;
-                if (walk.more) {
-                    next_unit(n, at);
-                    walk.n = n;
-                    walk.at = at;
-                    walk.t = 0;
-                    walk.t_stop = (int)min(w_end - at - kUnitCost, (long long)n.n_tiles);
-                }
-            }
-            __syncwarp();
-        }
+    // The first warp also brings the tiles in, one ahead: a tile's place is free once all warps have met at the barrier of the
+    // tile after it.  Blocks that lie in one page are one copy (a.run of them: a power of two that divides a page's blocks and
+    // a tile's).  The pages are looked up another tile before, so that the table's latency is not waited for.
+    int nx_page = 0, nx_block = -1;  // lane: page and first block of its run in the tile to copy next; block -1: none
+    auto look_up = [&](const AttnUnit& n, int t) {
         nx_block = -1;
-        if (walk.more && lane < NB) {
-            const int pos = walk.n.t_lo + walk.t * TILE + lane * kKv4Block;
-            if (pos < walk.n.len) {
-                const int pg = pos / a.cache.page_size;
-                nx_block = (pos - pg * a.cache.page_size) / kKv4Block;
-                nx_page = -1;
-                if (pg < a.seqs.max_pages) nx_page = a.seqs.page_table[(size_t)walk.n.b * a.seqs.max_pages + pg];  // used in bring()
-            }
+        const int pos = n.t_lo + t * TILE + lane * a.run * kKv4Block;
+        if (lane * a.run < NB && pos < n.len) {
+            const int pg = pos / a.cache.page_size;
+            nx_block = (pos - pg * a.cache.page_size) / kKv4Block;
+            nx_page = -1;
+            if (pg < a.seqs.max_pages) nx_page = a.seqs.page_table[(size_t)n.b * a.seqs.max_pages + pg];
         }
     };
-    auto bring = [&](int st) {
-        if (!walk.more) return;
+    auto copy_in = [&](int h, int st) {
         bool copy = nx_block >= 0;
         if (copy && (nx_page < 0 || nx_page >= a.cache.num_pages)) {
             atomicExch(err, kErrKv4Page);
             copy = false;
         }
         const unsigned have = __ballot_sync(0xffffffffu, copy);
-        if (lane == 0) mbar_expect_tx(full + st, __popc(have) * C::BLK);
+        if (lane == 0) mbar_expect_tx(full + st, __popc(have) * a.run * C::BLK);
         __syncwarp();
-        if (copy) {
-            const int blocks = a.cache.page_size / kKv4Block;
-            bulk_g2s(sm + st * C::STAGE + lane * C::BLK,
-                     a.cache.pages + (((size_t)nx_page * a.cache.kv_heads + walk.n.h) * blocks + nx_block) * C::BLK, C::BLK, full + st);
-        }
-        __syncwarp();
-        if (lane == 0) ++walk.t;
-        __syncwarp();
-        look_up();
+        if (copy)
+            bulk_g2s(sm + st * C::STAGE + lane * a.run * C::BLK,
+                     a.cache.pages + (((size_t)nx_page * a.cache.kv_heads + h) * (a.cache.page_size / kKv4Block) + nx_block) * C::BLK,
+                     a.run * C::BLK, full + st);
     };
-    int stage = 0, st_in = 0;
+    auto first_of = [&](long long at) { return (int)max(w_begin - at - kUnitCost, 0ll); };
+    auto stop_of = [&](const AttnUnit& n, long long at) { return (int)min(w_end - at - kUnitCost, (long long)n.n_tiles); };
+    // the first tile of the units behind (n, at), if there is one
+    auto bring_next_unit = [&](AttnUnit n, long long at, int st) {
+        while (at + n.n_tiles + kUnitCost < w_end) {
+            next_unit(n, at);
+            if (stop_of(n, at) > 0) {
+                look_up(n, 0);
+                copy_in(n.h, st);
+                return;
+            }
+        }
+    };
+    int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     if (warp == 0) {
-        if (lane == 0) {
-            walk.n = u;
-            walk.at = w_at;
-            walk.more = 1;
-            walk.t = (int)max(w_begin - w_at - kUnitCost, 0ll);
-            walk.t_stop = (int)min(w_end - w_at - kUnitCost, (long long)u.n_tiles);
+        const int t = first_of(w_at);
+        if (t < stop_of(u, w_at)) {
+            look_up(u, t);
+            copy_in(u.h, 0);
+        } else {
+            bring_next_unit(u, w_at, 0);
         }
-        __syncwarp();
-        look_up();
-#pragma unroll
-        for (; st_in < C::STAGES - 1; ++st_in) bring(st_in);
     }
 
     const int r = lane >> 2, c = lane & 3;      // scores: positions 2 r, 2 r + 1 of a block, rows 2 c, 2 c + 1 of eight
@@ -326,7 +304,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     unsigned* flags = reinterpret_cast<unsigned*>(sm + C::OFF_FL);
     float* sums = reinterpret_cast<float*>(sm + C::OFF_L);
     for (bool more = true; more && ok;) {
-        const int t_first = (int)max(w_begin - w_at - kUnitCost, 0ll), t_stop = (int)min(w_end - w_at - kUnitCost, (long long)u.n_tiles);
+        const int t_first = first_of(w_at), t_stop = stop_of(u, w_at);
+        if (warp == 0 && t_first + 1 < t_stop) look_up(u, t_first + 1);
         const int rows_all = u.q_len * a.group;
         const int pos_base = u.len - u.q_len;
 
@@ -586,8 +565,12 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             compute_barrier();
             if (*(volatile int*)abort_flag) ok = false;
             if (warp == 0 && ok) {
-                bring(st_in);
-                st_in = st_in + 1 == C::STAGES ? 0 : st_in + 1;
+                if (ti + 1 < t_stop) {
+                    copy_in(u.h, stage ^ 1);
+                    if (ti + 2 < t_stop) look_up(u, ti + 2);
+                } else {
+                    bring_next_unit(u, w_at, stage ^ 1);
+                }
             }
             // ── values ──
             const uint4 fl = *reinterpret_cast<const uint4*>(flags + buf * 4);
@@ -712,10 +695,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[nt][x][i] += acc[nt][x][i];
             }
-            if (++stage == C::STAGES) {
-                stage = 0;
-                phase ^= 1;
-            }
+            phase ^= stage;
+            stage ^= 1;
             if (!ok) break;
         }
         if (!ok) break;
@@ -742,12 +723,24 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                 o[nt][x][3] += b1;
             }
         }
-        compute_barrier();
         const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles + kUnitCost <= w_end;
+        const int d0 = 64 * g_own + 8 * r;
+        // the gates of all of this lane's rows are requested before the first is used
+        float gt[NT][2][8];
+        if (gatep && tp == 0 && (!C::SPLIT || whole_unit)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int rr = min(u.rt * ROWS + nt * 8 + 2 * c + e, rows_all - 1);
+                    const int j = over_group(rr, a.by_group);
+                    ld_act8(gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)(u.h * a.group + rr - j * a.group) * a.gh + d0, a.vec_gate, gt[nt][e]);
+                }
+        }
+        compute_barrier();
         float* slot = nullptr;
         if (C::SPLIT && !whole_unit) slot = a.part + (size_t)(2 * blockIdx.x + (w_at <= w_begin ? 0 : 1)) * ROWS * (D + 2);
         float* red_o = reinterpret_cast<float*>(sm + C::OFF_P);
-        const int d0 = 64 * g_own + 8 * r;
         if (C::TP > 1) {
             if (tp > 0) {
 #pragma unroll
@@ -764,18 +757,6 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         if (tp == 0) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                // the gates of both rows are requested before either is used
-                int64_t at_out[2];
-                bool live[2];
-                float gt[2][8];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int rr = u.rt * ROWS + nt * 8 + 2 * c + e;
-                    live[e] = rr < rows_all;
-                    const int j = live[e] ? over_group(rr, a.by_group) : 0, hq = u.h * a.group + (live[e] ? rr - j * a.group : 0);
-                    at_out[e] = ((int64_t)(u.row0 + j) * a.heads + hq) * D + d0;
-                    if (gatep && !slot && live[e]) ld_act8(gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)hq * a.gh + d0, a.vec_gate, gt[e]);
-                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int row = nt * 8 + 2 * c + e;
@@ -798,14 +779,15 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
                             slot[(size_t)ROWS * D + row] = ref[nt][e];
                             slot[(size_t)ROWS * (D + 1) + row] = l;
                         }
-                    } else if (live[e]) {
+                    } else if (u.rt * ROWS + row < rows_all) {
+                        const int rr = u.rt * ROWS + row, j = over_group(rr, a.by_group);
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
                         for (int n = 0; n < 8; ++n) {
                             y[n] *= inv;
-                            if (gatep) y[n] = gated(y[n], gt[e][n]);
+                            if (gatep) y[n] = gated(y[n], gt[nt][e][n]);
                         }
-                        st_act8(outp + at_out[e], true, y);
+                        st_act8(outp + ((int64_t)(u.row0 + j) * a.heads + u.h * a.group + rr - j * a.group) * D + d0, true, y);
                     }
                 }
             }
@@ -816,7 +798,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
     }
     if (!ok) {  // a copy did not arrive within the limit: reported; the others in flight are waited for (again with a limit)
         if (lane == 0) atomicExch(err, 1u);
-        for (int k = 1; k < C::STAGES && warp == 0; ++k) mbar_wait(full + (stage + k) % C::STAGES, stage + k >= C::STAGES ? phase ^ 1 : phase);
+        if (warp == 0) mbar_wait(full + (stage ^ 1), stage ? phase ^ 1 : phase);
         compute_barrier();
     }
 }
@@ -1004,6 +986,8 @@ int kv4_reserve(moe_engine* e, size_t bytes) {
 
 template <class C, typename T>
 static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
+    a.run = 1;
+    while (a.run < C::NB && a.cache.page_size / kKv4Block % (2 * a.run) == 0) a.run *= 2;
     auto* kernel = kv4_attn_kernel<C, T>;
     int& occ = e->kv4.occupancy[variant];
     if (occ == 0) {

@@ -28,6 +28,7 @@ struct AttnArgs {
     GroupDiv by_group;
     float scale_log2;        // scale * log2(e)
     int window;              // 0: none
+    int run;                 // blocks of a tile that one copy brings (they lie in one page)
     float* part;             // work area of the call
 };
 
