@@ -62,6 +62,11 @@ inline bool rows_disjoint(int64_t na, int64_t sa, int64_t nb, int64_t sb, int64_
     return a_outer || b_outer;
 }
 
+inline bool ranges_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 // One 4-bit tensor on the device: u32 words, bf16 scales, bf16 biases.
 struct Q4Dev {
     const uint32_t* w = nullptr;

@@ -282,7 +282,6 @@ int moe_kv4_page_bytes(int32_t page_size, int32_t num_kv_heads, int32_t head_dim
 int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, const void* k_dev,
                        int64_t k_token_stride, int64_t k_head_stride, const void* v_dev, int64_t v_token_stride,
                        int64_t v_head_stride, int32_t dtype, const moe_rope_t* rope, const int32_t* rope_positions_dev) {
-    MOE_REQUIRE(e, "kv4_append: null engine");
     int rc = check_kv4(cache, batch);
     if (rc) return rc;
     MOE_REQUIRE(dtype == MOE_DT_F32 || dtype == MOE_DT_BF16, "kv4_append: keys and values are f32 or bf16 (got dtype %d)", dtype);
@@ -293,6 +292,7 @@ int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
     const uintptr_t amask = dtype == MOE_DT_F32 ? 3 : 1;
     MOE_REQUIRE((((uintptr_t)k_dev | (uintptr_t)v_dev) & amask) == 0, "kv4_append: misaligned pointer");
     MOE_REQUIRE(k_token_stride >= 0 && k_head_stride >= 0 && v_token_stride >= 0 && v_head_stride >= 0, "kv4_append: negative stride");
+    MOE_REQUIRE(e, "kv4_append: null engine");
     DeviceScope scope(e->device);
     MOE_CUDA(scope.status);
     const int vec = dtype == MOE_DT_F32 ? 4 : 8;
@@ -329,7 +329,6 @@ int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
 
 int moe_kv4_gather_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, void* k_out_dev, void* v_out_dev,
                        int32_t dtype) {
-    MOE_REQUIRE(e, "kv4_gather: null engine");
     int rc = check_kv4(cache, batch);
     if (rc) return rc;
     MOE_REQUIRE(dtype == MOE_DT_F32 || dtype == MOE_DT_BF16, "kv4_gather: outputs are f32 or bf16 (got dtype %d)", dtype);
@@ -337,6 +336,10 @@ int moe_kv4_gather_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
     MOE_REQUIRE(k_out_dev && v_out_dev, "kv4_gather: null argument");
     const uintptr_t amask = dtype == MOE_DT_F32 ? 3 : 1;
     MOE_REQUIRE((((uintptr_t)k_out_dev | (uintptr_t)v_out_dev) & amask) == 0, "kv4_gather: misaligned pointer");
+    MOE_REQUIRE(k_out_dev != v_out_dev && !ranges_overlap(k_out_dev, (int64_t)batch->n_tokens * cache->num_kv_heads * cache->head_dim * (dtype == MOE_DT_F32 ? 4 : 2), v_out_dev,
+                                                          (int64_t)batch->n_tokens * cache->num_kv_heads * cache->head_dim * (dtype == MOE_DT_F32 ? 4 : 2)),
+                "kv4_gather: the outputs overlap");
+    MOE_REQUIRE(e, "kv4_gather: null engine");
     DeviceScope scope(e->device);
     MOE_CUDA(scope.status);
     MOE_REQUIRE(blocks_of(batch) <= 65535 && batch->n_seqs <= 65535, "kv4_gather: too many rows or sequences for one call");

@@ -95,7 +95,7 @@ __device__ AttnPlan attn_scan(const AttnArgs& a, int nthreads, long long (&red)[
     AttnPlan p{0, 0, 0, a.seqs.n_seqs};
     auto cost = [&](int b) -> long long {
         if (b >= a.seqs.n_seqs) return 0;
-        const Kv4Seq s = kv4_seq(a.seqs, b, err);
+        const Kv4Seq s = attn_seq(a, b, err);
         int rts, lo, tiles;
         attn_seq_tiles<C>(a, s, rts, lo, tiles);
         return (long long)rts * (tiles + kUnitCost) * a.cache.kv_heads;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
             w_begin = p.begin;
             w_end = p.end;
             if (w_begin >= w_end) return;
-            const Kv4Seq s = kv4_seq(a.seqs, p.b, err);
+            const Kv4Seq s = attn_seq(a, p.b, err);
             int rts;
             attn_seq_tiles<C>(a, s, rts, u.t_lo, u.n_tiles);
             u.b = p.b; u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len;
@@ -199,18 +199,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         } else {
             // one unit per CTA, the units of a sequence's last rows (the longest) first; units are counted in row tiles
             const int h = blockIdx.x % a.cache.kv_heads;
-            long long at = blockIdx.x / a.cache.kv_heads;
-            int b = 0;
-            Kv4Seq s{0, 0, 0};
-            int rts = 0;
-            for (; b < a.seqs.n_seqs; ++b) {
-                s = kv4_seq(a.seqs, b, err);
-                rts = (int)(((int64_t)s.q_len * a.group + ROWS - 1) / ROWS);
-                if (at < rts) break;
-                at -= rts;
-            }
-            if (b >= a.seqs.n_seqs) return;
-            u.b = b; u.h = h; u.rt = rts - 1 - (int)at;
+            const RowTile where = locate_row_tile(a, blockIdx.x / a.cache.kv_heads, ROWS, 128, red, err);
+            if (where.b >= a.seqs.n_seqs) return;
+            const Kv4Seq s = attn_seq(a, where.b, err);
+            u.b = where.b; u.h = h; u.rt = where.rts - 1 - where.rt;
             u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len;
             const int j0 = u.rt * ROWS / a.group, j1 = min((u.rt * ROWS + ROWS - 1) / a.group, s.q_len - 1);
             const int p0 = s.len - s.q_len + j0, p1 = s.len - s.q_len + j1;
@@ -233,7 +225,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2
         n.h = 0;
         do {
             if (++n.b >= a.seqs.n_seqs) return;
-            s = kv4_seq(a.seqs, n.b, err);
+            s = attn_seq(a, n.b, err);
         } while (s.q_len == 0);
         n.row0 = s.row0; n.q_len = s.q_len; n.len = s.len;
         attn_seq_tiles<C>(a, s, rts, n.t_lo, n.n_tiles);
@@ -817,7 +809,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto cost = [&](int b, int& rts, int& tiles) -> long long {
         int lo;
-        const Kv4Seq s = kv4_seq(a.seqs, b, err);
+        const Kv4Seq s = attn_seq(a, b, err);
         attn_seq_tiles<C>(a, s, rts, lo, tiles);
         tiles += kUnitCost;
         return (long long)rts * tiles * a.cache.kv_heads;
@@ -907,7 +899,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     }
     pdl_wait();
     if (!work) return;
-    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const Kv4Seq s = attn_seq(a, b, err);
     const int rows_all = s.q_len * a.group;
     const bool first_odd = total * i0 / n < at;  // CTA i0 began before this unit: its part is in the odd slot
     auto slot_of = [&](int i) { return a.part + (size_t)(2 * i + (i == i0 && first_odd ? 1 : 0)) * ROWS * (D + 2); };
@@ -985,7 +977,7 @@ int kv4_reserve(moe_engine* e, size_t bytes) {
 }
 
 template <class C, typename T>
-static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
+static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64_t q_rows) {
     a.run = 1;
     while (a.run < C::NB && a.cache.page_size / kKv4Block % (2 * a.run) == 0) a.run *= 2;
     auto* kernel = kv4_attn_kernel<C, T>;
@@ -1005,7 +997,7 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
         return MOE_OK;
     } else {
         // no more CTAs than tiles there can be
-        const int64_t row_tiles = ((int64_t)a.seqs.max_q_len * a.group + C::ROWS - 1) / C::ROWS;
+        const int64_t row_tiles = (q_rows + C::ROWS - 1) / C::ROWS;
         const int64_t most = units * ((a.seqs.max_seq_len + C::TILE - 1) / C::TILE + 1 + kUnitCost);
         int64_t grid = (int64_t)e->sm_count * occ;
         if (grid > most) grid = most;
@@ -1030,24 +1022,44 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units) {
 // Rows of the tile: as few columns of eight as hold a sequence's rows, up to four.  Units of their own (no splitting) once
 // they fill the GPU twice over.
 template <int D, typename T>
-static int launch_attn(moe_engine* e, const AttnArgs& a) {
+static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int V0 = (D == 64 ? 0 : D == 128 ? 8 : 16) + (F32 ? 4 : 0);
-    const int64_t q_rows = (int64_t)a.seqs.max_q_len * a.group, n = a.seqs.n_seqs;
+    const int64_t n = a.seqs.n_seqs;
     auto units = [&](int rows) {  // at most: whole tiles of all rows, and one that is not full for every sequence
         const int64_t per_seq = (q_rows + rows - 1) / rows;
         const int64_t all = (int64_t)a.seqs.n_tokens * a.group / rows + n;
         return (all < per_seq * n ? all : per_seq * n) * a.cache.kv_heads;
     };
     constexpr int TB = 4 / (D / 64);
-    if constexpr (!F32) {
-        if (kv4_prompt_fits<D>(e, a)) return launch_kv4_prompt<D>(e, a);
-    } else {
-        if (q_rows > 16 && units(32) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(32));
+    if constexpr (F32) {
+        if (q_rows > 16 && units(32) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(32), q_rows);
     }
-    if (q_rows > 16) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(32));
-    if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16));
-    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8));
+    if (q_rows > 16) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(32), q_rows);
+    if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16), q_rows);
+    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8), q_rows);
+}
+
+template <int D, typename T>
+static int launch_attn(moe_engine* e, const AttnArgs& a) {
+    if constexpr (sizeof(T) == 2) {
+        if (kv4_prompt_fits<D>(e, a)) {
+            const int rc = launch_kv4_prompt<D>(e, a);
+            if (rc || a.seqs.n_seqs == 1 || a.seqs.max_q_len == a.seqs.n_tokens) return rc;
+            // the sequences of fewer rows, where there can be any: single tokens in as small a tile as they need, then the others
+            const int one = (a.group + 7) / 8 * 8;
+            AttnArgs few = a;
+            if (one < kPromptRows) {
+                few.hi_rows = one + 1;
+                const int rc1 = launch_rows<D, T>(e, few, one);
+                if (rc1) return rc1;
+                few.lo_rows = one + 1;
+            }
+            few.hi_rows = kPromptRows;
+            return few.lo_rows < kPromptRows ? launch_rows<D, T>(e, few, kPromptRows - 1) : rc;
+        }
+    }
+    return launch_rows<D, T>(e, a, (int64_t)a.seqs.max_q_len * a.group);
 }
 
 int check_kv4(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b);
@@ -1061,7 +1073,6 @@ using namespace moe;
 extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_kv4_batch_t* batch, const void* q_dev,
                                      int64_t q_token_stride, int64_t q_head_stride, const void* gate_dev, int64_t gate_token_stride,
                                      int64_t gate_head_stride, void* out_dev, int32_t dtype, int32_t num_heads, float scale, int32_t window) {
-    MOE_REQUIRE(e, "kv4_attention: null engine");
     int rc = check_kv4(cache, batch);
     if (rc) return rc;
     MOE_REQUIRE(dtype == MOE_DT_F32 || dtype == MOE_DT_BF16, "kv4_attention: queries are f32 or bf16 (got dtype %d)", dtype);
@@ -1076,6 +1087,12 @@ extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cac
     MOE_REQUIRE((((uintptr_t)q_dev | (uintptr_t)gate_dev) & amask) == 0, "kv4_attention: misaligned pointer");
     MOE_REQUIRE(((uintptr_t)out_dev & 15) == 0, "kv4_attention: the output must be 16-byte aligned");
     MOE_REQUIRE(q_token_stride >= 0 && q_head_stride >= 0 && gate_token_stride >= 0 && gate_head_stride >= 0, "kv4_attention: negative stride");
+    const int64_t esize = dtype == MOE_DT_F32 ? 4 : 2, D = cache->head_dim, T = batch->n_tokens;
+    auto extent = [&](int64_t ts, int64_t hs) { return ((T - 1) * ts + (num_heads - 1) * hs + D) * esize; };
+    MOE_REQUIRE(!ranges_overlap(q_dev, extent(q_token_stride, q_head_stride), out_dev, T * num_heads * D * esize) &&
+                    (!gate_dev || !ranges_overlap(gate_dev, extent(gate_token_stride, gate_head_stride), out_dev, T * num_heads * D * esize)),
+                "kv4_attention: the output overlaps the queries or gates");
+    MOE_REQUIRE(e, "kv4_attention: null engine");
     DeviceScope scope(e->device);
     MOE_CUDA(scope.status);
     AttnArgs a{};
@@ -1088,6 +1105,7 @@ extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cac
     a.by_group = make_group_div((uint32_t)a.group);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.window = window;
+    a.hi_rows = 0x7FFFFFFF;
     const int vec = dtype == MOE_DT_F32 ? 4 : 8;
     a.vec_q = ((uintptr_t)q_dev & 15) == 0 && (q_token_stride | q_head_stride) % vec == 0;
     a.vec_gate = ((uintptr_t)gate_dev & 15) == 0 && (gate_token_stride | gate_head_stride) % vec == 0;

@@ -28,18 +28,73 @@ struct AttnArgs {
     GroupDiv by_group;
     float scale_log2;        // scale * log2(e)
     int window;              // 0: none
+    int lo_rows, hi_rows;    // sequences with lo_rows <= rows < hi_rows (rows x query heads per KV head) are this launch's
     int run;                 // blocks of a tile that one copy brings (they lie in one page)
     float* part;             // work area of the call
 };
 
 int kv4_reserve(moe_engine* e, size_t bytes);
-// Prompts of bf16 rows on the fifth-generation tensor cores; whether the call suits that path
+// Prompts of bf16 rows on the fifth-generation tensor cores: sequences of at least kPromptRows rows x query heads per KV
+// head; whether the call has such and its work area is not too large
+constexpr int kPromptRows = 128;
 template <int D>
 bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a);
 template <int D>
 int launch_kv4_prompt(moe_engine* e, AttnArgs a);
 
 #ifdef __CUDACC__
+// A sequence as a launch sees it: without rows where they are another launch's.
+__device__ __forceinline__ Kv4Seq attn_seq(const AttnArgs& a, int b, unsigned int* err) {
+    Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const long long rows = (long long)s.q_len * a.group;
+    if (rows < a.lo_rows || rows >= a.hi_rows) s.q_len = 0;
+    return s;
+}
+// Row tile `at` in the line of all sequences' row tiles (of `rows` rows): its sequence (n_seqs: none), its index there and the
+// number of sequences with rows before that one.  Called by all threads of a CTA of n_threads (a multiple of 32);
+// red: one word per warp and two more, in shared memory.
+struct RowTile {
+    int b, rt, rts, before;
+};
+__device__ __forceinline__ RowTile locate_row_tile(const AttnArgs& a, long long at, int rows, int n_threads, long long* red, unsigned int* err) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = n_threads >> 5;
+    constexpr long long kOne = 1ll << 44;  // sequences counted above the row tiles
+    long long carry = 0;
+    for (int b0 = 0; b0 < a.seqs.n_seqs; b0 += n_threads) {
+        long long mine = 0;
+        if (b0 + tid < a.seqs.n_seqs) {
+            const Kv4Seq s = attn_seq(a, b0 + tid, err);
+            mine = ((long long)s.q_len * a.group + rows - 1) / rows;
+        }
+        const long long own = mine > 0 ? mine + kOne : 0;
+        long long inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        __syncthreads();
+        if (lane == 31) red[warp] = inc;
+        __syncthreads();
+        long long before = carry, sum = 0;
+        for (int w = 0; w < nw; ++w) {
+            if (w < warp) before += red[w];
+            sum += red[w];
+        }
+        before += inc - own;
+        const long long lo = before & (kOne - 1);
+        if (mine > 0 && at >= lo && at < lo + mine) {
+            red[nw] = (long long)(b0 + tid) << 32 | (at - lo);
+            red[nw + 1] = (before >> 44) << 32 | mine;
+        }
+        carry += sum;
+        if (at < (carry & (kOne - 1))) {
+            __syncthreads();
+            return RowTile{(int)(red[nw] >> 32), (int)(red[nw] & 0xFFFFFFFFll), (int)(red[nw + 1] & 0xFFFFFFFFll), (int)(red[nw + 1] >> 32)};
+        }
+    }
+    return RowTile{a.seqs.n_seqs, 0, 0, 0};
+}
 __device__ __forceinline__ int over_group(int n, const GroupDiv& g) { return (int)((__umulhi((uint32_t)n, g.mul) + (uint32_t)n) >> g.shift); }
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;

@@ -41,7 +41,8 @@ __device__ __forceinline__ void pt_range(const AttnArgs& a, const Kv4Seq& s, int
     n = s.q_len > 0 ? (s.len + kPtTile - 1) / kPtTile - t0 : 0;
 }
 
-// One CTA expands K or V of one tile of one head.  image: [(sequence, head, tile)][K, V][IMG bytes]; meta alike, kPtMeta ints.
+// One CTA expands K or V of one tile of one head.  image: [(sequence, head, tile)][K, V][IMG bytes], the sequences that have
+// rows here counted; meta alike, kPtMeta ints.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_per_seq, uint8_t* image, int* meta, unsigned int* err) {
     using C = PtCfg<D>;
@@ -53,10 +54,12 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool is_v = blockIdx.x & 1;
     const int ti = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
-    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const Kv4Seq s = attn_seq(a, b, err);
     int tile0, n;
     pt_range(a, s, tile0, n);
-    if (ti >= n || ti >= tiles_per_seq) return;
+    if (ti >= n || ti >= tiles_per_seq) return;  // (a sequence without rows here has no tiles)
+    int before = 0;                              // sequences with rows before this one
+    for (int b0 = 0; b0 < b; b0 += 256) before += __syncthreads_count(b0 + tid < b && attn_seq(a, b0 + tid, err).q_len > 0);
     const int p0 = (tile0 + ti) * kPtTile;
     if (tid < 8) blocks[tid] = p0 + tid * 16 < s.len ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
     if (tid < 4) nan_bits[tid] = 0;
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     // scaled into [1, 2); an all-zero tile keeps a harmless exponent
     const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 126);
     const float down = pow2f(-e);
-    const size_t at = ((size_t)(b * a.cache.kv_heads + h) * tiles_per_seq + ti);
+    const size_t at = ((size_t)before * a.cache.kv_heads + h) * tiles_per_seq + ti;
     if (tid == 0) meta[at * kPtMeta + (is_v ? 1 : 0)] = e;
     if (is_v && tid < 4) meta[at * kPtMeta + 2 + tid] = (int)nan_bits[tid];
 
@@ -185,24 +188,18 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
 
     // which rows: units are counted in row tiles, the last rows of a sequence (which see most) first
     const int h = blockIdx.x % a.cache.kv_heads;
-    long long at = blockIdx.x / a.cache.kv_heads;
-    int b = 0, rts = 0;
-    Kv4Seq s{0, 0, 0};
-    for (; b < a.seqs.n_seqs; ++b) {
-        s = kv4_seq(a.seqs, b, err);
-        rts = (int)(((int64_t)s.q_len * a.group + kPtTile - 1) / kPtTile);
-        if (at < rts) break;
-        at -= rts;
-    }
+    const RowTile where = locate_row_tile(a, blockIdx.x / a.cache.kv_heads, kPtTile, 320, reinterpret_cast<long long*>(sm + C::OFF_TOP), err);
+    const int b = where.b;
     if (b >= a.seqs.n_seqs) return;
-    const int rt = rts - 1 - (int)at, rows_all = s.q_len * a.group, pos_base = s.len - s.q_len;
+    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const int rt = where.rts - 1 - where.rt, rows_all = s.q_len * a.group, pos_base = s.len - s.q_len;
     int seq_t0, seq_n;
     pt_range(a, s, seq_t0, seq_n);
     const int j_first = rt * kPtTile / a.group, j_last = min((rt * kPtTile + kPtTile - 1) / a.group, s.q_len - 1);
     const int p_last = pos_base + j_last;  // may be negative: rows without a position
     const int t_begin = a.window > 0 ? max(pos_base + j_first - a.window + 1, 0) / kPtTile : 0;
     const int n_tiles = p_last >= 0 ? min(p_last / kPtTile + 1, seq_t0 + min(seq_n, tiles_per_seq)) - t_begin : 0;
-    const size_t img0 = (size_t)(b * a.cache.kv_heads + h) * tiles_per_seq + (t_begin - seq_t0);
+    const size_t img0 = ((size_t)where.before * a.cache.kv_heads + h) * tiles_per_seq + (t_begin - seq_t0);
 
     if (tid == 0) {
         mbar_init(k_full, 1);
@@ -501,15 +498,19 @@ static int pt_tiles_per_seq(const AttnArgs& a) {
     const int64_t seen = ((int64_t)a.window + a.seqs.max_q_len + kPtTile - 1) / kPtTile + 1;
     return (int)(seen < all ? seen : all);
 }
+static int64_t pt_max_seqs(const AttnArgs& a) {  // sequences that can have kPromptRows rows
+    const int64_t n = (int64_t)a.seqs.n_tokens * a.group / kPromptRows;
+    return n < a.seqs.n_seqs ? n : a.seqs.n_seqs;
+}
 template <int D>
 static size_t pt_image_bytes(const AttnArgs& a) {
-    return (size_t)a.seqs.n_seqs * a.cache.kv_heads * pt_tiles_per_seq(a) * 2 * PtCfg<D>::IMG;
+    return (size_t)pt_max_seqs(a) * a.cache.kv_heads * pt_tiles_per_seq(a) * 2 * PtCfg<D>::IMG;
 }
 
-// At least a full tile of rows per sequence, and images of at most 4 GB.
+// Images of at most 4 GB: a call that could need more (many sequences of unknown lengths) takes the kernel that needs none.
 template <int D>
 bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a) {
-    return (int64_t)a.seqs.max_q_len * a.group >= kPtTile && pt_image_bytes<D>(a) <= (size_t)4 << 30 && a.cache.kv_heads <= 65535 &&
+    return (int64_t)a.seqs.max_q_len * a.group >= kPromptRows && pt_image_bytes<D>(a) <= (size_t)4 << 30 && a.cache.kv_heads <= 65535 &&
            a.seqs.n_seqs <= 65535;
 }
 
@@ -517,7 +518,9 @@ template <int D>
 int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
     using C = PtCfg<D>;
     const int tiles = pt_tiles_per_seq(a);
-    const size_t image = pt_image_bytes<D>(a), meta = (size_t)a.seqs.n_seqs * a.cache.kv_heads * tiles * kPtMeta * 4;
+    const size_t image = pt_image_bytes<D>(a), meta = (size_t)pt_max_seqs(a) * a.cache.kv_heads * tiles * kPtMeta * 4;
+    a.lo_rows = kPromptRows;
+    a.hi_rows = 0x7FFFFFFF;
     int rc = kv4_reserve(e, image + meta);
     if (rc) return rc;
     uint8_t* img = reinterpret_cast<uint8_t*>(e->kv4.work);

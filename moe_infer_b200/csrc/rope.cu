@@ -215,7 +215,6 @@ int moe_rope_table_host(const moe_rope_params_t* p, int64_t first_position, int6
 int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int64_t x_token_stride, int64_t x_head_stride,
                  void* out_dev, int64_t out_token_stride, int64_t out_head_stride, int32_t dtype, int64_t n_tokens, int32_t num_heads,
                  int32_t head_dim, const int32_t* positions_dev) {
-    MOE_REQUIRE(e, "rope: null engine");
     MOE_REQUIRE(n_tokens >= 0 && num_heads > 0 && head_dim > 0, "rope: bad shape [%lld, %d, %d]", (long long)n_tokens, num_heads, head_dim);
     int rc = check_rope(rope, head_dim);
     if (rc) return rc;
@@ -228,6 +227,11 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
     MOE_REQUIRE(rows_disjoint(n_tokens, out_token_stride, num_heads, out_head_stride, head_dim), "rope: output rows overlap");
     MOE_REQUIRE(x_dev != out_dev || (x_token_stride == out_token_stride && x_head_stride == out_head_stride),
                 "rope: in place needs equal strides");
+    const int64_t esize = dtype == MOE_DT_F32 ? 4 : 2;
+    auto extent = [&](int64_t ts, int64_t hs) { return ((n_tokens - 1) * ts + (num_heads - 1) * hs + head_dim) * esize; };
+    MOE_REQUIRE(x_dev == out_dev || !ranges_overlap(x_dev, extent(x_token_stride, x_head_stride), out_dev, extent(out_token_stride, out_head_stride)),
+                "rope: input and output overlap without being the same");
+    MOE_REQUIRE(e, "rope: null engine");
     DeviceScope scope(e->device);
     MOE_CUDA(scope.status);
     RopeArgs a{rope->cos_sin, rope->n_positions, rope->rotary_dim, num_heads, head_dim, n_tokens, x_token_stride, x_head_stride,

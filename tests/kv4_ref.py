@@ -48,7 +48,7 @@ def rotate_f32(x, cs, interleaved):
 def attention(q, k, v, lens, q_lens, window, scale):
     """q f64 [rows, heads, dim]; k, v of the sequences back to back [sum lens, kv_heads, dim] -> result f64, and what the
     kernel's rounding is relative to: per row and element the weighted sum of |v| + 8 scales, per row and head the largest
-    scale * sum |q_d k_td| of the positions it sees."""
+    |scale| * sum |q_d k_td| of the positions it sees."""
     rows, heads, dim = sum(q_lens), q.shape[1], q.shape[2]
     group = heads // k.shape[1]
     out, size, reach = np.zeros((rows, heads, dim)), np.zeros((rows, heads, dim)), np.zeros((rows, heads, 1))
@@ -70,7 +70,7 @@ def attention(q, k, v, lens, q_lens, window, scale):
             out[at:at + nq, h] = p @ vb[:, h // group]
             vh = vb[:, h // group]
             size[at:at + nq, h] = p @ (np.abs(vh) + np.repeat(np.ptp(vh.reshape(n, -1, 64), 2) * 8 / 15, 64, 1))
-            reach[at:at + nq, h, 0] = np.where(see, np.abs(q[at:at + nq, h]) @ np.abs(kb[:, h // group]).T * scale, 0).max(1)
+            reach[at:at + nq, h, 0] = np.where(see, np.abs(q[at:at + nq, h]) @ np.abs(kb[:, h // group]).T * abs(scale), 0).max(1)
         at += nq
     return out, size, reach
 

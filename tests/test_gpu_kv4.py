@@ -89,26 +89,31 @@ def as_f64(x, dtype):
 # in all for f32 rows, hence 2^-21 reach; then the 2-ulp exponential, the weight as an operand and the f32 sums of the value
 # pass: 2^-19 for f32 rows (22-bit weights), 2^-11 for bf16 rows (11-bit weights: half a step 2^-12, numerator against the
 # unrounded sum), and half a step of bf16, 2^-8 of its value at most, for their result.
+# Prompts of bf16 rows also hold keys and values as f16 (11 bits: half a step 2^-12 of a value, and of a key's elements, so
+# 2^-12 reach in a score, twice that in a weight).
 def bound_of(dtype, want, size, reach):
-    own = 2.0 ** -24 if dtype == L.DT_F32 else 2.0 ** -8
-    return size * (2.0 ** -19 if dtype == L.DT_F32 else 2.0 ** -11) + 2.0 ** -21 * reach * size + own * np.abs(want) + 1e-30
+    if dtype == L.DT_F32:
+        return size * 2.0 ** -19 + 2.0 ** -21 * reach * size + 2.0 ** -24 * np.abs(want) + 1e-30
+    return size * (2.0 ** -11 + 2.0 ** -12) + 2.0 ** -11 * reach * size + 2.0 ** -8 * np.abs(want) + 1e-30
 
 
 def check_attention(eng, lens, q_lens, *, heads, kv_heads, dim, page, dtype, window=0, gate=False, seed=0, spare_rows=0, q_scale=1.5, max_q=None,
-                    strided=False):
+                    strided=False, odd=0, scale=None):
     c = Case(eng, lens, q_lens, kv_heads=kv_heads, dim=dim, page=page, seed=seed, spare_rows=spare_rows, max_q=max_q)
     k, v = c.fill()
     wide = 2 if strided else 1
+    scale = 1 / math.sqrt(dim) if scale is None else scale
     q = as_type(q_scale * c.rng.standard_normal((c.n_tokens, heads, wide * dim)), dtype)
     g = as_type(c.rng.standard_normal((c.n_tokens, heads, dim)), dtype) if gate else None
     out = c.up(np.full((c.n_tokens, heads, dim), 7, q.dtype))
-    args = dict(scale=1 / math.sqrt(dim), window=window, q_strides=(heads * wide * dim, wide * dim))
+    args = dict(scale=scale, window=window, q_strides=(heads * wide * dim, wide * dim))
+    at = lambda x: c.up(np.concatenate([np.zeros(odd, x.dtype), x.reshape(-1)])).ptr + odd * x.dtype.itemsize  # noqa: E731  (off its alignment)
     if gate:
-        args["gate"] = c.up(g).ptr
-    eng.kv4_attention_dev(c.cache, c.batch, c.up(q).ptr, out.ptr, dtype, heads, **args)
+        args["gate"] = at(g)
+    eng.kv4_attention_dev(c.cache, c.batch, at(q), out.ptr, dtype, heads, **args)
     eng.sync()
     got = out.download(q.dtype, (c.n_tokens, heads, dim))
-    want, size, reach = R.attention(as_f64(q[..., :dim], dtype), k, v, lens, q_lens, window, 1 / math.sqrt(dim))
+    want, size, reach = R.attention(as_f64(q[..., :dim], dtype), k, v, lens, q_lens, window, scale)
     if gate:
         s = 1 / (1 + np.exp(-as_f64(g, dtype)[:c.rows]))
         want, size = want * s, size * s
@@ -171,6 +176,82 @@ def test_long_and_ragged(eng, dtype):
 def test_query_sizes(eng, q_scale):
     """All-equal weights, scores that underflow to equal, and nearly one-hot weights."""
     check_attention(eng, [200, 70], [1, 1], heads=4, kv_heads=1, dim=128, page=16, dtype=L.DT_F32 if q_scale < 10 else L.DT_BF16, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+def test_scales(eng, scale, dtype):
+    check_attention(eng, [200, 140], [1, 130], heads=4, kv_heads=1, dim=64, page=16, dtype=dtype, scale=scale)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 14, 2), (128, 8, 8), (256, 16, 2)])
+@pytest.mark.parametrize("window", [0, 1, 90, 300])
+def test_batches_of_prompts_and_decodes(eng, dim, heads, kv_heads, window):
+    """Prompts, chunks, verifications, single tokens, idle slots and sequences without rows in one call; rows and gates off
+    their 16-byte alignment."""
+    check_attention(eng, [700, 33, 1, 0, 650, 500, 64, 40], [200, 1, 1, 1, 650, 4, 0, 40], heads=heads, kv_heads=kv_heads, dim=dim, page=16,
+                    dtype=L.DT_BF16, window=window, gate=True, spare_rows=1, odd=3)
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+def test_unaligned_rows(eng, dtype):
+    check_attention(eng, [90, 17], [2, 2], heads=8, kv_heads=2, dim=128, page=16, dtype=dtype, gate=True, odd=1)
+
+
+def test_same_call_same_bits(eng):
+    for dtype, q_lens in ((L.DT_F32, [1, 1]), (L.DT_BF16, [300, 7])):
+        c = Case(eng, [5000, 900], q_lens, kv_heads=2, dim=128, page=16, seed=8)
+        c.fill()
+        q = c.up(as_type(c.rng.standard_normal((c.n_tokens, 8, 128)), dtype))
+        got = []
+        for _ in range(3):
+            out = c.up(np.zeros((c.n_tokens, 8, 128), np.float32 if dtype == L.DT_F32 else np.uint16))
+            eng.kv4_attention_dev(c.cache, c.batch, q.ptr, out.ptr, dtype, 8, scale=0.1)
+            eng.sync()
+            got.append(out.download(np.uint8, (c.n_tokens * 8 * 128 * (4 if dtype == L.DT_F32 else 2),)))
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+        c.free()
+
+
+def test_calls_behind_one_another(eng):
+    """Calls of different shapes enqueued without waiting share the engine's work area in turn."""
+    cases, outs = [], []
+    for k, (lens, q_lens, dtype) in enumerate((([3000], [1], L.DT_F32), ([400], [400], L.DT_BF16), ([2500, 300], [1, 1], L.DT_BF16), ([130], [130], L.DT_F32))):
+        c = Case(eng, lens, q_lens, kv_heads=2, dim=128, page=16, seed=30 + k)
+        kv = c.fill()
+        q = as_type(c.rng.standard_normal((c.n_tokens, 8, 128)), dtype)
+        outs.append((c.up(q).ptr, c.up(np.zeros_like(q)), q, kv, dtype))
+        cases.append(c)
+    for _ in range(2):
+        for c, (qp, out, _, _, dtype) in zip(cases, outs):
+            eng.kv4_attention_dev(c.cache, c.batch, qp, out.ptr, dtype, 8, scale=0.1)
+    eng.sync()
+    for c, (_, out, q, (k, v), dtype) in zip(cases, outs):
+        want, size, reach = R.attention(as_f64(q, dtype), k, v, c.lens, c.q_lens, 0, 0.1)
+        assert np.all(np.abs(as_f64(out.download(q.dtype, q.shape), dtype) - want) <= bound_of(dtype, want, size, reach))
+        c.free()
+
+
+def test_pages_beyond_4_gib(eng):
+    """Byte offsets of pages pass 32 bits."""
+    kv_heads, dim, page = 8, 256, 64
+    per = kv4_page_bytes(page, kv_heads, dim)
+    num = (9 << 29) // per  # 4.5 GiB
+    pages = eng.alloc(num * per)
+    c = Case(eng, [150, 70], [150, 1], kv_heads=kv_heads, dim=dim, page=page, seed=12)
+    c.cache = Kv4Cache(pages.ptr, num, page, kv_heads, dim)
+    c.table = np.array([[num - 1, 3, num - 7], [num - 2, num // 2, -1]], np.int32)
+    c.batch = c.batch_of(c.q_start, c.n_tokens, c.max_q)
+    k, v = c.fill()
+    for dtype in (L.DT_F32, L.DT_BF16):
+        q = as_type(c.rng.standard_normal((c.n_tokens, 8, dim)), dtype)
+        out = c.up(np.zeros_like(q))
+        eng.kv4_attention_dev(c.cache, c.batch, c.up(q).ptr, out.ptr, dtype, 8, scale=0.1)
+        eng.sync()
+        want, size, reach = R.attention(as_f64(q, dtype), k, v, c.lens, c.q_lens, 0, 0.1)
+        assert np.all(np.abs(as_f64(out.download(q.dtype, q.shape), dtype) - want) <= bound_of(dtype, want, size, reach))
+    pages.free()
+    c.free()
 
 
 def test_many_sequences(eng):
@@ -294,6 +375,27 @@ def test_non_finite_values(eng):
     c.free()
 
 
+def test_non_finite_values_in_a_prompt(eng):
+    """The same for many bf16 rows: rows before the position (or with it outside their window) keep their results."""
+    c = Case(eng, [300], [300], kv_heads=1, dim=128, page=16, seed=2)
+    k = c.rng.standard_normal((300, 1, 128)).astype(np.float32)
+    v = c.rng.standard_normal((300, 1, 128)).astype(np.float32)
+    v[170, 0, 5] = np.inf
+    eng.kv4_append_dev(c.cache, c.batch, c.up(k).ptr, c.up(v).ptr, L.DT_F32)
+    q = as_type(c.rng.standard_normal((300, 4, 128)), L.DT_BF16)
+    out = c.up(np.zeros_like(q))
+    v[170] = 0.0
+    for window in (0, 20):
+        eng.kv4_attention_dev(c.cache, c.batch, c.up(q).ptr, out.ptr, L.DT_BF16, 4, scale=0.1, window=window)
+        eng.sync()
+        got = as_f64(out.download(q.dtype, q.shape), L.DT_BF16)
+        hit = np.arange(300) >= 170 if window == 0 else (np.arange(300) >= 170) & (np.arange(300) < 190)
+        assert np.isnan(got[hit][..., :64]).all() and np.isfinite(got[~hit]).all()
+        want, size, reach = R.attention(as_f64(q, L.DT_BF16), R.codec(k), R.codec(v), [300], [300], window, 0.1)
+        assert np.all(np.abs(got - want)[~hit] <= bound_of(L.DT_BF16, want, size, reach)[~hit])
+    c.free()
+
+
 # ─── rotary positions ───────────────────────────────────────────────────────
 @pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
 @pytest.mark.parametrize("interleaved", [0, 1])
@@ -358,7 +460,7 @@ def test_bad_entries_are_reported_and_touch_nothing(eng):
     c.fill()
     before = c.pages.download(np.uint8, (c.bytes,))
     kv = c.up(np.ones((3, 2, 64), np.float32))
-    q, out = c.up(np.ones((3, 2, 64), np.float32)), c.up(np.zeros((3, 2, 64), np.float32))
+    q, out, out2 = c.up(np.ones((3, 2, 64), np.float32)), c.up(np.zeros((3, 2, 64), np.float32)), c.up(np.zeros((3, 2, 64), np.float32))
     tab = RopeTable(c.up(rope_table(8, 30, 1e4)).ptr, 30, 8, 0)
     for bad in (-5, c.num_pages, 1 << 30):
         saved = c.table.copy()
@@ -366,7 +468,7 @@ def test_bad_entries_are_reported_and_touch_nothing(eng):
         batch = c.batch_of(c.q_start, 3, 2)
         c.table = saved
         for call in (lambda: eng.kv4_append_dev(c.cache, batch, kv.ptr, kv.ptr, L.DT_F32),
-                     lambda: eng.kv4_gather_dev(c.cache, batch, out.ptr, out.ptr, L.DT_F32),
+                     lambda: eng.kv4_gather_dev(c.cache, batch, out.ptr, out2.ptr, L.DT_F32),
                      lambda: eng.kv4_attention_dev(c.cache, batch, q.ptr, out.ptr, L.DT_F32, 2, scale=0.1)):
             call()
             with pytest.raises(ValueError, match="page table"):
