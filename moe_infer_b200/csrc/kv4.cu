@@ -98,6 +98,140 @@ __device__ __forceinline__ int kv4_k_offset(int l, int t) {
     return (g / U) * (512 * U) + ((t & 1) * 8 + (t >> 1)) * (32 * U) + c * (8 * U) + (g % U) * 8 + j * 4;
 }
 
+// Stores four positions' words and pairs; [lo, hi): which of the four exist.
+template <int D>
+__device__ __forceinline__ void kv4_store(uint8_t* nib, bool is_v, int l, int t0, int lo, int hi, const uint32_t (&word)[4], uint32_t pair) {
+    if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= lo && i < hi) *reinterpret_cast<uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i)) = word[i];
+    } else {
+        // bytes of the four positions, elements (2x, 2x + 1): word x of the lane's 16
+        uint8_t* dst = nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16;
+        uint32_t w[4];
+        transpose_bytes(word, w);
+        if (lo <= 0 && hi == 4) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int x4 = 0; x4 < 4; ++x4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= lo && i < hi) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
+        }
+    }
+    const int mine = l & 7;
+    if (mine >= lo && mine < hi) *(reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0 + mine) = pair;
+}
+
+enum { kRotNone = 0, kRotHalf = 1, kRotInter = 2 };
+
+// Rows readable 16 bytes at a time and a rotation of whole lanes (rotary a multiple of 16 in the half layout, 8 interleaved):
+// a CTA walks `per` heads of its 16 positions, the next head's rows requested before this one's are worked on; in the
+// interleaved layout a lane keeps the cosines and sines of its pairs for all of them.
+template <typename T, int D, int kRot>
+__global__ void __launch_bounds__(D, 512 / D) kv4_append_heads_kernel(Kv4AppendArgs a, int per, unsigned int* err) {
+    constexpr int LPT = D / 8, W = sizeof(T) / 2;                    // 16-byte words of a lane's eight elements
+    const int l = threadIdx.x % LPT, sub = threadIdx.x / LPT;        // eight sub-warps: four quads of keys, then of values
+    const bool is_v = sub >= 4;
+    const int b = blockIdx.z, h0 = blockIdx.x * per, h1 = min(h0 + per, a.cache.kv_heads);
+    const Kv4Seq s = kv4_seq(a.seqs, b, err);
+    const int first = max(s.len - s.q_len, 0);
+    const int p0 = (first & ~15) + 16 * (int)blockIdx.y;
+    if (p0 >= s.len || s.len <= first) return;
+    const int q0 = p0 + 4 * (sub & 3), lo = max(first - q0, 0), hi = min(s.len - q0, 4);
+    const int64_t ts = is_v ? a.vt : a.kt, hs = is_v ? a.vh : a.kh;
+    const int64_t row0 = s.row0 + s.q_len - s.len + q0;              // row of the quad's first position (may lie before the rows)
+    const T* src = (is_v ? (const T*)a.v : (const T*)a.k) + row0 * ts + h0 * hs + 8 * l;
+    uint4 raw[4][W];
+    auto load = [&](const T* p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= lo && i < hi) {
+#pragma unroll
+                for (int w = 0; w < W; ++w) raw[i][w] = reinterpret_cast<const uint4*>(p + i * ts)[w];
+            }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < W; ++w) raw[i][w] = make_uint4(0, 0, 0, 0);
+    load(src);
+    float cs[4][4], sn[4][4];  // interleaved: of the lane's four pairs
+    const float* turn_at[4];   // half: where those of the lane's eight elements are
+    const int half = a.rotary >> 1;
+    const bool turns = kRot != kRotNone && !is_v && 8 * l < a.rotary, second = kRot == kRotHalf && 8 * l >= half;
+    unsigned turned = 0;
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < lo || i >= hi) continue;
+            const int64_t pos = a.rope_positions ? a.rope_positions[row0 + i] : q0 + i;
+            if (pos < 0 || pos >= a.n_positions) {
+                atomicExch(err, kErrRopePos);
+                continue;
+            }
+            turned |= 1u << i;
+            turn_at[i] = a.table + pos * a.rotary + (kRot == kRotInter ? 4 * l : second ? 8 * l - half : 8 * l);
+            if constexpr (kRot == kRotInter) {
+                *reinterpret_cast<float4*>(cs[i]) = *reinterpret_cast<const float4*>(turn_at[i]);
+                *reinterpret_cast<float4*>(sn[i]) = *reinterpret_cast<const float4*>(turn_at[i] + half);
+            }
+        }
+    }
+    uint8_t* blk = kv4_block(a.cache, a.seqs, b, h0, p0, kv4_block_bytes(D), err);
+    const size_t head_bytes = (size_t)(a.cache.page_size / kKv4Block) * kv4_block_bytes(D);
+    const int partner = (threadIdx.x & 31) + (second ? -(half >> 3) : half >> 3);  // the lane that holds the pairs' other elements
+    for (int h = h0; h < h1; ++h) {
+        float x[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i][0]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (W == 2) x[i][k] = __uint_as_float(w[k]);
+                else x[i][k] = __uint_as_float((k & 1) ? w[k >> 1] & 0xFFFF0000u : w[k >> 1] << 16);
+            }
+        }
+        src += hs;
+        if (h + 1 < h1) load(src);
+        if constexpr (kRot == kRotHalf) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool on = turned >> i & 1;
+                float c8[8], s8[8];
+                if (on) {
+                    ld_act8(turn_at[i], true, c8);
+                    ld_act8(turn_at[i] + half, true, s8);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float o = __shfl_sync(0xffffffffu, x[i][k], partner & 31);
+                    if (on)
+                        x[i][k] = second ? __fadd_rn(__fmul_rn(o, s8[k]), __fmul_rn(x[i][k], c8[k]))
+                                         : __fsub_rn(__fmul_rn(x[i][k], c8[k]), __fmul_rn(o, s8[k]));
+                }
+            }
+        }
+        if constexpr (kRot == kRotInter) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (turned >> i & 1) {
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const float u = x[i][k], v = x[i][k + 1];
+                        x[i][k] = __fsub_rn(__fmul_rn(u, cs[i][k >> 1]), __fmul_rn(v, sn[i][k >> 1]));
+                        x[i][k + 1] = __fadd_rn(__fmul_rn(u, sn[i][k >> 1]), __fmul_rn(v, cs[i][k >> 1]));
+                    }
+                }
+        }
+        uint32_t word[4];
+        const uint32_t pair = kv4_quant(x, word);
+        if (blk && hi > lo) kv4_store<D>(blk + (h - h0) * head_bytes + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, lo, hi, word, pair);
+    }
+}
+
+// One head to a CTA; any strides and alignment, any rotation.
 template <typename T, int D>
 __global__ void __launch_bounds__(D, 1024 / D) kv4_append_kernel(Kv4AppendArgs a, unsigned int* err) {
     constexpr int LPT = D / 8;
@@ -169,31 +303,7 @@ __global__ void __launch_bounds__(D, 1024 / D) kv4_append_kernel(Kv4AppendArgs a
     }
     uint32_t word[4];
     const uint32_t pair = kv4_quant(x, word);
-    if (!blk || hi <= lo) return;
-
-    const int t0 = q0 % kKv4Block;  // 0, 4, 8 or 12
-    uint8_t* nib = blk + (is_v ? 9 * D : 0);
-    if (!is_v) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i >= lo && i < hi) *reinterpret_cast<uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i)) = word[i];
-    } else {
-        // bytes of the four positions, elements (2x, 2x + 1): word x of the lane's 16
-        uint8_t* dst = nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16;
-        uint32_t w[4];
-        transpose_bytes(word, w);
-        if (lo <= 0 && hi == 4) {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-            for (int x4 = 0; x4 < 4; ++x4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= lo && i < hi) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
-        }
-    }
-    const int mine = l & 7;
-    if (mine >= lo && mine < hi) *(reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0 + mine) = pair;
+    if (blk && hi > lo) kv4_store<D>(blk + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, lo, hi, word, pair);
 }
 
 // The way back: same mapping, values = nibble * scale + bias (the product is exact, so one rounding).
@@ -310,17 +420,37 @@ int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
     a.rope_positions = rope_positions_dev;
     a.vec_k = ((uintptr_t)k_dev & 15) == 0 && (k_token_stride | k_head_stride) % vec == 0;
     a.vec_v = ((uintptr_t)v_dev & 15) == 0 && (v_token_stride | v_head_stride) % vec == 0;
-    a.vec_table = a.rotary % 8 == 0 && ((uintptr_t)a.table & 15) == 0;
-    a.vec_partner = a.vec_k && a.rotary % 16 == 0 && ((uintptr_t)a.table & 15) == 0;
     MOE_REQUIRE(blocks_of(batch) <= 65535 && batch->n_seqs <= 65535, "kv4_append: too many rows or sequences for one call");
     unsigned int* err = e->dec_sync + 2;
-    const dim3 grid(cache->num_kv_heads, (unsigned)blocks_of(batch), batch->n_seqs);
-    auto run = [&](auto kernel) { kernel<<<grid, cache->head_dim, 0, e->stream>>>(a, err); };
     const bool f32 = dtype == MOE_DT_F32;
-    switch (cache->head_dim) {
-        case 64: f32 ? run(kv4_append_kernel<float, 64>) : run(kv4_append_kernel<__nv_bfloat16, 64>); break;
-        case 128: f32 ? run(kv4_append_kernel<float, 128>) : run(kv4_append_kernel<__nv_bfloat16, 128>); break;
-        default: f32 ? run(kv4_append_kernel<float, 256>) : run(kv4_append_kernel<__nv_bfloat16, 256>); break;
+    const int rot = !rope ? kRotNone : a.interleaved ? kRotInter : kRotHalf;
+    a.vec_table = a.rotary % 8 == 0 && ((uintptr_t)a.table & 15) == 0;
+    a.vec_partner = a.vec_k && a.rotary % 16 == 0 && a.vec_table;
+    const bool whole = a.vec_k && a.vec_v && (!rope || (a.vec_table && a.rotary % (a.interleaved ? 8 : 16) == 0));
+    // up to four heads to a CTA where that still leaves every SM four CTAs (14,000 bf16 rows of eight heads: 46 us with one head
+    // each, 24 us with four; with few CTAs the one-head kernel's smaller register count is worth more: 8,192 f32 rows of two
+    // heads, 18 us against 30)
+    int per = 1;
+    while (whole && per < 4 && per * 2 <= cache->num_kv_heads && blocks_of(batch) * batch->n_seqs * cache->num_kv_heads / (per * 2) >= 4 * e->sm_count) per *= 2;
+    if (per > 1) {
+        const dim3 grid((cache->num_kv_heads + per - 1) / per, (unsigned)blocks_of(batch), batch->n_seqs);
+        auto run = [&](auto kernel) { kernel<<<grid, cache->head_dim, 0, e->stream>>>(a, per, err); };
+        auto by_rot = [&](auto none, auto half, auto inter) { rot == kRotNone ? run(none) : rot == kRotHalf ? run(half) : run(inter); };
+#define KV4_HEADS(T, D) by_rot(kv4_append_heads_kernel<T, D, kRotNone>, kv4_append_heads_kernel<T, D, kRotHalf>, kv4_append_heads_kernel<T, D, kRotInter>)
+        switch (cache->head_dim) {
+            case 64: f32 ? KV4_HEADS(float, 64) : KV4_HEADS(__nv_bfloat16, 64); break;
+            case 128: f32 ? KV4_HEADS(float, 128) : KV4_HEADS(__nv_bfloat16, 128); break;
+            default: f32 ? KV4_HEADS(float, 256) : KV4_HEADS(__nv_bfloat16, 256); break;
+        }
+#undef KV4_HEADS
+    } else {
+        const dim3 grid(cache->num_kv_heads, (unsigned)blocks_of(batch), batch->n_seqs);
+        auto run = [&](auto kernel) { kernel<<<grid, cache->head_dim, 0, e->stream>>>(a, err); };
+        switch (cache->head_dim) {
+            case 64: f32 ? run(kv4_append_kernel<float, 64>) : run(kv4_append_kernel<__nv_bfloat16, 64>); break;
+            case 128: f32 ? run(kv4_append_kernel<float, 128>) : run(kv4_append_kernel<__nv_bfloat16, 128>); break;
+            default: f32 ? run(kv4_append_kernel<float, 256>) : run(kv4_append_kernel<__nv_bfloat16, 256>); break;
+        }
     }
     e->launches++;
     MOE_CUDA(cudaGetLastError());

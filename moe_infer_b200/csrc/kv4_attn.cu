@@ -163,7 +163,7 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <class C, typename T>
-__global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : C::NT == 2 ? 168 : 255) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
+__global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_attn_kernel(AttnArgs a, unsigned int* err) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long red[8];
     constexpr int D = C::D, G = C::G, NT = C::NT, ROWS = C::ROWS, NB = C::NB, TILE = C::TILE, TB = C::TB, PB = C::PB, PS = C::PS;
@@ -1019,8 +1019,9 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64
     }
 }
 
-// Rows of the tile: as few columns of eight as hold a sequence's rows, up to four.  Units of their own (no splitting) once
-// they fill the GPU twice over.
+// Rows of the tile: one column of eight where that holds a sequence's rows, two beyond (four columns share the work on a
+// position among more rows, but their 255 registers leave two CTAs to an SM: 162 against 143 us on f32 prompts, 36 against
+// 31 us on four-token verification).  f32 rows in units of their own (no splitting) once those fill the GPU four times over.
 template <int D, typename T>
 static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -1033,9 +1034,8 @@ static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows) {
     };
     constexpr int TB = 4 / (D / 64);
     if constexpr (F32) {
-        if (q_rows > 16 && units(32) >= 2 * e->sm_count) return run_attn<AttnCfg<D, F32, 4, 1, false>, T>(e, a, V0 + 3, units(32), q_rows);
+        if (q_rows > 16 && units(16) >= 4 * e->sm_count) return run_attn<AttnCfg<D, F32, 2, 1, false>, T>(e, a, V0 + 2, units(16), q_rows);
     }
-    if (q_rows > 16) return run_attn<AttnCfg<D, F32, 4, 1, true>, T>(e, a, V0 + 2, units(32), q_rows);
     if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16), q_rows);
     return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8), q_rows);
 }

@@ -309,6 +309,26 @@ def test_append_is_the_codec(eng, dim, rotary, interleaved, dtype):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("dim,kv_heads,rotary,interleaved", [(64, 8, 32, 1), (64, 7, 64, 0), (128, 8, 0, 0), (256, 6, 64, 0), (256, 4, 256, 1)])
+def test_append_many_rows(eng, dim, kv_heads, rotary, interleaved, dtype):
+    """Enough rows for several heads to a CTA; first and last positions inside quads and pages."""
+    c = Case(eng, [1813, 1502], [1810, 1502], kv_heads=kv_heads, dim=dim, page=48, seed=dim + kv_heads)
+    k = as_type(c.rng.standard_normal((c.rows, kv_heads, dim)), dtype)
+    v = as_type(c.rng.standard_normal((c.rows, kv_heads, dim)), dtype)
+    pos = c.rng.integers(0, 4000, c.rows).astype(np.int32)
+    tab = rope_table(rotary, 4000, 1e4, scaling=L.ROPE_NTK, factor=2.0) if rotary else None
+    eng.kv4_append_dev(c.cache, c.batch, c.up(k).ptr, c.up(v).ptr, dtype, rope=RopeTable(c.up(tab).ptr, 4000, rotary, interleaved) if rotary else None,
+                       rope_positions=c.up(pos).ptr if rotary else 0)
+    ko, vo = c.up(np.zeros((c.rows, kv_heads, dim), np.float32)), c.up(np.zeros((c.rows, kv_heads, dim), np.float32))
+    eng.kv4_gather_dev(c.cache, c.batch, ko.ptr, vo.ptr, L.DT_F32)
+    eng.sync()
+    kf, vf = as_f64(k, dtype).astype(np.float32), as_f64(v, dtype).astype(np.float32)
+    np.testing.assert_array_equal(ko.download(np.float32, k.shape), R.codec(R.rotate_f32(kf, tab[pos], interleaved) if rotary else kf))
+    np.testing.assert_array_equal(vo.download(np.float32, k.shape), R.codec(vf))
+    c.free()
+
+
 def test_append_leaves_other_positions(eng):
     c = Case(eng, [40, 21], [3, 2], kv_heads=2, dim=128, page=16, seed=5)
     c.fill()
