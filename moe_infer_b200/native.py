@@ -419,32 +419,42 @@ class NativeEngine:
     def rope_dev(self, rope: RopeTable, x: int, out: int, positions: int, dtype: int, n_tokens: int, heads: int, head_dim: int,
                  x_strides: Optional[Tuple[int, int]] = None, out_strides: Optional[Tuple[int, int]] = None) -> None:
         """Rotates [n_tokens, heads, head_dim]; strides are (token, head) in elements, contiguous by default."""
-        xs = x_strides or (heads * head_dim, head_dim)
-        os_ = out_strides or (heads * head_dim, head_dim)
-        L.check(self.lib.moe_rope_dev(self.h, rope, x, xs[0], xs[1], out, os_[0], os_[1], dtype, n_tokens, heads, head_dim,
-                                      positions))
+        dense = (heads * head_dim, head_dim)
+        xt, xh = x_strides or dense
+        ot, oh = out_strides or dense
+        rc = self.lib.moe_rope_dev(self.h, rope, x, xt, xh, out, ot, oh, dtype, n_tokens, heads, head_dim, positions)
+        if rc:
+            L.check(rc)
 
     def kv4_append_dev(self, cache: Kv4Cache, batch: Kv4Batch, k: int, v: int, dtype: int, *, rope: Optional[RopeTable] = None,
                        rope_positions: int = 0, k_strides: Optional[Tuple[int, int]] = None,
                        v_strides: Optional[Tuple[int, int]] = None) -> None:
         """Stores the batch rows' keys (rotated when rope is given) and values; strides are (token, head) in elements."""
-        dense = (cache.num_kv_heads * cache.head_dim, cache.head_dim)
-        ks, vs = k_strides or dense, v_strides or dense
-        L.check(self.lib.moe_kv4_append_dev(self.h, cache, batch, k, ks[0], ks[1], v, vs[0], vs[1], dtype, rope,
-                                            rope_positions or None))
+        dim = cache.head_dim
+        dense = (cache.num_kv_heads * dim, dim)
+        kt, kh = k_strides or dense
+        vt, vh = v_strides or dense
+        rc = self.lib.moe_kv4_append_dev(self.h, cache, batch, k, kt, kh, v, vt, vh, dtype, rope, rope_positions or None)
+        if rc:
+            L.check(rc)
 
     def kv4_gather_dev(self, cache: Kv4Cache, batch: Kv4Batch, k_out: int, v_out: int, dtype: int) -> None:
         """The batch rows' stored keys and values, [n_tokens, num_kv_heads, head_dim] each."""
-        L.check(self.lib.moe_kv4_gather_dev(self.h, cache, batch, k_out, v_out, dtype))
+        rc = self.lib.moe_kv4_gather_dev(self.h, cache, batch, k_out, v_out, dtype)
+        if rc:
+            L.check(rc)
 
     def kv4_attention_dev(self, cache: Kv4Cache, batch: Kv4Batch, q: int, out: int, dtype: int, heads: int, *, scale: float,
                           window: int = 0, gate: int = 0, q_strides: Optional[Tuple[int, int]] = None,
                           gate_strides: Optional[Tuple[int, int]] = None) -> None:
         """Attention of the batch rows' (rotated) queries [n_tokens, heads, head_dim] over the cache; strides as above."""
-        dense = (heads * cache.head_dim, cache.head_dim)
-        qs, gs = q_strides or dense, gate_strides or dense
-        L.check(self.lib.moe_kv4_attention_dev(self.h, cache, batch, q, qs[0], qs[1], gate or None, gs[0], gs[1], out, dtype,
-                                               heads, scale, window))
+        dim = cache.head_dim
+        dense = (heads * dim, dim)
+        qt, qh = q_strides or dense
+        gt, gh = gate_strides or dense
+        rc = self.lib.moe_kv4_attention_dev(self.h, cache, batch, q, qt, qh, gate or None, gt, gh, out, dtype, heads, scale, window)
+        if rc:
+            L.check(rc)
 
     def telemetry(self) -> dict:
         n = C.c_int(0)
