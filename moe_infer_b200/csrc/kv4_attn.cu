@@ -72,7 +72,7 @@ struct AttnUnit {
 
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (lengths 100 to 16,000: 107 us without, @@ us with).
-constexpr int kUnitCost = 3;
+constexpr int kUnitCost = 2;
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
 template <class C>
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                     for (int uu = 0; uu < U; ++uu) {
                         const int g = it * U + uu;
-                        float acc[NT][4];
+                        float acc[NT][4], acc_lo[C::F32 ? NT : 1][4];  // f32 rows: high and low terms apart, two chains of MMAs at a time
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             uint32_t nb[2][4];
@@ -440,9 +440,13 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                                     const uint8_t* qa = sm + C::OFF_Q + (((g * 4 + j * 2 + v) * NT + nt) * 32 + lane) * C::QW;
                                     if constexpr (C::F32) {
                                         const uint4 qf = *reinterpret_cast<const uint4*>(qa);
-                                        if (j == 0 && v == 0) mma_f16_zero(acc[nt], ka, qf.x, qf.y);
-                                        else mma_f16(acc[nt], ka, qf.x, qf.y);
-                                        mma_f16(acc[nt], ka, qf.z, qf.w);
+                                        if (j == 0 && v == 0) {
+                                            mma_f16_zero(acc[nt], ka, qf.x, qf.y);
+                                            mma_f16_zero(acc_lo[nt], ka, qf.z, qf.w);
+                                        } else {
+                                            mma_f16(acc[nt], ka, qf.x, qf.y);
+                                            mma_f16(acc_lo[nt], ka, qf.z, qf.w);
+                                        }
                                     } else {
                                         const uint2 qf = *reinterpret_cast<const uint2*>(qa);
                                         if (j == 0 && v == 0) mma_f16_zero(acc[nt], ka, qf.x, qf.y);
@@ -461,7 +465,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     const float qs = NT == 1 ? qs_reg[NT == 1 ? g : 0][e] : q_sum[g * ROWS + nt * 8 + 2 * c + e];
-                                    s[tb][nt][2 * k + e] = fmaf(sc, acc[nt][2 * k + e], fmaf(bi, qs, s[tb][nt][2 * k + e]));
+                                    const float dot = C::F32 ? acc[nt][2 * k + e] + acc_lo[C::F32 ? nt : 0][2 * k + e] : acc[nt][2 * k + e];
+                                    s[tb][nt][2 * k + e] = fmaf(sc, dot, fmaf(bi, qs, s[tb][nt][2 * k + e]));
                                 }
                         }
                     }
