@@ -311,8 +311,9 @@ int moe_model_state_host(moe_engine_t* e, int32_t layer, int32_t which, float* h
 int moe_model_set_pos(moe_engine_t* e, int64_t pos);
 
 /* ── rotary positions ────────────────────────────────────────────────────────
- * apply_rotary_emb (src/math_util.rs:136-168) as an operator of its own: half and interleaved layouts, part of the head,
- * scaled for contexts longer than the trained one.  Pair i of a head's first rotary_dim elements turns by position *
+ * apply_rope (src/engine/qwen35_moe/mtp.rs:285-303: interleaved pairs) and the rotation inside q_head_norm_rope /
+ * k_head_norm_rope (src/math_util.rs:501-597: half layout) as an operator of its own: part of the head, scaled for contexts
+ * longer than the trained one.  Pair i of a head's first rotary_dim elements turns by position *
  * theta^(-2i / rotary_dim).  Angles are formed in 64 bits on the host:
  * moe_rope_table_host fills f32 [n_positions, rotary_dim]: cosines, then sines, of positions first_position ...  Scalings:
  *   MOE_ROPE_LINEAR  every frequency divided by factor
@@ -365,8 +366,12 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        h / (num_heads / num_kv_heads); scale multiplies the scores.  With gate the result is multiplied by
  *                        sigmoid(gate) (the output gate of the full-attention layers, src/engine/qwen35_moe/cpu.rs:218-347).
  *                        out is [n_tokens, num_heads, head_dim] of the queries' type, contiguous; it must not overlap them.
- *                        bf16 rows: products of f16 operands exact to 11 bits, sums and softmax in f32; f32 rows: operands
- *                        split in two, f32 results to about 2^-21.
+ *                        f32 rows: operands in two f16 terms, results to about 2^-21; bf16 rows: weights rounded to f16
+ *                        (2^-12), and for sequences of at least 128 rows x query heads per KV head (prompts) keys and values
+ *                        too; scores, sums and the softmax f32.  A row that sees a value stored as NaN is NaN in that group of
+ *                        64 (in a prompt, in the whole row).  Prompts of bf16 rows need a work area, the positions they see as
+ *                        f16 (4 head_dim bytes per position and KV head), grown on demand and kept by the engine; calls whose
+ *                        bounds could need more than 4 GB of it run without, more slowly.
  * head_dim is 64, 128 or 256; page_size a multiple of 16. */
 typedef struct {
     void* pages;           /* device, [num_pages, moe_kv4_page_bytes] */
