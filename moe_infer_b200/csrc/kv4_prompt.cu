@@ -176,6 +176,13 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const float (&v)[3
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// A wait ran out: reported; copies and MMAs in flight get some 10 ms to end before the CTA's memory is given back.
+__device__ __noinline__ void give_up(unsigned int* err) {
+    atomicExch(err, 1u);
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles / 100) {}
+}
+
 template <int D>
 __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_per_seq, const uint8_t* image, const int* meta, unsigned int* err) {
     using C = PtCfg<D>;
@@ -248,7 +255,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 if (!(ok = mbar_wait(pv_done, i & 1))) break;
                 load(i + 1, 1);
             }
-            if (!ok) atomicExch(err, 1u);
+            if (!ok) give_up(err);
         }
     } else if (warp == 9) {
         // ── MMAs ──
@@ -280,7 +287,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                                    umma::make_desc_sw128_kmajor(smem_u32(sm + C::OFF_V + (k >> 2) * (D * 128) + (k & 3) * 32)), id_pv, (i > 0 || k > 0));
                 umma::commit(pv_done);
             }
-            if (!ok) atomicExch(err, 1u);
+            if (!ok) give_up(err);
         }
     } else {
         // ── two threads per row: positions 64 half .. 64 half + 63 of a tile, elements half * D / 2 .. of O ──
