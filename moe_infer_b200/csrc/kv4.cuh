@@ -6,7 +6,7 @@
 // Every 64 elements of a key or value share one (scale, bias) pair, both bf16, value = nibble * scale + bias: the codec
 // of the 4-bit weights (moe_pack_int4_*), bit for bit.  A pair is one 32-bit word (scale low), stored [group][position].
 //
-// The nibbles lie in the order in which a warp feeds them to mma.m16n8k16 as its B operand, so that one 16-byte load per
+// The nibbles lie in the order in which a warp feeds them to mma.m16n8k16, so that one 16-byte load per
 // lane (512 contiguous bytes per warp, no bank conflicts, no shuffles) covers two 64-element groups of 8 keys, or one
 // group of the values of 16 positions:
 //   K: position t of the block sits in row (t % 2) * 8 + t / 2; the row's 64-byte segment of two groups is

@@ -2,15 +2,15 @@
 //
 //   o[j, h] = sum_t softmax_t(scale q[j, h] . k_t) v_t   over the positions t that row j sees.
 //
-// The nibbles go to the tensor cores as they are: n - 8 (or 7) is exact in f16, so with
+// The nibbles go to the tensor cores as they are: as a bit pattern, n is the f16 subnormal n 2^-24, exactly.  With
 // k_t = s n + b (per 64 elements, group g)
-//   q . k_t = sum_g  s[t, g] (q_g . (n - 8)) + (b + 8 s)[t, g] sum(q_g)
-//   o_g     = sum_t (w_t s[t, g]) (n - 8)    + sum_t w_t (b + 8 s)[t, g]
-// which leaves one scale per score and group instead of one per element, and no rounding of keys or values.  Keys and
-// values are the A operand of mma.m16n8k16 (16 positions, 16 elements), eight query rows the columns: the eight query
-// heads of a KV head fill it.  Queries and weights are f16 operands scaled by powers of two; for f32 rows they are split
-// into a high and a low f16 term (22 bits) that two MMAs add into the same sums, for bf16 rows one term is exact (queries)
-// or three bits finer than the result's type (weights).  Sums and the softmax are f32.
+//   q . k_t = sum_g  s[t, g] (q_g . n) + b[t, g] sum(q_g)
+//   o_g     = sum_t (w_t s[t, g]) n    + sum_t w_t b[t, g]
+// (every other pair of values as b + 15 s - s (15 - n)), which leaves one scale per score and group instead of one per element,
+// and no rounding of keys or values.  Keys and values are the A operand of mma.m16n8k16 (16 positions, 16 elements), eight
+// query rows the columns: the eight query heads of a KV head fill it.  Queries and weights are f16 operands scaled by powers
+// of two; for f32 rows they are split into a high and a low f16 term (22 bits) that two MMAs add into the same sums, for bf16
+// rows one term is exact (queries) or three bits finer than the result's type (weights).  Sums and the softmax are f32.
 //
 // Weights are w = exp2(x - ref), one reference per row: it moves only when a weight times its scale would leave f16's
 // range, then to 2^8 below that; a row's result does not depend on it otherwise.
@@ -24,8 +24,8 @@
 // sequences of any lengths balance; units that cross CTAs leave partial sums that a second kernel joins.  Many rows
 // (f32 prompts; bf16 ones have kv4_prompt.cu): one CTA per unit over the positions its rows see, nothing to join.
 //
-// Bound by issue slots: about 900 instructions per 16 positions and head of 256, 360 of them integer (nibbles to f16), 57 % of
-// the slots used at four CTAs per SM; 250,001 positions of two heads, f32, eight query heads each: 57.6 us, 2.5 TB/s.
+// Bound by issue slots and dependent instructions: about 850 instructions per 16 positions and head of 256, 54 % of the slots
+// used at four CTAs per SM (barrier and MMA latency take the rest); 250,001 positions of two heads, f32, eight query heads each: 57.3 us, 2.5 TB/s.
 #include <math.h>
 
 #include <type_traits>
@@ -75,7 +75,7 @@ struct AttnUnit {
 
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (48 sequences of 100 to 16,000 positions, when a tile took a third
-// longer than now: 110 us without, 76 with 3; now 63 us with 3, 61 with 2).
+// longer than later: 110 us without, 76 with 3; then 63 us with 3, 61 with 2).
 constexpr int kUnitCost = 2;
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
@@ -163,6 +163,29 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// The eight nibbles of a word as four pairs of f16 subnormals: the pattern n is n 2^-24, n << 4 is 16 n 2^-24, both exact.
+// bf16 rows: where the nibbles lie, a mask per pair (words 1 and 3 count 16 times: the other operand or the sum makes up for
+// it).  The tensor core aligns products by their exponents, and a subnormal's is that of 2^-14, so n << 4 keeps four more bits
+// of a sum: kWide (f32 rows) moves all of them there.  Measured (250,001 positions, f32): 54.3 us and 6.5e-6 off where they
+// lie, 57.3 us and 9.6e-7 wide, 57.5 us and 6.0e-7 with n - 8 made a normal number (two instructions more per pair); the ragged
+// bf16 batch 61.1 us with n - 8, 57.4 now.  kFlip: words 2 and 3 hold 15 - n.
+constexpr float kSub = 16777216.0f;  // 2^24
+template <bool kWide, bool kFlip = false>
+__device__ __forceinline__ void nibbles_sub(uint32_t w, uint32_t (&o)[4]) {
+    if constexpr (kWide) {
+        const uint32_t wl = w << 4, wr = w >> 4, w8 = w >> 8;
+        o[0] = wl & 0x00F000F0u;
+        o[1] = w & 0x00F000F0u;
+        o[2] = (kFlip ? ~wr : wr) & 0x00F000F0u;
+        o[3] = (kFlip ? ~w8 : w8) & 0x00F000F0u;
+        return;
+    }
+    const uint32_t w8 = w >> 8;
+    o[0] = w & 0x000F000Fu;
+    o[1] = w & 0x00F000F0u;
+    o[2] = (kFlip ? ~w8 : w8) & 0x000F000Fu;
+    o[3] = (kFlip ? ~w8 : w8) & 0x00F000F0u;
 }
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -337,12 +360,13 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                 float sum = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float v0 = x[k] * up, v1 = x[k + 4] * up;
+                    const float sh = !C::F32 && (k & 1) ? 0.0625f : 1.0f;  // odd words of nibbles_sub count 16 times
+                    const float v0 = x[k] * up * sh, v1 = x[k + 4] * up * sh;
                     const __half2 h = __floats2half2_rn(v0, v1);
                     const float2 f = __half22float2(h);
                     hi[k] = h2_bits(h);
                     lo[k] = h2_bits(__floats2half2_rn(v0 - f.x, v1 - f.y));
-                    sum += C::F32 ? v0 + v1 : f.x + f.y;
+                    sum = fmaf(C::F32 ? v0 + v1 : f.x + f.y, !C::F32 && (k & 1) ? 16.0f : 1.0f, sum);
                 }
 #pragma unroll
                 for (int k = 1; k < 8; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);  // over the group of 64
@@ -434,8 +458,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             uint32_t nb[2][4];
-                            nibbles_h2(kw[0][uu * 2 + j], nb[0]);
-                            nibbles_h2(kw[1][uu * 2 + j], nb[1]);
+                            nibbles_sub<C::F32>(kw[0][uu * 2 + j], nb[0]);
+                            nibbles_sub<C::F32>(kw[1][uu * 2 + j], nb[1]);
 #pragma unroll
                             for (int v = 0; v < 2; ++v) {
                                 const uint4 ka = make_uint4(nb[0][2 * v], nb[1][2 * v], nb[0][2 * v + 1], nb[1][2 * v + 1]);
@@ -463,7 +487,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                         const uint32_t pw[2] = {pr.x, pr.y};
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const float sc = __uint_as_float(pw[k] << 16), bi = fmaf(8.0f, sc, __uint_as_float(pw[k] & 0xFFFF0000u));
+                            const float sc = __uint_as_float(pw[k] << 16) * (C::F32 ? kSub / 16.0f : kSub), bi = __uint_as_float(pw[k] & 0xFFFF0000u);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -615,10 +639,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                 for (int e = 0; e < 2; ++e) l_run[nt][e] += sum[nt][e];
             float acc[C::F32 ? NT : 1][4][4];  // f32 rows: the tile's sums, added to the unit's with f32 rounding
-            // mid: n - 8 and n - 7 in turn, so that the sums of the nibbles, whose middle is 7.5, have no drift: the tensor core's
-            // truncating sums then stay relative to what they hold (f32 rows over 250,001 positions: 9e-7 off, 1.5e-5 with n - 8 alone)
-            auto block_of_values = [&](int pb, auto slow, auto first, auto mid) {
-                constexpr int kMid = decltype(mid)::value;
+            // positions 1 and 3 of four: 15 - n under a negative weight, so that the sums of the nibbles, whose middle is 7.5, have
+            // no drift: the tensor core's truncating sums then stay relative to what they hold (f32 rows over 250,001 positions:
+            // 9.6e-7 off; 1.5e-5 with n - 8 at every position)
+            auto block_of_values = [&](int pb, auto slow, auto first) {
                 const int blk = tp * PB + pb;
                 const uint8_t* vb = st + blk * C::BLK + 9 * D;
                 const uint4 vw = *reinterpret_cast<const uint4*>(vb + g_own * 512 + lane * 16);
@@ -633,13 +657,17 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     sc[k] = __uint_as_float(pw[k] << 16);
-                    bi[k] = fmaf((float)kMid, sc[k], __uint_as_float(pw[k] & 0xFFFF0000u));
+                    bi[k] = __uint_as_float(pw[k] & 0xFFFF0000u);
+                    if (k & 1) {
+                        bi[k] = fmaf(15.0f, sc[k], bi[k]);
+                        sc[k] = -sc[k];
+                    }
                 }
                 uint32_t nb[4][4];  // word x: elements 8 r + 2 x, 8 r + 2 x + 1 of positions (0, 2), then of (1, 3)
-                nibbles_h2<kMid>(vw.x, nb[0]);
-                nibbles_h2<kMid>(vw.y, nb[1]);
-                nibbles_h2<kMid>(vw.z, nb[2]);
-                nibbles_h2<kMid>(vw.w, nb[3]);
+                nibbles_sub<C::F32, true>(vw.x, nb[0]);
+                nibbles_sub<C::F32, true>(vw.y, nb[1]);
+                nibbles_sub<C::F32, true>(vw.z, nb[2]);
+                nibbles_sub<C::F32, true>(vw.w, nb[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float4 p = *reinterpret_cast<const float4*>(sm + C::OFF_P + buf * C::P_BYTES + ((blk * ROWS + nt * 8 + r) * PS + 4 * c) * 4);
@@ -674,19 +702,17 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             };
             using Yes = std::true_type;
             using No = std::false_type;
-            using M8 = std::integral_constant<int, 8>;
-            using M7 = std::integral_constant<int, 7>;
             if ((any & (kFlagNan | kFlagTail)) == 0) {
-                block_of_values(0, No{}, Yes{}, M8{});
-                if constexpr (PB > 1) block_of_values(1, No{}, No{}, M7{});
+                block_of_values(0, No{}, Yes{});
+                if constexpr (PB > 1) block_of_values(1, No{}, No{});
                 if constexpr (PB > 2) {
-                    block_of_values(2, No{}, No{}, M8{});
-                    block_of_values(3, No{}, No{}, M7{});
+                    block_of_values(2, No{}, No{});
+                    block_of_values(3, No{}, No{});
                 }
             } else {
-                block_of_values(0, Yes{}, Yes{}, M8{});
+                block_of_values(0, Yes{}, Yes{});
 #pragma unroll 1
-                for (int pb = 1; pb < PB; ++pb) block_of_values(pb, Yes{}, No{}, M7{});
+                for (int pb = 1; pb < PB; ++pb) block_of_values(pb, Yes{}, No{});
             }
             if constexpr (C::F32) {
 #pragma unroll
@@ -718,10 +744,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             const float b0 = __shfl_sync(0xffffffffu, ob, 8 * c), b1 = __shfl_sync(0xffffffffu, ob, 8 * c + 4);  // of rows 2 c, 2 c + 1
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                o[nt][x][0] += b0;
-                o[nt][x][1] += b1;
-                o[nt][x][2] += b0;
-                o[nt][x][3] += b1;
+                o[nt][x][0] = fmaf(o[nt][x][0], C::F32 ? kSub / 16.0f : kSub, b0);
+                o[nt][x][1] = fmaf(o[nt][x][1], C::F32 ? kSub / 16.0f : kSub, b1);
+                o[nt][x][2] = fmaf(o[nt][x][2], kSub / 16.0f, b0);
+                o[nt][x][3] = fmaf(o[nt][x][3], kSub / 16.0f, b1);
             }
         }
         const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles + kUnitCost <= w_end;

@@ -111,13 +111,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t m, uint32_t c) {
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(m), "r"(c));
     return d;
 }
-// four nibble pairs of a word as f16 pairs of n - 8 (or 7): word bits {0-3, 16-19}, {4-7, 20-23}, {8-11, 24-27}, {12-15, 28-31}.
+// four nibble pairs of a word as f16 pairs of n - 8: word bits {0-3, 16-19}, {4-7, 20-23}, {8-11, 24-27}, {12-15, 28-31}.
 // 0x6400 | n is the f16 number 1024 + n, 0x6400 | n << 4 is 1024 + 16 n; both subtractions are exact.
-template <int kMid = 8>
 __device__ __forceinline__ void nibbles_h2(uint32_t w, uint32_t (&o)[4]) {
-    static_assert(kMid == 7 || kMid == 8, "");
-    const __half2 m1032 = bits_h2(kMid == 8 ? 0xE408E408u : 0xE407E407u), sixteenth = bits_h2(0x2C002C00u),
-                  m72 = bits_h2(kMid == 8 ? 0xD480D480u : 0xD470D470u);  // -1024 - kMid, -64 - kMid
+    const __half2 m1032 = bits_h2(0xE408E408u), sixteenth = bits_h2(0x2C002C00u), m72 = bits_h2(0xD480D480u);  // -1032, 1 / 16, -72
     const uint32_t w8 = w >> 8;
     o[0] = h2_bits(__hadd2(bits_h2(and_or(w, 0x000F000Fu, 0x64006400u)), m1032));
     o[1] = h2_bits(__hfma2(bits_h2(and_or(w, 0x00F000F0u, 0x64006400u)), sixteenth, m72));
