@@ -75,7 +75,7 @@ struct AttnUnit {
 
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (48 sequences of 100 to 16,000 positions, when a tile took a third
-// longer than later: 110 us without, 76 with 3; then 63 us with 3, 61 with 2).
+// longer than now: 110 us without, 76 with 3; now 58.2 us with 1, 57.4 with 2, 59.4 with 3).
 constexpr int kUnitCost = 2;
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).

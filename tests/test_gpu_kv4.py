@@ -80,15 +80,17 @@ def as_f64(x, dtype):
     return x.astype(np.float64) if dtype == L.DT_F32 else R.from_bf16(x).astype(np.float64)
 
 
-# A result may be off by what its weights are off and by its own rounding.  v = s (n - 8) + (b + 8 s), and the two parts are
-# summed apart: the first with the weights as MMA operands, the second with the weights before that rounding.  An error of a
-# weight as an operand is therefore relative to s |n - 8| <= 8 s, any other error of a weight to |v|: both are covered by the
-# weighted sum of |v| + 8 s ("size"); a group holds a 0 and a 15, so 8 s is 8 / 15 of its range.
+# A result may be off by what its weights are off and by its own rounding.  v = s n + b (or b + 15 s - s (15 - n)), and the two
+# parts are summed apart: the first with the weights as MMA operands, the second with the weights before that rounding.  An
+# error of a weight as an operand is therefore relative to at most 15 s, less than twice 8 s, any other error of a weight to |v|:
+# both are covered by the weighted sum of |v| + 8 s ("size"), the first counted twice; a group holds a 0 and a 15, so 8 s is
+# 8 / 15 of its range.
 # A weight is off by twice (numerator and sum) the error of its score: operands of 22 bits (half a step 2^-23) and f32
-# roundings of the sums over groups, which the centred nibbles keep within twice scale * sum |q k| ("reach"): 2^-22 of it
-# in all for f32 rows, hence 2^-21 reach; then the 2-ulp exponential, the weight as an operand and the f32 sums of the value
-# pass: 2^-19 for f32 rows (22-bit weights), 2^-11 for bf16 rows (11-bit weights: half a step 2^-12, numerator against the
-# unrounded sum), and half a step of bf16, 2^-8 of its value at most, for their result.
+# roundings of the sums over groups, which the nibbles (s n is at most a group's range) keep within a few times
+# scale * sum |q k| ("reach"): 2^-22 of it in all for f32 rows, hence 2^-21 reach; then the 2-ulp exponential, the weight as
+# an operand and the sums of the value pass, whose products an MMA cuts some 2^-22 below its largest, with both signs: 2^-19 for
+# f32 rows (22-bit weights); 2^-11 and 2^-12 for bf16 rows (11-bit weights: half a step 2^-12, counted twice, the numerator
+# against the unrounded sum), and half a step of bf16, 2^-8 of its value at most, for their result.
 # Prompts of bf16 rows also hold keys and values as f16 (11 bits: half a step 2^-12 of a value, and of a key's elements, so
 # 2^-12 reach in a score, twice that in a weight).
 def bound_of(dtype, want, size, reach):
