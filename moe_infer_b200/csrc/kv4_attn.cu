@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
         nx_block = -1;
         const int pos = n.t_lo + t * TILE + lane * a.run * kKv4Block;
         if (lane * a.run < NB && pos < n.len) {
-            const int pg = pos / a.cache.page_size;
-            nx_block = (pos - pg * a.cache.page_size) / kKv4Block;
+            const int pg = over_group(pos, a.by_page);
+            nx_block = (int)((unsigned)(pos - pg * a.cache.page_size) / kKv4Block);
             nx_page = -1;
             if (pg < a.seqs.max_pages) nx_page = a.seqs.page_table[(size_t)n.b * a.seqs.max_pages + pg];
         }
@@ -1149,6 +1149,7 @@ extern "C" int moe_kv4_attention_dev(moe_engine_t* e, const moe_kv4_cache_t* cac
     a.heads = num_heads;
     a.group = num_heads / cache->num_kv_heads;
     a.by_group = make_group_div((uint32_t)a.group);
+    a.by_page = make_group_div((uint32_t)a.cache.page_size);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.window = window;
     a.hi_rows = 0x7FFFFFFF;

@@ -25,7 +25,7 @@ struct AttnArgs {
     int64_t qt, qh, gt, gh;  // element strides
     int vec_q, vec_gate;     // rows readable 16 bytes at a time
     int heads, group;        // query heads; query heads per KV head
-    GroupDiv by_group;
+    GroupDiv by_group, by_page;  // divisions of rows by heads that share a KV head, of positions by a page's
     float scale_log2;        // scale * log2(e)
     int window;              // 0: none
     int lo_rows, hi_rows;    // sequences with lo_rows <= rows < hi_rows (rows x query heads per KV head) are this launch's
