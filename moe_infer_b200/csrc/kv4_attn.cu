@@ -25,7 +25,7 @@
 // (f32 prompts; bf16 ones have kv4_prompt.cu): one CTA per unit over the positions its rows see, nothing to join.
 //
 // Bound by issue slots and dependent instructions: about 850 instructions per 16 positions and head of 256, 54 % of the slots
-// used at four CTAs per SM (barrier and MMA latency take the rest); 250,001 positions of two heads, f32, eight query heads each: 57.3 us, 2.5 TB/s.
+// used at four CTAs per SM (barrier and MMA latency take the rest); 250,001 positions of two heads, f32, eight query heads each: 55.6 us, 2.6 TB/s.
 #include <math.h>
 
 #include <type_traits>
@@ -75,7 +75,7 @@ struct AttnUnit {
 
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
 // CTA that got many short sequences would finish last (48 sequences of 100 to 16,000 positions, when a tile took a third
-// longer than now: 110 us without, 76 with 3; now 58.2 us with 1, 57.4 with 2, 59.4 with 3).
+// longer: 110 us without, 76 with 3; later 58.2 us with 1, 57.4 with 2, 59.4 with 3).
 constexpr int kUnitCost = 2;
 
 // Row tiles of a sequence and tiles of each (SPLIT: every row tile of a sequence counts the same positions).
@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 
     // The first warp also brings the tiles in, one ahead: a tile's place is free once all warps have met at the barrier of the
     // tile after it.  Blocks that lie in one page are one copy (a.run of them: a power of two that divides a page's blocks and
-    // a tile's).  The pages are looked up another tile before, so that the table's latency is not waited for.
+    // a tile's).  The pages are looked up another tile before, so that the table's latency is not waited for; the
+    // others wait for this warp, so a position's page is found without a division (57.3 us with it on one long sequence, 55.9).
     int nx_page = 0, nx_block = -1;  // lane: page and first block of its run in the tile to copy next; block -1: none
     auto look_up = [&](const AttnUnit& n, int t) {
         nx_block = -1;
@@ -272,6 +273,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             if (pg < a.seqs.max_pages) nx_page = a.seqs.page_table[(size_t)n.b * a.seqs.max_pages + pg];
         }
     };
+    const unsigned page_blocks = (unsigned)a.cache.page_size / kKv4Block;  // a block's number fits 32 bits: 2^32 blocks are 4.9 TB
     auto copy_in = [&](int h, int st) {
         bool copy = nx_block >= 0;
         if (copy && (nx_page < 0 || nx_page >= a.cache.num_pages)) {
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
         __syncwarp();
         if (copy)
             bulk_g2s(sm + st * C::STAGE + lane * a.run * C::BLK,
-                     a.cache.pages + (((size_t)nx_page * a.cache.kv_heads + h) * (a.cache.page_size / kKv4Block) + nx_block) * C::BLK,
+                     a.cache.pages + (size_t)(((unsigned)nx_page * a.cache.kv_heads + h) * page_blocks + nx_block) * C::BLK,
                      a.run * C::BLK, full + st);
     };
     auto first_of = [&](long long at) { return (int)max(w_begin - at - kUnitCost, 0ll); };
