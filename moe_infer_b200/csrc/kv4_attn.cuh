@@ -30,6 +30,7 @@ struct AttnArgs {
     int window;              // 0: none
     int lo_rows, hi_rows;    // sequences with lo_rows <= rows < hi_rows (rows x query heads per KV head) are this launch's
     int run;                 // blocks of a tile that one copy brings (they lie in one page)
+    int image_seqs;          // prompts: sequences the expanded tiles have room for
     float* part;             // work area of the call
 };
 

@@ -63,6 +63,10 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     if (ti >= n || ti >= tiles_per_seq) return;  // (a sequence without rows here has no tiles)
     int before = 0;                              // sequences with rows before this one
     for (int b0 = 0; b0 < b; b0 += 256) before += __syncthreads_count(b0 + tid < b && attn_seq(a, b0 + tid, err).q_len > 0);
+    if (before >= a.image_seqs) {                // sequences that share rows: each is in bounds, together they are more than n_tokens
+        if (tid == 0) atomicExch(err, kErrKv4Batch);
+        return;
+    }
     const int p0 = (tile0 + ti) * kPtTile;
     if (tid < 8) blocks[tid] = p0 + tid * 16 < s.len ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
     if (tid < 4) nan_bits[tid] = 0;
@@ -202,6 +206,10 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
     const RowTile where = locate_row_tile(a, blockIdx.x / a.cache.kv_heads, kPtTile, 320, reinterpret_cast<long long*>(sm + C::OFF_TOP), err);
     const int b = where.b;
     if (b >= a.seqs.n_seqs) return;
+    if (where.before >= a.image_seqs) {  // as above: nothing was expanded for it
+        if (tid == 0) atomicExch(err, kErrKv4Batch);
+        return;
+    }
     const Kv4Seq s = kv4_seq(a.seqs, b, err);
     const int rt = where.rts - 1 - where.rt, rows_all = s.q_len * a.group, pos_base = s.len - s.q_len;
     int seq_t0, seq_n;
@@ -534,6 +542,7 @@ int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
     const size_t image = pt_image_bytes<D>(a), meta = (size_t)pt_max_seqs(a) * a.cache.kv_heads * tiles * kPtMeta * 4;
     a.lo_rows = a.seqs.n_seqs == 1 ? 1 : kPromptRows;
     a.hi_rows = 0x7FFFFFFF;
+    a.image_seqs = (int)pt_max_seqs(a);
     int rc = kv4_reserve(e, image + meta);
     if (rc) return rc;
     uint8_t* img = reinterpret_cast<uint8_t*>(e->kv4.work);
