@@ -292,20 +292,34 @@ def prepare(case, seed):
 
 
 # ─── the framework's calls ──────────────────────────────────────────────────
-_engine = None
+_engine = _stream = _made = _done = None
 
 
 def _eng():
-    global _engine
+    global _engine, _stream, _made, _done
     if _engine is None:
         from moe_infer_b200.native import Dims, NativeEngine
         _engine = NativeEngine(Dims(num_experts=4, top_k=4, num_layers=1))
+        _stream = torch.cuda.ExternalStream(_engine.stream())
+        _made, _done = torch.cuda.Event(), torch.cuda.Event()
     return _engine
 
 
 def _run_own(st):
+    """The engine has a stream of its own: it waits for what torch's stream has made of the inputs (and for earlier users of the
+    outputs' memory), and torch's stream waits for the results."""
+    eng, mine = _eng(), torch.cuda.current_stream()
+    _made.record(mine)
+    _stream.wait_event(_made)
+    out = _calls(st, eng)
+    _done.record(_stream)
+    mine.wait_event(_done)
+    return out
+
+
+def _calls(st, eng):
     from moe_infer_b200.native import Kv4Batch, Kv4Cache, RopeTable
-    case, eng = st["case"], _eng()
+    case = st["case"]
     dtype = 0 if case["dtype"] == "f32" else 1  # MOE_DT_F32, MOE_DT_BF16
     if case["op"] == "rope":
         x, d = st["x"], case["dim"]
