@@ -12,8 +12,10 @@
 // of two; for f32 rows they are split into a high and a low f16 term (22 bits) that two MMAs add into the same sums, for bf16
 // rows one term is exact (queries) or three bits finer than the result's type (weights).  Sums and the softmax are f32.
 //
-// Weights are w = exp2(x - ref), one reference per row: it moves only when a weight times its scale would leave f16's
-// range, then to 2^8 below that; a row's result does not depend on it otherwise.
+// Weights are w = exp2(x - ref), one reference per row, a whole number: it moves only when a score passes it, then to 2^8
+// above.  As operands the products w s are scaled by a power of two, one per row and group, that moves only when a
+// product would leave f16's range: a group's bits depend on the products that the row sees in that group, not on other groups
+// or on positions hidden from it.
 //
 // A work unit is (sequence, KV head, row tile): `rows` query rows of the heads that share a KV head against its positions,
 // 64 * TB at a time.  The tiles' blocks come in by bulk copies (as many blocks at once as lie in one page, so pages may end
@@ -31,6 +33,7 @@
 #include <type_traits>
 
 #include "kv4_attn.cuh"
+#include "umma.cuh"
 
 namespace moe {
 
@@ -63,8 +66,9 @@ struct AttnCfg {
     static constexpr int OFF_BAR = (OFF_L + 4 * ROWS * 4 + 15) / 16 * 16;
     static constexpr int SMEM = OFF_BAR + STAGES * 8 + 16;
 };
-constexpr float kWeightTop = 14.0f, kWeightSet = 6.0f;  // log2 of weight * scale: at most, and where a new reference puts the largest
-constexpr unsigned kFlagMoved = 1u, kFlagNan = 2u, kFlagTail = 4u;
+constexpr float kRefAbove = 8.0f;    // a new reference lies this far above the row's largest score (weights stay at most 1)
+constexpr float kProdTop = 32768.0f; // weight * scale * power of two: at most this,
+constexpr int kProdSet = 7;          // and log2 of where a new power puts the largest
 
 // A unit of work and the tiles of it that exist.
 struct AttnUnit {
@@ -187,6 +191,13 @@ __device__ __forceinline__ void nibbles_sub(uint32_t w, uint32_t (&o)[4]) {
     o[2] = (kFlip ? ~w8 : w8) & 0x000F000Fu;
     o[3] = (kFlip ? ~w8 : w8) & 0x00F000F0u;
 }
+// the largest; NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }  // of a positive number (-127 below 2^-126)
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <class C, typename T>
@@ -390,9 +401,11 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
         int see_hi[NT][2], see_lo[NT][2];  // positions the row sees: see_lo <= t <= see_hi
         int all_hi = 0x7FFFFFFF, all_lo = -1;
         float o[NT][4][4], o_bias[NT];     // elements 8 r + 2 x and + 1 of the group, rows 2 c and 2 c + 1; row r
+        float power[NT];                   // row r: its products are taken times this power of two, o with them
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             o_bias[nt] = 0.0f;
+            power[nt] = pow2f(126);        // the first product lowers it
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 ref[nt][e] = -INFINITY;
@@ -423,6 +436,20 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                 qs_reg[g][1] = q_sum[g * ROWS + 2 * c + 1];
             }
         }
+
+        // row r's products times 2^k from now on, its sums so far times 2^by (not above 1)
+        auto set_power = [&](int nt, int k, int by) {
+            power[nt] = pow2f(k);
+            const float f = pow2f(max(by, -126));
+            const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);  // of rows 2 c, 2 c + 1
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                o[nt][x][0] *= f0;
+                o[nt][x][1] *= f1;
+                o[nt][x][2] *= f0;
+                o[nt][x][3] *= f1;
+            }
+        };
 
         int buf = 0;
         for (int ti = t_first; ti < t_stop; ++ti, buf ^= 1) {
@@ -502,33 +529,6 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                     }
                 }
             }
-            // the largest scale of each block's values (NaN, as a bit pattern, above every number)
-            const bool tail = t0 + TILE > u.len;
-            unsigned my_flags = tail ? kFlagTail : 0u;
-            float ev[TB];
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb) {
-                const int blk = warp * TB + tb, t = lane & 15;
-                const uint8_t* vp = st + blk * C::BLK + 17 * D + t * 4;
-                const bool in = !tail || t0 + blk * kKv4Block + t < u.len;
-                // a lane's pairs: of one position, every other group
-                uint32_t x[(G + 1) / 2], m = 0;
-#pragma unroll
-                for (int i = 0; i < (G + 1) / 2; ++i) {
-                    x[i] = *reinterpret_cast<const uint32_t*>(vp + (G == 1 ? 0 : 2 * i + (lane >> 4)) * 64) << 16;
-                    if (!in) x[i] = 0;
-                    m = max(m, x[i]);
-                }
-                m = __reduce_max_sync(0xffffffffu, m);
-                if (m >= 0x7F800000u) {
-                    my_flags |= kFlagNan;
-                    m = 0;
-#pragma unroll
-                    for (int i = 0; i < (G + 1) / 2; ++i) m = max(m, x[i] < 0x7F800000u ? x[i] : 0u);
-                    m = __reduce_max_sync(0xffffffffu, m);
-                }
-                ev[tb] = (float)(max((int)(m >> 23) - 126, -100));  // scales below 2^ev
-            }
             // weights
             const bool whole = t0 + TILE - 1 <= all_hi && t0 >= all_lo;
             float use[NT][2], sum[NT][2];
@@ -553,9 +553,9 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    use[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]) + ev[0];
+                    use[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-                    for (int tb = 1; tb < TB; ++tb) use[nt][e] = fmaxf(use[nt][e], fmaxf(s[tb][nt][e], s[tb][nt][2 + e]) + ev[tb]);
+                    for (int tb = 1; tb < TB; ++tb) use[nt][e] = fmaxf(use[nt][e], fmaxf(s[tb][nt][e], s[tb][nt][2 + e]));
                 }
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1)
@@ -568,9 +568,9 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const bool mv = use[nt][e] > ref[nt][e] + kWeightTop;
+                    const bool mv = use[nt][e] > ref[nt][e];
                     moved |= mv;
-                    use[nt][e] = mv ? use[nt][e] - kWeightSet : ref[nt][e];
+                    use[nt][e] = mv ? ceilf(use[nt][e]) + kRefAbove : ref[nt][e];
                     const float off = use[nt][e] == -INFINITY ? 0.0f : use[nt][e];
                     sum[nt][e] = 0.0f;
 #pragma unroll
@@ -582,13 +582,13 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                             make_float2(s[tb][nt][e], s[tb][nt][2 + e]);
                     }
                 }
-            if (__any_sync(0xffffffffu, moved)) my_flags |= kFlagMoved;
+            moved = __any_sync(0xffffffffu, moved);
             if (r == 0) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     *reinterpret_cast<float2*>(refs + (buf * 4 + warp) * ROWS + nt * 8 + 2 * c) = make_float2(use[nt][0], use[nt][1]);
             }
-            if (lane == 0) flags[buf * 4 + warp] = my_flags;
+            if (lane == 0) flags[buf * 4 + warp] = moved;
             compute_barrier();
             if (*(volatile int*)abort_flag) ok = false;
             if (warp == 0 && ok) {
@@ -601,12 +601,12 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             }
             // ── values ──
             const uint4 fl = *reinterpret_cast<const uint4*>(flags + buf * 4);
-            const unsigned any = fl.x | fl.y | fl.z | fl.w;
-            if (any & kFlagMoved) {
+            const bool any_moved = (fl.x | fl.y | fl.z | fl.w) != 0;
+            if (any_moved) {
                 // rare: the rows' references become the largest of the warps'; every warp corrects the weights it wrote
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float fix[2];
+                    float fix[2], up[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int row = nt * 8 + 2 * c + e;
@@ -615,6 +615,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                         for (int i = 0; i < 4; ++i) m = fmaxf(m, refs[(buf * 4 + i) * ROWS + row]);
                         const float off = m == -INFINITY ? 0.0f : m, f = exp2_approx(use[nt][e] - off);
                         fix[e] = exp2_approx(ref[nt][e] - off);
+                        up[e] = m > ref[nt][e] ? m - ref[nt][e] : 0.0f;  // infinite from none
                         l_run[nt][e] *= fix[e];
                         sum[nt][e] *= f;
                         ref[nt][e] = m;
@@ -623,16 +624,13 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                             *reinterpret_cast<float2*>(sm + C::OFF_P + buf * C::P_BYTES + (((warp * TB + tb) * ROWS + row) * PS + 2 * r) * 4) =
                                 make_float2(s[tb][nt][e] * f, s[tb][nt][2 + e] * f);
                     }
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        o[nt][x][0] *= fix[0];
-                        o[nt][x][1] *= fix[1];
-                        o[nt][x][2] *= fix[0];
-                        o[nt][x][3] *= fix[1];
-                    }
                     // row r: its correction is held by lane r / 2 (rows 2 c, 2 c + 1)
                     const float x0 = __shfl_sync(0xffffffffu, fix[0], r >> 1), x1 = __shfl_sync(0xffffffffu, fix[1], r >> 1);
+                    const float u0 = __shfl_sync(0xffffffffu, up[0], r >> 1), u1 = __shfl_sync(0xffffffffu, up[1], r >> 1);
                     o_bias[nt] *= (r & 1) ? x1 : x0;
+                    // the sums of the products stay as they are, their power of two grows with the reference
+                    const int k = exponent_of(power[nt]) + (int)fminf((r & 1) ? u1 : u0, 1000.0f);
+                    set_power(nt, min(k, 126), min(126 - k, 0));
                 }
                 compute_barrier();
             }
@@ -644,78 +642,132 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             // positions 1 and 3 of four: 15 - n under a negative weight, so that the sums of the nibbles, whose middle is 7.5, have
             // no drift: the tensor core's truncating sums then stay relative to what they hold (f32 rows over 250,001 positions:
             // 9.6e-7 off; 1.5e-5 with n - 8 at every position)
-            auto block_of_values = [&](int pb, auto slow, auto first) {
+            uint8_t* pairs = sm + stage * C::STAGE + 17 * D + g_own * 64 + c * 16;                                          // of positions 4 c ..
+            const float* weights = reinterpret_cast<const float*>(sm + C::OFF_P + buf * C::P_BYTES) + r * PS + 4 * c;  // of row r
+            using Pairs = uint32_t[NT][2];
+            using Lows = uint32_t[C::F32 ? NT : 1][2];
+            // operands of a block for this warp's group: weight times scale times the power of two; the weighted sum of the biases
+            // so far; the largest product (NaN where there is one)
+            auto weigh = [&](int pb, Pairs& b, Lows& lo, float* ob, float& top) {
                 const int blk = tp * PB + pb;
-                const uint8_t* vb = st + blk * C::BLK + 9 * D;
-                const uint4 vw = *reinterpret_cast<const uint4*>(vb + g_own * 512 + lane * 16);
-                const uint4 pr = *reinterpret_cast<const uint4*>(vb + 8 * D + g_own * 64 + c * 16);
-                uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
-                if constexpr (decltype(slow)::value) {  // positions past the sequence's end
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (t0 + blk * kKv4Block + 4 * c + k >= u.len) pw[k] = 0;
-                }
+                const uint4 pr = *reinterpret_cast<const uint4*>(pairs + blk * C::BLK);
+                const uint32_t pw[4] = {pr.x, pr.y, pr.z, pr.w};
                 float sc[4], bi[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     sc[k] = __uint_as_float(pw[k] << 16);
                     bi[k] = __uint_as_float(pw[k] & 0xFFFF0000u);
-                    if (k & 1) {
-                        bi[k] = fmaf(15.0f, sc[k], bi[k]);
-                        sc[k] = -sc[k];
+                    if (k & 1) bi[k] = fmaf(15.0f, sc[k], bi[k]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float4 p = *reinterpret_cast<const float4*>(weights + (blk * ROWS + nt * 8) * PS);
+                    ob[nt] = fmaf(p.x, bi[0], fmaf(p.y, bi[1], fmaf(p.z, bi[2], fmaf(p.w, bi[3], ob[nt]))));
+                    // (in this order nothing that is hidden, a weight of 0, overflows)
+                    p.x = p.x * power[nt] * sc[0]; p.y = p.y * power[nt] * sc[1]; p.z = p.z * power[nt] * sc[2]; p.w = p.w * power[nt] * sc[3];
+                    top = max_nan(max_nan(top, p.x, p.y), p.z, p.w);
+                    const __half2 h02 = __floats2half2_rn(p.x, p.z), h13 = __floats2half2_rn(-p.y, -p.w);
+                    b[nt][0] = h2_bits(h02);
+                    b[nt][1] = h2_bits(h13);
+                    if constexpr (C::F32) {
+                        const float2 f02 = __half22float2(h02), f13 = __half22float2(h13);
+                        lo[nt][0] = h2_bits(__floats2half2_rn(p.x - f02.x, p.z - f02.y));
+                        lo[nt][1] = h2_bits(__floats2half2_rn(-p.y - f13.x, -p.w - f13.y));
                     }
                 }
+            };
+            auto multiply = [&](int pb, auto first, const Pairs& b, const Lows& lo) {
+                const uint4 vw = *reinterpret_cast<const uint4*>(st + (tp * PB + pb) * C::BLK + 9 * D + g_own * 512 + lane * 16);
                 uint32_t nb[4][4];  // word x: elements 8 r + 2 x, 8 r + 2 x + 1 of positions (0, 2), then of (1, 3)
                 nibbles_sub<C::F32, true>(vw.x, nb[0]);
                 nibbles_sub<C::F32, true>(vw.y, nb[1]);
                 nibbles_sub<C::F32, true>(vw.z, nb[2]);
                 nibbles_sub<C::F32, true>(vw.w, nb[3]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float4 p = *reinterpret_cast<const float4*>(sm + C::OFF_P + buf * C::P_BYTES + ((blk * ROWS + nt * 8 + r) * PS + 4 * c) * 4);
-                    if constexpr (!decltype(slow)::value) {
-                        o_bias[nt] = fmaf(p.x, bi[0], fmaf(p.y, bi[1], fmaf(p.z, bi[2], fmaf(p.w, bi[3], o_bias[nt]))));
-                        p.x *= sc[0]; p.y *= sc[1]; p.z *= sc[2]; p.w *= sc[3];
-                    } else {  // a group that was stored as NaN must not reach rows that do not see it (weight 0)
-                        o_bias[nt] += (p.x == 0.0f ? 0.0f : p.x * bi[0]) + (p.y == 0.0f ? 0.0f : p.y * bi[1]) +
-                                      (p.z == 0.0f ? 0.0f : p.z * bi[2]) + (p.w == 0.0f ? 0.0f : p.w * bi[3]);
-                        p.x = p.x == 0.0f ? 0.0f : p.x * sc[0];
-                        p.y = p.y == 0.0f ? 0.0f : p.y * sc[1];
-                        p.z = p.z == 0.0f ? 0.0f : p.z * sc[2];
-                        p.w = p.w == 0.0f ? 0.0f : p.w * sc[3];
-                    }
-                    const __half2 h02 = __floats2half2_rn(p.x, p.z), h13 = __floats2half2_rn(p.y, p.w);
-                    const uint32_t b0 = h2_bits(h02), b1 = h2_bits(h13);
-                    if constexpr (C::F32) {
-                        const float2 f02 = __half22float2(h02), f13 = __half22float2(h13);
-                        const uint32_t l0 = h2_bits(__floats2half2_rn(p.x - f02.x, p.z - f02.y)), l1 = h2_bits(__floats2half2_rn(p.y - f13.x, p.w - f13.y));
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint4 va = make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]);
-                            if constexpr (decltype(first)::value) mma_f16_zero(acc[nt][x], va, b0, b1);
-                            else mma_f16(acc[nt][x], va, b0, b1);
-                            mma_f16(acc[nt][x], va, l0, l1);
+                    for (int x = 0; x < 4; ++x) {
+                        const uint4 va = make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]);
+                        if constexpr (C::F32) {
+                            if constexpr (decltype(first)::value) mma_f16_zero(acc[nt][x], va, b[nt][0], b[nt][1]);
+                            else mma_f16(acc[nt][x], va, b[nt][0], b[nt][1]);
+                            mma_f16(acc[nt][x], va, lo[nt][0], lo[nt][1]);
+                        } else {
+                            mma_f16(o[nt][x], va, b[nt][0], b[nt][1]);
                         }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) mma_f16(o[nt][x], make_uint4(nb[x][0], nb[x][1], nb[x][2], nb[x][3]), b0, b1);
                     }
+            };
+            // Rare: something is NaN.  Pairs that are (or were never written) are taken out, and the rows that see them get a NaN.
+            auto take_out = [&]() {
+#pragma unroll 1
+                for (int i = 0; i < 4 * PB; ++i) {
+                    const int blk = tp * PB + (i >> 2), k = i & 3;
+                    uint32_t* at = reinterpret_cast<uint32_t*>(pairs + blk * C::BLK) + k;
+                    const float sc = __uint_as_float(*at << 16), bi = __uint_as_float(*at & 0xFFFF0000u);
+                    const bool bad = !(fabsf(sc) < INFINITY && fabsf(bi) < INFINITY && fabsf(fmaf(15.0f, sc, bi)) < INFINITY);
+                    __syncwarp();  // the rows share the pairs
+                    if (!bad) continue;
+                    if (r == 0) *at = 0;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        if (weights[(blk * ROWS + nt * 8) * PS + k] != 0.0f) o_bias[nt] = NAN;
+                }
+                umma::fence_smem_to_async();  // before the copies that come here next
+                __syncwarp();
+            };
+            // Rare: a reference moved or a product is too large.  Smaller powers of two for the rows that need them.
+            auto lower_powers = [&]() {
+                float m[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) m[nt] = 0.0f;
+#pragma unroll(NT == 1 ? PB : 1)
+                for (int pb = 0; pb < PB; ++pb) {
+                    const uint4 pr = *reinterpret_cast<const uint4*>(pairs + (tp * PB + pb) * C::BLK);
+                    const float sc[4] = {__uint_as_float(pr.x << 16), __uint_as_float(pr.y << 16), __uint_as_float(pr.z << 16), __uint_as_float(pr.w << 16)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {  // (fmaxf leaves NaN out)
+                        const float4 p = *reinterpret_cast<const float4*>(weights + ((tp * PB + pb) * ROWS + nt * 8) * PS);
+                        m[nt] = fmaxf(fmaxf(m[nt], fmaxf(p.x * sc[0], p.y * sc[1])), fmaxf(p.z * sc[2], p.w * sc[3]));
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    m[nt] = fmaxf(m[nt], __shfl_xor_sync(0xffffffffu, m[nt], 1));
+                    m[nt] = fmaxf(m[nt], __shfl_xor_sync(0xffffffffu, m[nt], 2));
+                    const int old = exponent_of(power[nt]), k = m[nt] * power[nt] > kProdTop ? min(kProdSet - exponent_of(m[nt]), 126) : old;
+                    set_power(nt, k, k - old);
                 }
             };
-            using Yes = std::true_type;
-            using No = std::false_type;
-            if ((any & (kFlagNan | kFlagTail)) == 0) {
-                block_of_values(0, No{}, Yes{});
-                if constexpr (PB > 1) block_of_values(1, No{}, No{});
-                if constexpr (PB > 2) {
-                    block_of_values(2, No{}, No{});
-                    block_of_values(3, No{}, No{});
-                }
-            } else {
-                block_of_values(0, Yes{}, Yes{});
+            Pairs b[C::F32 ? 1 : PB];
+            Lows lo;
+            float ob[NT];
+            bool again = any_moved;
 #pragma unroll 1
-                for (int pb = 1; pb < PB; ++pb) block_of_values(pb, Yes{}, No{});
+            for (int attempt = 0; attempt < 2; ++attempt) {
+                if (attempt > 0) take_out();
+                if (again) lower_powers();
+                float top = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) ob[nt] = o_bias[nt];
+                // f32 rows add a tile up by itself, so they look at its products afterwards; the others before
+                weigh(0, b[0], lo, ob, top);
+                if constexpr (C::F32) multiply(0, std::true_type{}, b[0], lo);
+#pragma unroll
+                for (int pb = 1; pb < PB; ++pb) {
+                    weigh(pb, b[C::F32 ? 0 : pb], lo, ob, top);
+                    if constexpr (C::F32) multiply(pb, std::false_type{}, b[0], lo);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) top = max_nan(top, ob[nt] * 0.0f, 0.0f);
+                again = __any_sync(0xffffffffu, !(top <= kProdTop));
+                if (!again) break;
             }
+            if constexpr (!C::F32) {
+#pragma unroll
+                for (int pb = 0; pb < PB; ++pb) multiply(pb, std::false_type{}, b[pb], lo);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) o_bias[nt] = ob[nt];
             if constexpr (C::F32) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -743,13 +795,15 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             float ob = o_bias[nt];
             ob += __shfl_xor_sync(0xffffffffu, ob, 1);
             ob += __shfl_xor_sync(0xffffffffu, ob, 2);
+            const float down = __uint_as_float(0x7F000000u - __float_as_uint(power[nt]));  // 1 / power
             const float b0 = __shfl_sync(0xffffffffu, ob, 8 * c), b1 = __shfl_sync(0xffffffffu, ob, 8 * c + 4);  // of rows 2 c, 2 c + 1
+            const float d0 = __shfl_sync(0xffffffffu, down, 8 * c), d1 = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                o[nt][x][0] = fmaf(o[nt][x][0], C::F32 ? kSub / 16.0f : kSub, b0);
-                o[nt][x][1] = fmaf(o[nt][x][1], C::F32 ? kSub / 16.0f : kSub, b1);
-                o[nt][x][2] = fmaf(o[nt][x][2], kSub / 16.0f, b0);
-                o[nt][x][3] = fmaf(o[nt][x][3], kSub / 16.0f, b1);
+                o[nt][x][0] = fmaf(o[nt][x][0] * (C::F32 ? kSub / 16.0f : kSub), d0, b0);
+                o[nt][x][1] = fmaf(o[nt][x][1] * (C::F32 ? kSub / 16.0f : kSub), d1, b1);
+                o[nt][x][2] = fmaf(o[nt][x][2] * (kSub / 16.0f), d0, b0);
+                o[nt][x][3] = fmaf(o[nt][x][3] * (kSub / 16.0f), d1, b1);
             }
         }
         const bool whole_unit = w_at >= w_begin && w_at + u.n_tiles + kUnitCost <= w_end;

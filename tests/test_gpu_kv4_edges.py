@@ -38,3 +38,122 @@ def test_prompts_that_share_rows(eng, q_start, dim):  # noqa: F811
     eng.kv4_attention_dev(c.cache, c.batch_of([0, 150, 300] + [300] * (n - 2), 300, 300), qb.ptr, out.ptr, L.DT_BF16, 1, scale=0.1)
     eng.sync()  # and the engine carries on
     c.free()
+
+
+# ─── plain attention over a case's cache ────────────────────────────────────
+def attend(eng, c, q, heads, dtype, *, scale, window=0, gate=None, batch=None):  # noqa: F811
+    out = c.up(np.zeros_like(q))
+    eng.kv4_attention_dev(c.cache, batch or c.batch, c.up(q).ptr, out.ptr, dtype, heads, scale=scale, window=window, gate=c.up(gate).ptr if gate is not None else 0)
+    eng.sync()
+    return as_f64(out.download(q.dtype, q.shape), dtype)
+
+
+def store(eng, c, k, v):  # noqa: F811
+    """Every position of every sequence, in one call."""
+    start = np.concatenate([[0], np.cumsum(c.lens)])
+    eng.kv4_append_dev(c.cache, c.batch_of(start, sum(c.lens), max(c.lens)), c.up(k).ptr, c.up(v).ptr, L.DT_F32)
+    eng.sync()
+    return R.codec(k), R.codec(v)
+
+
+def close(got, want, size, reach, dtype, rows=slice(None)):
+    bound = bound_of(dtype, want, size, reach)
+    r = np.abs(got - want) / bound
+    assert np.all(r[rows] <= 1), f"worst {np.max(r[rows]):.3f} of the bound"
+
+
+# shapes that take every kernel: few rows (one and two columns of eight), many f32 rows, prompts of bf16 rows
+FORMS = [(t, lens, q_lens) for lens, q_lens in (([300], [1]), ([300, 200], [4, 3]), ([700, 600], [700, 600])) for t in (L.DT_F32, L.DT_BF16)][:-1]
+
+
+# ─── values and keys of unequal size ────────────────────────────────────────
+# Bounds: bound_of, whose size is of an element's own group of 64.  What the other groups, other positions' weights and positions
+# that a row does not see hold adds nothing to it.
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("big", [2.0 ** 11, 1e5, 1e8, 1e30])
+def test_large_values_that_rows_do_not_see(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
+    """Positions behind a row's own, or before its window, in the tile it reads: large values and keys there change nothing."""
+    for window in (0, 20):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=11)
+        k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
+        at = 0
+        hidden = np.zeros(c.rows, bool)
+        hit = {n - 1 if nq > 1 else n - 25 for n, nq in zip(lens, q_lens)}
+        for b, (n, nq) in enumerate(zip(lens, q_lens)):
+            base, pos = sum(lens[:b]), np.arange(n - nq, n)
+            p = n - 1 if nq > 1 else n - 25  # the last row's own position; or one just before the window of the only row
+            v[base + p] *= big
+            k[base + p] *= min(big, 1e15)
+            hidden[at:at + nq] = (pos < p) | ((pos - p >= window) if window else False)
+            at += nq
+        assert hit and (hidden.any() or window == 0)
+        kc, vc = store(eng, c, k, v)
+        q = as_type(c.rng.standard_normal((c.rows, 8, dim)), dtype)
+        got = attend(eng, c, q, 8, dtype, scale=0.1, window=window)
+        with np.errstate(all="ignore"):
+            want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, window, 0.1)
+        close(got, want, size, reach, dtype, hidden)
+        c.free()
+
+
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("big", [2.0 ** 11, 1e5, 1e8, 1e30, 1e-8, 1e-30])
+def test_groups_of_unequal_size(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
+    """One group of 64 of a head holds values `big` times the others', at all positions or at a few."""
+    for every in (1, 97):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=12)
+        k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
+        v[::every, :, 64:128] *= big
+        kc, vc = store(eng, c, k, v)
+        q = as_type(c.rng.standard_normal((c.rows, 8, dim)), dtype)
+        want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
+        close(attend(eng, c, q, 8, dtype, scale=0.1), want, size, reach, dtype)
+        c.free()
+
+
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("big", [1e5, 1e9])
+def test_large_values_of_small_weight(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
+    """Positions that a row sees, with weights of 1e-3 to 1e-12 of the largest, hold large values: in every group, and in one."""
+    for part in (slice(0, dim), slice(0, 64)):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=13)
+        k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
+        k[..., 0] = 0.0
+        rows = np.arange(3, sum(lens), 41)
+        k[rows, 0, 0] = -c.rng.uniform(1.0, 4.0, len(rows))
+        v[rows, 0, part] *= big
+        kc, vc = store(eng, c, k, v)
+        qf = c.rng.standard_normal((c.rows, 8, dim))
+        qf[..., 0] = 70.0
+        q = as_type(qf, dtype)
+        want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
+        close(attend(eng, c, q, 8, dtype, scale=0.1), want, size, reach, dtype)
+        c.free()
+
+
+# A score is the sum over groups of s (q . n) and b sum(q), both of which may be larger than the sum of q_d k_d: its error is
+# relative to sum |q_d| (|k_d| + 15 s), not to sum |q_d k_d| alone.  2^-24 of it for each of the (at most three) f32 roundings of
+# a group's terms, 2^-23 for the 22-bit query operands, some 2^-22 for the MMA's sums: 2^-21, and a weight is off by twice that.
+# bf16 rows: queries are exact, prompts hold keys to 2^-12 of |k|, which bound_of counts.
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("big", [20.0, 300.0, 1e6])
+def test_key_channels_of_unequal_size(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
+    """A few channels of the keys are `big` times the others (of one sign, as real caches have them), the queries small there."""
+    c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=14)
+    k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
+    k[..., [5, dim - 3]] = big * (1 + 0.1 * c.rng.standard_normal((sum(lens), 1, 2)))
+    kc, vc = store(eng, c, k, v)
+    qf = c.rng.standard_normal((c.rows, 8, dim)) / big
+    qf[..., [5, dim - 3]] /= 10.0
+    q = as_type(qf, dtype)
+    want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
+    span = np.repeat(np.ptp(kc.reshape(len(kc), -1, 64), 2), 64, 1).max(0)  # 15 s, at most, of every channel
+    formed = 0.1 * (np.abs(as_f64(q, dtype)) @ (np.abs(kc[:, 0]).max(0) + span))[..., None]
+    got = attend(eng, c, q, 8, dtype, scale=0.1)
+    bound = bound_of(dtype, want, size, reach) + 2.0 ** -20 * formed * size
+    assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
+    c.free()
