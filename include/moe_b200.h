@@ -351,7 +351,8 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  * A call works on n_seqs sequences: rows q_start[b] .. q_start[b + 1] - 1 of its activations are the LAST positions of
  * sequence b, which holds seq_lens[b] positions including them; position p lies in page page_table[b, p / page_size].
  * q_start (increasing), seq_lens and page_table are device memory, read on the device; the fields below them bound what
- * they hold.  Table entries beyond a sequence's length are not read.  Rows beyond q_start[n_seqs] and rows of a sequence
+ * they hold.  Table entries beyond a sequence's length are not read, by the attention under a window neither those of pages
+ * that end before the first position a row sees: such pages may have been given back.  Rows beyond q_start[n_seqs] and rows of a sequence
  * that has more rows than positions (an idle slot: one row, length 0) carry no position: append skips them, gather and
  * attention write zeros for the latter and leave the former as they are.  Entries that break the bounds, or lead outside
  * the cache, touch no memory; they are MOE_ERR_INVALID at the next moe_engine_sync.

@@ -75,6 +75,7 @@ struct AttnUnit {
     int b, h, rt;        // sequence, KV head, row tile
     int row0, q_len, len;
     int t_lo, n_tiles;   // first position (multiple of the tile) and tiles
+    int seen;            // first position that a row of the sequence sees
 };
 
 // What a unit costs beside its tiles (queries staged, result written), in tiles: counted where tiles are dealt to CTAs, or a
@@ -86,8 +87,7 @@ constexpr int kUnitCost = 2;
 template <class C>
 __device__ __forceinline__ void attn_seq_tiles(const AttnArgs& a, const Kv4Seq& s, int& rts, int& lo, int& tiles) {
     rts = (int)(((int64_t)s.q_len * a.group + C::ROWS - 1) / C::ROWS);
-    const int first = max(s.len - s.q_len, 0);
-    lo = a.window > 0 ? max(first - a.window + 1, 0) / C::TILE * C::TILE : 0;
+    lo = first_seen(a, s.len, s.q_len) / C::TILE * C::TILE;
     tiles = max((s.len - lo + C::TILE - 1) / C::TILE, 1);  // a sequence without positions still has rows to write
 }
 
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             const Kv4Seq s = attn_seq(a, p.b, err);
             int rts;
             attn_seq_tiles<C>(a, s, rts, u.t_lo, u.n_tiles);
-            u.b = p.b; u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len;
+            u.b = p.b; u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len; u.seen = first_seen(a, s.len, s.q_len);
             const long long in = w_begin - p.prefix;
             const int unit = (int)(in / (u.n_tiles + kUnitCost));
             u.h = unit / rts;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             if (where.b >= a.seqs.n_seqs) return;
             const Kv4Seq s = attn_seq(a, where.b, err);
             u.b = where.b; u.h = h; u.rt = where.rts - 1 - where.rt;
-            u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len;
+            u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len; u.seen = first_seen(a, s.len, s.q_len);
             const int j0 = u.rt * ROWS / a.group, j1 = min((u.rt * ROWS + ROWS - 1) / a.group, s.q_len - 1);
             const int p0 = s.len - s.q_len + j0, p1 = s.len - s.q_len + j1;
             u.t_lo = a.window > 0 ? max(p0 - a.window + 1, 0) / TILE * TILE : 0;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             if (++n.b >= a.seqs.n_seqs) return;
             s = attn_seq(a, n.b, err);
         } while (s.q_len == 0);
-        n.row0 = s.row0; n.q_len = s.q_len; n.len = s.len;
+        n.row0 = s.row0; n.q_len = s.q_len; n.len = s.len; n.seen = first_seen(a, s.len, s.q_len);
         attn_seq_tiles<C>(a, s, rts, n.t_lo, n.n_tiles);
     };
 
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
     auto look_up = [&](const AttnUnit& n, int t) {
         nx_block = -1;
         const int pos = n.t_lo + t * TILE + lane * a.run * kKv4Block;
-        if (lane * a.run < NB && pos < n.len) {
+        if (lane * a.run < NB && pos < n.len && pos + a.run * kKv4Block > n.seen) {
             const int pg = over_group(pos, a.by_page);
             nx_block = (int)((unsigned)(pos - pg * a.cache.page_size) / kKv4Block);
             nx_page = -1;

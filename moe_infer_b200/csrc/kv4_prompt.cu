@@ -39,8 +39,7 @@ struct PtCfg {
 
 // Tiles of a sequence that its rows see: the first one's index and their number.
 __device__ __forceinline__ void pt_range(const AttnArgs& a, const Kv4Seq& s, int& t0, int& n) {
-    const int first = max(s.len - s.q_len, 0);
-    t0 = a.window > 0 ? max(first - a.window + 1, 0) / kPtTile : 0;
+    t0 = first_seen(a, s.len, s.q_len) / kPtTile;
     n = s.q_len > 0 ? (s.len + kPtTile - 1) / kPtTile - t0 : 0;
 }
 
@@ -68,7 +67,8 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
         return;
     }
     const int p0 = (tile0 + ti) * kPtTile;
-    if (tid < 8) blocks[tid] = p0 + tid * 16 < s.len ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
+    if (tid < 8)
+        blocks[tid] = p0 + tid * 16 < s.len && p0 + tid * 16 + 16 > first_seen(a, s.len, s.q_len) ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
     if (tid < 4) nan_bits[tid] = 0;
     __syncthreads();
     // the largest |value| a pair can stand for

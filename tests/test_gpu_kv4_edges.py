@@ -66,6 +66,23 @@ def close(got, want, size, reach, dtype, rows=slice(None)):
 FORMS = [(t, lens, q_lens) for lens, q_lens in (([300], [1]), ([300, 200], [4, 3]), ([700, 600], [700, 600])) for t in (L.DT_F32, L.DT_BF16)][:-1]
 
 
+# ─── windows ────────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 2), (128, 8, 8), (256, 16, 2)])
+@pytest.mark.parametrize("lens,q_lens", [([900, 333], [1, 1]), ([900, 333], [3, 3]), ([900, 700], [550, 500])])
+def test_pages_behind_the_window_may_be_gone(eng, lens, q_lens, dim, heads, kv_heads, dtype):  # noqa: F811
+    """Pages that end before the first position a row sees are not looked up: their table entries may be anything (-1 here)."""
+    for window in (1, 37, 130):
+        c = Case(eng, lens, q_lens, kv_heads=kv_heads, dim=dim, page=16, seed=window)
+        k, v = c.fill()
+        for b, (n, nq) in enumerate(zip(lens, q_lens)):
+            c.table[b, :max(n - nq - window + 1, 0) // 16] = -1
+        q = as_type(c.rng.standard_normal((c.rows, heads, dim)), dtype)
+        want, size, reach = R.attention(as_f64(q, dtype), k, v, lens, q_lens, window, 0.1)
+        close(attend(eng, c, q, heads, dtype, scale=0.1, window=window, batch=c.batch_of(c.q_start, c.rows, c.max_q)), want, size, reach, dtype)
+        c.free()
+
+
 # ─── values and keys of unequal size ────────────────────────────────────────
 # Bounds: bound_of, whose size is of an element's own group of 64.  What the other groups, other positions' weights and positions
 # that a row does not see hold adds nothing to it.
