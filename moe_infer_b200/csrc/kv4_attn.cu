@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             u.row0 = s.row0; u.q_len = s.q_len; u.len = s.len; u.seen = first_seen(a, s.len, s.q_len);
             const int j0 = u.rt * ROWS / a.group, j1 = min((u.rt * ROWS + ROWS - 1) / a.group, s.q_len - 1);
             const int p0 = s.len - s.q_len + j0, p1 = s.len - s.q_len + j1;
-            u.t_lo = a.window > 0 ? max(p0 - a.window + 1, 0) / TILE * TILE : 0;
+            u.t_lo = window_from(a, p0) / TILE * TILE;
             u.n_tiles = max((p1 + 1 - u.t_lo + TILE - 1) / TILE, 1);
             w_begin = 0; w_end = u.n_tiles + kUnitCost; w_at = 0;
         }
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                 rf[nt][e] = row_f[row];
                 // rows behind the last are computed unmasked and not written
                 see_hi[nt][e] = rr < rows_all ? pos_base + over_group(rr, a.by_group) : 0x7FFFFFFF;
-                see_lo[nt][e] = a.window > 0 && rr < rows_all ? see_hi[nt][e] - a.window + 1 : 0;
+                see_lo[nt][e] = rr < rows_all ? window_from(a, see_hi[nt][e]) : 0;
                 all_hi = min(all_hi, see_hi[nt][e]);
                 all_lo = max(all_lo, see_lo[nt][e]);
             }

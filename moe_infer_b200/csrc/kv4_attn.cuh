@@ -51,8 +51,11 @@ __device__ __forceinline__ Kv4Seq attn_seq(const AttnArgs& a, int b, unsigned in
     if (rows < a.lo_rows || rows >= a.hi_rows) s.q_len = 0;
     return s;
 }
+// First position of the window that ends at position p; a row before the first position (p < 0) sees none, and its p is not
+// taken further down, where p - window would pass 32 bits.
+__device__ __forceinline__ int window_from(const AttnArgs& a, int p) { return a.window > 0 ? max(max(p, 0) - a.window + 1, 0) : 0; }
 // First position that a row of a sequence sees; pages that end before it may be gone and are not looked up.
-__device__ __forceinline__ int first_seen(const AttnArgs& a, int len, int q_len) { return a.window > 0 ? max(max(len - q_len, 0) - a.window + 1, 0) : 0; }
+__device__ __forceinline__ int first_seen(const AttnArgs& a, int len, int q_len) { return window_from(a, len - q_len); }
 // Row tile `at` in the line of all sequences' row tiles (of `rows` rows): its sequence (n_seqs: none), its index there and the
 // number of sequences with rows before that one.  Called by all threads of a CTA of n_threads (a multiple of 32);
 // red: one word per warp and two more, in shared memory.

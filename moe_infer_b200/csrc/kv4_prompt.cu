@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
     pt_range(a, s, seq_t0, seq_n);
     const int j_first = rt * kPtTile / a.group, j_last = min((rt * kPtTile + kPtTile - 1) / a.group, s.q_len - 1);
     const int p_last = pos_base + j_last;  // may be negative: rows without a position
-    const int t_begin = a.window > 0 ? max(pos_base + j_first - a.window + 1, 0) / kPtTile : 0;
+    const int t_begin = window_from(a, pos_base + j_first) / kPtTile;
     const int n_tiles = p_last >= 0 ? min(p_last / kPtTile + 1, seq_t0 + min(seq_n, tiles_per_seq)) - t_begin : 0;
     const size_t img0 = ((size_t)where.before * a.cache.kv_heads + h) * tiles_per_seq + (t_begin - seq_t0);
 
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the place is used for the tiles' maxima next
         const int j = valid ? over_group(rr, a.by_group) : 0;
         const int see_hi = valid ? pos_base + j : 0x7FFFFFFF;
-        const int see_lo = valid && a.window > 0 ? see_hi - a.window + 1 : 0;
+        const int see_lo = valid ? window_from(a, see_hi) : 0;
         float m_ref = -INFINITY, l = 0.0f;
         for (int i = 0; i < n_tiles; ++i) {
             const int t0 = (t_begin + i) * kPtTile + 64 * half;  // this thread's positions

@@ -83,6 +83,22 @@ def test_pages_behind_the_window_may_be_gone(eng, lens, q_lens, dim, heads, kv_h
         c.free()
 
 
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("lens,q_lens", [([5, 40], [9, 2]), ([90], [400]), ([600], [700])])
+@pytest.mark.parametrize("window", [0x7FFFFFFF, 0x7FFFFFF0, 0x7FFE0000])
+def test_widest_windows(eng, lens, q_lens, window, dtype):  # noqa: F811
+    """A window wider than any sequence sees everything, for rows of a sequence that has more rows than positions too."""
+    c = Case(eng, lens, q_lens, kv_heads=2, dim=64, page=16, seed=1)
+    k, v = c.fill()
+    q = as_type(c.rng.standard_normal((c.rows, 16, 64)), dtype)
+    want, size, reach = R.attention(as_f64(q, dtype), k, v, lens, q_lens, 0, 0.1)
+    batch = c.batch_of(c.q_start, c.rows, c.max_q)
+    batch.max_seq_len = 0x7FFF0000  # a bound no tighter than it has to be
+    close(attend(eng, c, q, 16, dtype, scale=0.1, window=window, batch=batch), want, size, reach, dtype)
+    close(attend(eng, c, q, 16, dtype, scale=0.1, window=window), want, size, reach, dtype)
+    c.free()
+
+
 # ─── values and keys of unequal size ────────────────────────────────────────
 # Bounds: bound_of, whose size is of an element's own group of 64.  What the other groups, other positions' weights and positions
 # that a row does not see hold adds nothing to it.
