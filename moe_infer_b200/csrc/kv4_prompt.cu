@@ -531,8 +531,9 @@ static size_t pt_image_bytes(const AttnArgs& a) {
 // Images of at most 4 GB: a call that could need more (many sequences of unknown lengths) takes the kernel that needs none.
 template <int D>
 bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a) {
-    return (int64_t)a.seqs.max_q_len * a.group >= kPromptRows && pt_image_bytes<D>(a) <= (size_t)4 << 30 && a.cache.kv_heads <= 65535 &&
-           a.seqs.n_seqs <= 65535;
+    // (counted in tiles first, 2^17 of which are 4 GB at least: 65,535 sequences x 65,535 heads x 2^24 tiles pass 64 bits in bytes)
+    return (int64_t)a.seqs.max_q_len * a.group >= kPromptRows && a.cache.kv_heads <= 65535 && a.seqs.n_seqs <= 65535 &&
+           pt_max_seqs(a) * a.cache.kv_heads * pt_tiles_per_seq(a) <= 1 << 17 && pt_image_bytes<D>(a) <= (size_t)4 << 30;
 }
 
 template <int D>
