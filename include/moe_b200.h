@@ -344,8 +344,8 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
 /* ── paged KV cache in 4 bits, many sequences ────────────────────────────────
  * No counterpart in the reference, whose caches are f32, contiguous and hold one sequence (src/cache.rs:32-94): what
  * serving several sequences or contexts beyond max_seq needs next to the 4-bit weights.  Keys and values are held by the
- * codec of moe_pack_int4_* (64 elements to a bf16 scale and bias; 18 bytes per 16 elements of K and V together, against
- * 128 in f32).  The caller owns the pages (moe_kv4_page_bytes each, one allocation per layer, 16-byte aligned) and hands
+ * codec of moe_pack_int4_* (64 elements to a bf16 scale and bias, 64 equal ones with a scale of 0; 18 bytes per 16 elements of
+ * K and V together, against 128 in f32).  The caller owns the pages (moe_kv4_page_bytes each, one allocation per layer, 16-byte aligned) and hands
  * them to sequences through a page table; nothing is kept between calls.
  *
  * A call works on n_seqs sequences: rows q_start[b] .. q_start[b + 1] - 1 of its activations are the LAST positions of

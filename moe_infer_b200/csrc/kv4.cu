@@ -1,7 +1,8 @@
 // Writing and reading back the paged 4-bit KV cache (page format: kv4.cuh).
 //
 // Append: key (rotated on the way) and value rows -> nibbles and (scale, bias) pairs, bit for bit the codec of pack.cu:
-//   scale = (max - min) / 15, nibble = trunc((x - min) * (1 / scale) + 0.5), scale and bias = min stored in bf16.
+//   scale = (max - min) / 15, nibble = trunc((x - min) * (1 / scale) + 0.5), scale and bias = min stored in bf16
+// (a group of equal values: scale 0).
 // Memory bound (f32, head 256: 2 KB read, 288 B written per position and head).  A CTA takes 16 positions of a sequence (one
 // block of the cache) and a head, so what it has to know first (sequence, page) is one chain of loads, and the rows are
 // requested before the page is known.  A sub-warp of D / 8 lanes takes one quad (four positions that share words of V) of
@@ -58,10 +59,11 @@ __device__ __forceinline__ uint32_t kv4_quant(const float (&x)[4][8], uint32_t (
             mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
         }
     const float lo = (lane & 2) ? ((lane & 1) ? mn[3] : mn[2]) : ((lane & 1) ? mn[1] : mn[0]);
-    float hi = (lane & 2) ? ((lane & 1) ? mx[3] : mx[2]) : ((lane & 1) ? mx[1] : mx[0]);
-    if (hi == lo) hi = __fadd_rn(lo, 1.0f);
-    const float scale = __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
-    float inv = __fdiv_rn(1.0f, scale);
+    const float hi = (lane & 2) ? ((lane & 1) ? mx[3] : mx[2]) : ((lane & 1) ? mx[1] : mx[0]);
+    // equal values: scale 0 (the packer's 1 / 15 stands for the same values, but would enter the attention's sums as s (15 - n))
+    const bool flat = hi == lo;
+    const float scale = flat ? 0.0f : __fdiv_rn(__fsub_rn(hi, lo), 15.0f);
+    float inv = flat ? 0.0f : __fdiv_rn(1.0f, scale);
     uint32_t pair = (uint32_t)f32_to_bf16_ref(scale) | (uint32_t)f32_to_bf16_ref(lo) << 16;
     // not finite, or too large for its pair to be: both halves NaN (the attention kernel looks at the scale alone)
     if (!(fabsf(lo) < INFINITY && fabsf(scale) < INFINITY && (pair & 0x7F80u) != 0x7F80u && (pair & 0x7F800000u) != 0x7F800000u)) {

@@ -4,7 +4,8 @@
 // 18 * head_dim bytes:
 //   K nibbles   8 * D bytes   K pairs   D bytes   V nibbles   8 * D bytes   V pairs   D bytes
 // Every 64 elements of a key or value share one (scale, bias) pair, both bf16, value = nibble * scale + bias: the codec
-// of the 4-bit weights (moe_pack_int4_*), bit for bit.  A pair is one 32-bit word (scale low), stored [group][position].
+// of the 4-bit weights (moe_pack_int4_*), bit for bit but for groups of equal values, whose scale is 0 here.  A
+// pair is one 32-bit word (scale low), stored [group][position].
 //
 // The nibbles lie in the order in which a warp feeds them to mma.m16n8k16, so that one 16-byte load per
 // lane (512 contiguous bytes per warp, no bank conflicts, no shuffles) covers two 64-element groups of 8 keys, or one

@@ -190,3 +190,23 @@ def test_key_channels_of_unequal_size(eng, big, dim, dtype, lens, q_lens):  # no
     bound = bound_of(dtype, want, size, reach) + 2.0 ** -20 * formed * size
     assert np.all(np.abs(got - want) <= bound), np.max(np.abs(got - want) / bound)
     c.free()
+
+
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+def test_groups_of_equal_values(eng, dtype, lens, q_lens):  # noqa: F811
+    """A group of 64 equal values has no range: zeros come out as zeros, others as themselves, beside small and large ones."""
+    for small in (1e-6, 1.0, 1e6):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=256, page=16, seed=15)
+        k, v = (c.rng.standard_normal((sum(lens), 1, 256)).astype(np.float32) for _ in range(2))
+        v *= np.float32(small)
+        v[..., 64:128] = 0.0
+        v[..., 128:192] = 0.37e-3 * small
+        v[::3] = 0.0
+        k[1::7, :, 128:192] = 0.0
+        kc, vc = store(eng, c, k, v)
+        q = as_type(c.rng.standard_normal((c.rows, 8, 256)), dtype)
+        got = attend(eng, c, q, 8, dtype, scale=0.1)
+        want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
+        close(got, want, size, reach, dtype)
+        assert np.all(got[..., 64:128] == 0.0)
+        c.free()
