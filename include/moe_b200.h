@@ -370,7 +370,10 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        out is [n_tokens, num_heads, head_dim] of the queries' type, contiguous; it must not overlap them.
  *                        f32 rows: operands in two f16 terms, results to about 2^-21; bf16 rows: weights rounded to f16
  *                        (2^-12), and for sequences of at least 128 rows x query heads per KV head (prompts) keys and values
- *                        too; scores, sums and the softmax f32.  A row that sees a value stored as NaN is NaN in that group of
+ *                        too; scores, sums and the softmax f32.  Sizes of keys and values may differ as they like: what is lost
+ *                        is relative to the weighted |values| and ranges of the same group of 64 that the row sees.  (A prompt
+ *                        over keys with a group below 2^-11 of its 128 neighbours' largest, or values with one below 2^-9 of their
+ *                        position's, zeros aside, is computed without f16 keys and values, more slowly.)  A row that sees a value stored as NaN is NaN in that group of
  *                        64 (in a prompt, in the whole row).  Prompts of bf16 rows need a work area, the positions they see as
  *                        f16 (4 head_dim bytes per position and KV head), grown on demand and kept by the engine; calls whose
  *                        bounds could need more than 4 GB of it run without, more slowly.

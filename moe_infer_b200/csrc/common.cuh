@@ -227,6 +227,8 @@ struct ModelAttnState {
 struct Kv4State {
     float* work = nullptr;
     size_t work_bytes = 0;
+    unsigned* wide = nullptr;                // prompts: number of the last call that found a sequence's values too unequal for f16 tiles
+    unsigned calls = 0;                      // of prompts
     int occupancy[64] = {};                  // resident CTAs per SM of each kernel variant (0: not asked yet)
 };
 

@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
         *abort_flag = 0;
     }
     pdl_trigger();
+    pdl_wait();  // (behind a prompt kernel: that one still reads the work area)
 
     // this CTA's tiles [w_begin, w_end) of the line of all tiles (SPLIT), or one unit
     long long w_begin = 0, w_end = 0, w_at = 0;
@@ -894,6 +895,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 template <class C, typename T>
 __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, int row_tiles, int by_border, int parts, unsigned int* err) {
     constexpr int D = C::D, ROWS = C::ROWS;
+    if (a.wide_too && a.hi_rows == 0 && a.seqs.n_seqs == 1 && a.wide[0] != a.call) {  // the prompt kernel took it
+        pdl_wait();
+        return;
+    }
     __shared__ long long red[8], found[4];
     __shared__ float4 acc_s[256];
     __shared__ float m_s[256], l_s[256];
@@ -1053,6 +1058,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
 // ─── host side ──────────────────────────────────────────────────────────────
 void kv4_destroy(moe_engine* e) {
     if (e->kv4.work) cudaFree(e->kv4.work);
+    if (e->kv4.wide) cudaFree(e->kv4.wide);
     e->kv4 = Kv4State{};
 }
 
@@ -1073,7 +1079,7 @@ int kv4_reserve(moe_engine* e, size_t bytes) {
 }
 
 template <class C, typename T>
-static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64_t q_rows) {
+static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64_t q_rows, bool dependent) {
     a.run = 1;
     while (a.run < C::NB && a.cache.page_size / kKv4Block % (2 * a.run) == 0) a.run *= 2;
     auto* kernel = kv4_attn_kernel<C, T>;
@@ -1100,7 +1106,7 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64
         int rc = kv4_reserve(e, (size_t)grid * 2 * C::ROWS * (C::D + 2) * 4);
         if (rc) return rc;
         a.part = e->kv4.work;
-        MOE_CUDA(launch_kernel(false, kernel, dim3((unsigned)grid), dim3(128), C::SMEM, e->stream, a, err));
+        MOE_CUDA(launch_kernel(dependent, kernel, dim3((unsigned)grid), dim3(128), C::SMEM, e->stream, a, err));
         e->launches++;
         if (grid == 1) return MOE_OK;  // nothing can be split
         const int64_t all = (int64_t)a.seqs.n_seqs * a.cache.kv_heads * row_tiles;
@@ -1119,7 +1125,7 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64
 // position among more rows, but their 255 registers leave two CTAs to an SM: 162 against 143 us on f32 prompts, 36 against
 // 31 us on four-token verification).  f32 rows in units of their own (no splitting) once those fill the GPU four times over.
 template <int D, typename T>
-static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows) {
+static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows, bool dependent = false) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int V0 = (D == 64 ? 0 : D == 128 ? 8 : 16) + (F32 ? 4 : 0);
     const int64_t n = a.seqs.n_seqs;
@@ -1130,21 +1136,26 @@ static int launch_rows(moe_engine* e, const AttnArgs& a, int64_t q_rows) {
     };
     constexpr int TB = 4 / (D / 64);
     if constexpr (F32) {
-        if (q_rows > 16 && units(16) >= 4 * e->sm_count) return run_attn<AttnCfg<D, F32, 2, 1, false>, T>(e, a, V0 + 2, units(16), q_rows);
+        if (q_rows > 16 && units(16) >= 4 * e->sm_count) return run_attn<AttnCfg<D, F32, 2, 1, false>, T>(e, a, V0 + 2, units(16), q_rows, false);
     }
-    if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16), q_rows);
-    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8), q_rows);
+    if (q_rows > 8) return run_attn<AttnCfg<D, F32, 2, 1, true>, T>(e, a, V0 + 1, units(16), q_rows, dependent);
+    return run_attn<AttnCfg<D, F32, 1, TB, true>, T>(e, a, V0, units(8), q_rows, dependent);
 }
 
 template <int D, typename T>
 static int launch_attn(moe_engine* e, const AttnArgs& a) {
     if constexpr (sizeof(T) == 2) {
         if (kv4_prompt_fits<D>(e, a)) {
-            const int rc = launch_kv4_prompt<D>(e, a);
-            if (rc || a.seqs.n_seqs == 1) return rc;  // (a single sequence is its, however many rows it turns out to have)
+            AttnArgs few = a;
+            const int rc = launch_kv4_prompt<D>(e, few);
+            if (rc) return rc;
+            const int64_t all_rows = (int64_t)a.seqs.max_q_len * a.group;
+            few.hi_rows = 0;
+            few.wide_too = 1;
+            if (a.seqs.n_seqs == 1) return launch_rows<D, T>(e, few, all_rows, true);  // (the sequence is its, however many rows it has)
+            few.wide_too = 0;
             // the sequences of fewer rows (the host knows bounds only): single tokens in as small a tile as they need, then the others
             const int one = (a.group + 7) / 8 * 8;
-            AttnArgs few = a;
             if (one < kPromptRows) {
                 few.hi_rows = one + 1;
                 const int rc1 = launch_rows<D, T>(e, few, one);
@@ -1152,7 +1163,8 @@ static int launch_attn(moe_engine* e, const AttnArgs& a) {
                 few.lo_rows = one + 1;
             }
             few.hi_rows = kPromptRows;
-            return few.lo_rows < kPromptRows ? launch_rows<D, T>(e, few, kPromptRows - 1) : rc;
+            few.wide_too = 1;
+            return launch_rows<D, T>(e, few, all_rows);
         }
     }
     return launch_rows<D, T>(e, a, (int64_t)a.seqs.max_q_len * a.group);

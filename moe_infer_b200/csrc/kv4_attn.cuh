@@ -31,6 +31,9 @@ struct AttnArgs {
     int lo_rows, hi_rows;    // sequences with lo_rows <= rows < hi_rows (rows x query heads per KV head) are this launch's
     int run;                 // blocks of a tile that one copy brings (they lie in one page)
     int image_seqs;          // prompts: sequences the expanded tiles have room for
+    unsigned* wide;          // prompts: [sequence] == call where its values are too unequal for f16 tiles
+    unsigned call;
+    int wide_too;            // those sequences are this launch's too
     float* part;             // work area of the call
 };
 
@@ -41,14 +44,14 @@ constexpr int kPromptRows = 128;
 template <int D>
 bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a);
 template <int D>
-int launch_kv4_prompt(moe_engine* e, AttnArgs a);
+int launch_kv4_prompt(moe_engine* e, AttnArgs& call);  // sets wide and call
 
 #ifdef __CUDACC__
 // A sequence as a launch sees it: without rows where they are another launch's.
 __device__ __forceinline__ Kv4Seq attn_seq(const AttnArgs& a, int b, unsigned int* err) {
     Kv4Seq s = kv4_seq(a.seqs, b, err);
     const long long rows = (long long)s.q_len * a.group;
-    if (rows < a.lo_rows || rows >= a.hi_rows) s.q_len = 0;
+    if ((rows < a.lo_rows || rows >= a.hi_rows) && !(a.wide_too && a.wide[b] == a.call)) s.q_len = 0;
     return s;
 }
 // First position of the window that ends at position p; a row before the first position (p < 0) sees none, and its p is not

@@ -3,7 +3,10 @@
 // With hundreds of rows per position the products dominate (4 D flops per row, head and position) and every position is
 // read by many row tiles, so the positions the call sees are first expanded, once, into f16 tiles of 128 positions that
 // lie in memory exactly as the MMAs want them in shared memory (K-major, 128-byte swizzle): a tile then arrives by plain
-// bulk copies.  f16 values of a tile are scaled by a power of two of its own, so any range of values keeps 11 bits.
+// bulk copies.  Keys of a tile are scaled by a power of two, values by one per tile or, where the tile's positions differ by
+// more than 2^3, one per position, which the weights carry: so only what a row sees decides how its weights are scaled.  f16
+// keeps 11 bits down to 2^-14: a sequence with a key group of 64 below 2^-11 of its tile's largest key, or a value group below
+// 2^-9 of its position's largest value (groups of zeros aside), is left to the kernel of few rows, which has no such limit.
 //
 // Attention kernel: a CTA owns 128 rows (of the query heads that share a KV head) and walks its positions.  One thread
 // copies, one issues MMAs, eight warps hold a row per pair of threads (half a tile's positions, then half of O, each):
@@ -21,7 +24,10 @@
 namespace moe {
 
 constexpr int kPtTile = 128;                 // positions of a tile, rows of a CTA
-constexpr int kPtMeta = 8;                   // ints per tile: exponents of K and V, four words of "value is NaN" bits
+// ints per tile: exponent of K; twice that of V, and 1 if every position has an exponent of its own; four words of "value is
+// NaN" bits; the positions' exponents (f32) from the eighth on
+constexpr int kPtMeta = 8 + kPtTile;
+constexpr float kKeySpan = 1.0f / 2048, kValueSpan = 1.0f / 512, kEven = 1.0f / 8;
 
 template <int D>
 struct PtCfg {
@@ -43,6 +49,12 @@ __device__ __forceinline__ void pt_range(const AttnArgs& a, const Kv4Seq& s, int
     n = s.q_len > 0 ? (s.len + kPtTile - 1) / kPtTile - t0 : 0;
 }
 
+// two values n s + b, given n - 8 and b + 8 s, rounded to f16 once
+__device__ __forceinline__ uint32_t value_pair(uint32_t n8, float s0, float b0, float s1, float b1) {
+    const float2 f = __half22float2(bits_h2(n8));
+    return h2_bits(__floats2half2_rn(fmaf(f.x, s0, b0), fmaf(f.y, s1, b1)));
+}
+
 // One CTA expands K or V of one tile of one head.  image: [(sequence, head, tile)][K, V][IMG bytes], the sequences that have
 // rows here counted; meta alike, kPtMeta ints.
 template <int D>
@@ -51,7 +63,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     constexpr int G = C::G;
     extern __shared__ __align__(1024) uint8_t ex_sm[];
     __shared__ uint8_t* blocks[8];
-    __shared__ float red[8];
+    __shared__ float mag[G * kPtTile], down[kPtTile], red[16];
     __shared__ unsigned int nan_bits[4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool is_v = blockIdx.x & 1;
@@ -71,31 +83,58 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
         blocks[tid] = p0 + tid * 16 < s.len && p0 + tid * 16 + 16 > first_seen(a, s.len, s.q_len) ? kv4_block(a.cache, a.seqs, b, h, p0 + tid * 16, kv4_block_bytes(D), err) : nullptr;
     if (tid < 4) nan_bits[tid] = 0;
     __syncthreads();
-    // the largest |value| a pair can stand for
-    float mx = 0.0f;
+    // the largest |value| that each group of each position holds
     for (int i = tid; i < G * kPtTile; i += 256) {
         const int t = i % kPtTile, g = i / kPtTile;
         const uint8_t* blk = blocks[t >> 4];
-        if (!blk || p0 + t >= s.len) continue;
-        const uint32_t pw = *reinterpret_cast<const uint32_t*>(blk + (is_v ? 17 * D : 8 * D) + g * 64 + (t & 15) * 4);
-        const float sc = __uint_as_float(pw << 16), bi = __uint_as_float(pw & 0xFFFF0000u);
-        const float v = fmaxf(fabsf(bi), fabsf(fmaf(15.0f, sc, bi)));
-        if (v < INFINITY && fabsf(sc) < INFINITY) mx = fmaxf(mx, v);
-        else atomicOr(nan_bits + (t >> 5), 1u << (t & 31));
+        float v = 0.0f;
+        if (blk && p0 + t < s.len) {
+            const uint32_t pw = *reinterpret_cast<const uint32_t*>(blk + (is_v ? 17 * D : 8 * D) + g * 64 + (t & 15) * 4);
+            const float sc = __uint_as_float(pw << 16), bi = __uint_as_float(pw & 0xFFFF0000u);
+            v = fmaxf(fabsf(bi), fabsf(fmaf(15.0f, sc, bi)));
+            if (!(v < INFINITY && fabsf(sc) < INFINITY && fabsf(bi) < INFINITY)) {
+                v = 0.0f;
+                atomicOr(nan_bits + (t >> 5), 1u << (t & 31));
+            }
+        }
+        mag[i] = v;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) red[warp] = mx;
     __syncthreads();
-    mx = red[0];
+    // of a position: the largest, and the smallest that is not 0
+    float top = 0.0f, least = INFINITY;
+    if (tid < kPtTile) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, red[i]);
-    // scaled into [1, 2); an all-zero tile keeps a harmless exponent
-    const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 126);
-    const float down = pow2f(-e);
+        for (int g = 0; g < G; ++g) {
+            const float v = mag[g * kPtTile + tid];
+            top = fmaxf(top, v);
+            if (v > 0.0f) least = fminf(least, v);
+        }
+    }
+    float mx = top, mn = least;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if (lane == 0) {
+        red[warp] = mx;
+        red[8 + warp] = mn;
+    }
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    mn = fminf(fminf(red[8], red[9]), fminf(red[10], red[11]));
+    const bool here = tid < kPtTile && p0 + tid < s.len && blocks[(tid & (kPtTile - 1)) >> 4];
+    if (is_v ? here && least < top * kValueSpan : tid == 0 && mn < mx * kKeySpan) a.wide[b] = a.call;
+    const bool uneven = __syncthreads_or(is_v && here && top < mx * kEven);
+    // scaled into [1, 2); what is all zero keeps a harmless exponent
+    auto exponent = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126); };
+    const int e = exponent(mx);
+    if (tid < kPtTile) down[tid] = pow2f(-(uneven ? exponent(top) : e));
+    __syncthreads();
     const size_t at = ((size_t)before * a.cache.kv_heads + h) * tiles_per_seq + ti;
-    if (tid == 0) meta[at * kPtMeta + (is_v ? 1 : 0)] = e;
+    if (tid == 0) meta[at * kPtMeta + (is_v ? 1 : 0)] = is_v ? 2 * e + (uneven ? 1 : 0) : e;
     if (is_v && tid < 4) meta[at * kPtMeta + 2 + tid] = (int)nan_bits[tid];
+    if (uneven && tid < kPtTile) reinterpret_cast<float*>(meta)[at * kPtMeta + 8 + tid] = (float)exponent(top);
 
     if (!is_v) {
         // a word = 8 elements of a position, f16 order 0 4 1 5 2 6 3 7 (the queries' too): one 16-byte chunk of the row
@@ -108,12 +147,11 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
                 const int tt = t & 15, cc = (c8 >> 1) & 3, j = c8 & 1;
                 const uint32_t w = *reinterpret_cast<const uint32_t*>(blk + (g / U) * (512 * U) + ((tt & 1) * 8 + (tt >> 1)) * (32 * U) + cc * (8 * U) + (g % U) * 8 + j * 4);
                 const uint32_t pw = *reinterpret_cast<const uint32_t*>(blk + 8 * D + g * 64 + tt * 4);
-                const float sc = __uint_as_float(pw << 16);
-                const __half2 hs = __float2half2_rn(sc * down), hb = __float2half2_rn(fmaf(8.0f, sc, __uint_as_float(pw & 0xFFFF0000u)) * down);
+                const float sc = __uint_as_float(pw << 16) * down[t], mid = fmaf(8.0f, __uint_as_float(pw << 16), __uint_as_float(pw & 0xFFFF0000u)) * down[t];
                 uint32_t nb[4];
                 nibbles_h2(w, nb);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = h2_bits(__hfma2(bits_h2(nb[k]), hs, hb));
+                for (int k = 0; k < 4; ++k) o[k] = value_pair(nb[k], sc, mid, sc, mid);
             }
             *reinterpret_cast<uint4*>(ex_sm + g * (kPtTile * 128) + umma::sw128_offset(t, c8 & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
@@ -139,19 +177,18 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
                     for (int k = 0; k < 4; ++k) {
                         const float s0 = __uint_as_float(pw[k] << 16), b0 = __uint_as_float(pw[k] & 0xFFFF0000u);
                         const bool in = p0 + ch * 8 + qd * 4 + k < s.len && fabsf(s0) < INFINITY && fabsf(b0) < INFINITY;  // NaN: marked above
-                        sc[k] = in ? s0 * down : 0.0f;
-                        bi[k] = in ? fmaf(8.0f, s0, b0) * down : 0.0f;
+                        const float d = down[ch * 8 + qd * 4 + k];
+                        sc[k] = in ? s0 * d : 0.0f;
+                        bi[k] = in ? fmaf(8.0f, s0, b0) * d : 0.0f;
                     }
-                    const __half2 s02 = __floats2half2_rn(sc[0], sc[2]), s13 = __floats2half2_rn(sc[1], sc[3]);
-                    const __half2 b02 = __floats2half2_rn(bi[0], bi[2]), b13 = __floats2half2_rn(bi[1], bi[3]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         uint32_t nb[4];
                         nibbles_h2(w[x], nb);
-                        o[2 * x][2 * qd] = h2_bits(__hfma2(bits_h2(nb[0]), s02, b02));
-                        o[2 * x + 1][2 * qd] = h2_bits(__hfma2(bits_h2(nb[1]), s02, b02));
-                        o[2 * x][2 * qd + 1] = h2_bits(__hfma2(bits_h2(nb[2]), s13, b13));
-                        o[2 * x + 1][2 * qd + 1] = h2_bits(__hfma2(bits_h2(nb[3]), s13, b13));
+                        o[2 * x][2 * qd] = value_pair(nb[0], sc[0], bi[0], sc[2], bi[2]);
+                        o[2 * x + 1][2 * qd] = value_pair(nb[1], sc[0], bi[0], sc[2], bi[2]);
+                        o[2 * x][2 * qd + 1] = value_pair(nb[2], sc[1], bi[1], sc[3], bi[3]);
+                        o[2 * x + 1][2 * qd + 1] = value_pair(nb[3], sc[1], bi[1], sc[3], bi[3]);
                     }
                 }
             }
@@ -210,6 +247,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         if (tid == 0) atomicExch(err, kErrKv4Batch);
         return;
     }
+    if (a.wide[b] == a.call) return;     // the kernel of few rows takes it
     const Kv4Seq s = kv4_seq(a.seqs, b, err);
     const int rt = where.rts - 1 - where.rt, rows_all = s.q_len * a.group, pos_base = s.len - s.q_len;
     int seq_t0, seq_n;
@@ -318,7 +356,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 else raw[i] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
             }
         };
-        int e_k = 0, e_v = 0;
+        int e_k = 0, e_v = 0;  // of the tile at hand, requested a tile ahead
         if (n_tiles > 0) {
             e_k = meta[img0 * kPtMeta];
             e_v = meta[img0 * kPtMeta + 1];
@@ -365,7 +403,8 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         for (int i = 0; i < n_tiles; ++i) {
             const int t0 = (t_begin + i) * kPtTile + 64 * half;  // this thread's positions
             const int* mt = meta + (img0 + i) * kPtMeta;
-            const int ek = e_k, ev = e_v;
+            const int ek = e_k, ev = e_v >> 1;
+            const bool uneven = e_v & 1;
             const uint32_t nb[2] = {(uint32_t)mt[2 + 2 * half], (uint32_t)mt[3 + 2 * half]};
             if (i + 1 < n_tiles) {
                 e_k = mt[kPtMeta];
@@ -386,6 +425,17 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                         if (t > see_hi || t < see_lo) v[q][k] = -INFINITY;
                     }
             }
+            // weights are exp2(S f + e - m): the tile's values are held divided by 2^e
+            float f = fmaxf(f_row * pow2f(ek), 1.2e-38f), e_top = (float)ev;
+            float2 e_own = make_float2(0.0f, 0.0f);  // of positions 2 lane, 2 lane + 1 of the 64
+            auto e_of = [&](int k) { return __shfl_sync(0xffffffffu, (k & 1) ? e_own.y : e_own.x, k >> 1); };
+            if (uneven) {  // an exponent per position
+                e_own = reinterpret_cast<const float2*>(mt + 8 + 64 * half)[lane];
+#pragma unroll
+                for (int k = 0; k < 64; ++k) v[k >> 5][k & 31] = fmaf(v[k >> 5][k & 31], f, e_of(k));
+                f = 1.0f;
+                e_top = 0.0f;
+            }
             float mx[4] = {v[0][0], v[0][1], v[1][0], v[1][1]};
 #pragma unroll
             for (int k = 2; k < 32; k += 2) {
@@ -394,9 +444,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 mx[2] = fmaxf(mx[2], v[1][k]);
                 mx[3] = fmaxf(mx[3], v[1][k + 1]);
             }
-            // weights are exp2(S f + e_v - m): the tile's values are held divided by 2^e_v
-            const float f = fmaxf(f_row * pow2f(ek), 1.2e-38f);
-            float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, (float)ev);
+            float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f, e_top);
             tops[((i & 1) * 2 + half) * 128 + row] = top;
             if (!ok) *gave_up = 1;
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -406,14 +454,20 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 break;
             }
             top = fmaxf(top, other);  // (NaN where a row's scores all are: the weights then carry it)
-            const bool grow = top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY);
+            // weights of 2^7 to 2^15 at the largest: the top of f16's range, so that the smallest keep most bits
+            const bool grow = top > m_ref + 15.0f || (m_ref == -INFINITY && top > -INFINITY);
             float fix = 1.0f;
             if (grow) {
-                fix = exp2_approx(m_ref - top);  // 0 from -infinity
-                m_ref = top;
+                fix = exp2_approx(m_ref - (top - 7.0f));  // 0 from -infinity
+                m_ref = top - 7.0f;
                 l *= fix;
             }
-            const float off = (float)ev - (m_ref == -INFINITY ? 0.0f : m_ref);
+            const float off = e_top - (m_ref == -INFINITY ? 0.0f : m_ref);
+            float l_uneven = 0.0f;
+            if (uneven) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k) l_uneven += exp2_approx(v[k >> 5][k & 31] + off - e_of(k));
+            }
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t w[32];
 #pragma unroll
@@ -451,12 +505,13 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             umma::fence_smem_to_async();
             umma::fence_before_sync();
             mbar_arrive(p_ready);
-            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(-ev), l);
+            l = uneven ? l + l_uneven : fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(-ev), l);
             if (nb[0] | nb[1]) {  // values that are NaN: held as 0; rows that see one become NaN
                 for (int t = 0; t < 64; ++t)
                     if ((nb[t >> 5] >> (t & 31) & 1u) && t0 + t <= see_hi && t0 + t >= see_lo) l = NAN;
             }
         }
+        pdl_trigger();
         // the gates of the rows this warp will write, all requested before the last product is waited for
         uint4 graw[NL];
         if (a.gate) {
@@ -537,8 +592,25 @@ bool kv4_prompt_fits(const moe_engine* e, const AttnArgs& a) {
 }
 
 template <int D>
-int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
+int launch_kv4_prompt(moe_engine* e, AttnArgs& call) {
     using C = PtCfg<D>;
+    Kv4State& st = e->kv4;
+    if (!st.wide) {
+        const cudaError_t rc = cudaMalloc(&st.wide, 65536 * sizeof(unsigned));
+        if (rc != cudaSuccess) {
+            cudaGetLastError();
+            st.wide = nullptr;
+            return cuda_fail(rc, "kv4_attention: work area", __FILE__, __LINE__);
+        }
+        st.calls = 0xFFFFFFFFu;
+    }
+    if (++st.calls == 0) {  // the first, or all numbers used: none is anybody's
+        MOE_CUDA(cudaMemsetAsync(st.wide, 0, 65536 * sizeof(unsigned), e->stream));
+        st.calls = 1;
+    }
+    call.wide = st.wide;
+    call.call = st.calls;
+    AttnArgs a = call;
     const int tiles = pt_tiles_per_seq(a);
     const size_t image = pt_image_bytes<D>(a), meta = (size_t)pt_max_seqs(a) * a.cache.kv_heads * tiles * kPtMeta * 4;
     a.lo_rows = a.seqs.n_seqs == 1 ? 1 : kPromptRows;
@@ -572,8 +644,8 @@ int launch_kv4_prompt(moe_engine* e, AttnArgs a) {
 template bool kv4_prompt_fits<64>(const moe_engine*, const AttnArgs&);
 template bool kv4_prompt_fits<128>(const moe_engine*, const AttnArgs&);
 template bool kv4_prompt_fits<256>(const moe_engine*, const AttnArgs&);
-template int launch_kv4_prompt<64>(moe_engine*, AttnArgs);
-template int launch_kv4_prompt<128>(moe_engine*, AttnArgs);
-template int launch_kv4_prompt<256>(moe_engine*, AttnArgs);
+template int launch_kv4_prompt<64>(moe_engine*, AttnArgs&);
+template int launch_kv4_prompt<128>(moe_engine*, AttnArgs&);
+template int launch_kv4_prompt<256>(moe_engine*, AttnArgs&);
 
 }  // namespace moe

@@ -63,7 +63,7 @@ def close(got, want, size, reach, dtype, rows=slice(None)):
 
 
 # shapes that take every kernel: few rows (one and two columns of eight), many f32 rows, prompts of bf16 rows
-FORMS = [(t, lens, q_lens) for lens, q_lens in (([300], [1]), ([300, 200], [4, 3]), ([700, 600], [700, 600])) for t in (L.DT_F32, L.DT_BF16)][:-1]
+FORMS = [(t, lens, q_lens) for lens, q_lens in (([300], [1]), ([300, 200], [4, 3]), ([700, 600], [700, 600])) for t in (L.DT_F32, L.DT_BF16)]
 
 
 # ─── windows ────────────────────────────────────────────────────────────────
@@ -106,8 +106,8 @@ def test_widest_windows(eng, lens, q_lens, window, dtype):  # noqa: F811
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("big", [2.0 ** 11, 1e5, 1e8, 1e30])
 def test_large_values_that_rows_do_not_see(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
-    """Positions behind a row's own, or before its window, in the tile it reads: large values and keys there change nothing."""
-    for window in (0, 20):
+    """Positions behind a row's own, or before its window, in the tile it reads: large values (and keys) there change nothing."""
+    for window, keys in ((0, 1), (0, 0), (20, 1), (20, 0)):
         c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=11)
         k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
         at = 0
@@ -117,7 +117,8 @@ def test_large_values_that_rows_do_not_see(eng, big, dim, dtype, lens, q_lens): 
             base, pos = sum(lens[:b]), np.arange(n - nq, n)
             p = n - 1 if nq > 1 else n - 25  # the last row's own position; or one just before the window of the only row
             v[base + p] *= big
-            k[base + p] *= min(big, 1e15)
+            if keys:
+                k[base + p] *= min(big, 1e15)
             hidden[at:at + nq] = (pos < p) | ((pos - p >= window) if window else False)
             at += nq
         assert hit and (hidden.any() or window == 0)
@@ -165,6 +166,61 @@ def test_large_values_of_small_weight(eng, big, dim, dtype, lens, q_lens):  # no
         want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
         close(attend(eng, c, q, 8, dtype, scale=0.1), want, size, reach, dtype)
         c.free()
+
+
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("big", [1e3, 1e12, 1e30])
+def test_values_of_zero_with_the_largest_weight(eng, big, dtype, lens, q_lens):  # noqa: F811
+    """The first position takes most of the weight and holds zeros, the others hold large values."""
+    for dim in (64, 256):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=dim, page=16, seed=18)
+        k, v = (c.rng.standard_normal((sum(lens), 1, dim)).astype(np.float32) for _ in range(2))
+        v *= np.float32(big)
+        for b in range(len(lens)):
+            k[sum(lens[:b]), 0, 0] = 4.0
+            v[sum(lens[:b])] = 0.0
+        kc, vc = store(eng, c, k, v)
+        qf = c.rng.standard_normal((c.rows, 8, dim))
+        qf[..., 0] = 40.0
+        q = as_type(qf, dtype)
+        want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, 0, 0.1)
+        close(attend(eng, c, q, 8, dtype, scale=0.1), want, size, reach, dtype)
+        c.free()
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("window", [0, 90])
+def test_sequences_of_unequal_and_ordinary_values_in_one_call(eng, window, dtype):  # noqa: F811
+    """Prompts, verifications and single tokens, some of them over values and keys of very unequal size, gated; twice, so that
+    nothing of the first call decides about the second."""
+    lens, q_lens = [700, 300, 250, 90, 500, 0, 333], [700, 300, 1, 40, 350, 1, 333]
+    c = Case(eng, lens, q_lens, kv_heads=2, dim=128, page=16, seed=19)
+    first = np.cumsum([0] + lens)
+    for unequal in ((1, 2, 3), (0, 4), ()):
+        k, v = (c.rng.standard_normal((sum(lens), 2, 128)).astype(np.float32) for _ in range(2))
+        for b in unequal:
+            v[first[b] + 5:first[b + 1]:50, :, 64:] *= 1e7
+            k[first[b] + 30:first[b + 1]:70, 1, :64] *= 1e-7
+        kc, vc = store(eng, c, k, v)
+        q, g = (as_type(c.rng.standard_normal((c.rows, 8, 128)), dtype) for _ in range(2))
+        want, size, reach = R.attention(as_f64(q, dtype), kc, vc, lens, q_lens, window, 0.1)
+        s = 1 / (1 + np.exp(-as_f64(g, dtype)))
+        close(attend(eng, c, q, 8, dtype, scale=0.1, window=window, gate=g), want * s, size * s, reach, dtype)
+    c.free()
+
+
+def test_prompts_among_many_sequences(eng):  # noqa: F811
+    """More sequences than a CTA has threads before a prompt, and the images of two prompts."""
+    rng = np.random.default_rng(20)
+    lens, q_lens = [int(x) for x in rng.integers(0, 60, 700)], [1] * 700
+    for b, n in ((290, 150), (655, 70), (699, 210)):
+        lens[b], q_lens[b] = n, n - 3
+    c = Case(eng, lens, q_lens, kv_heads=2, dim=64, page=16, seed=20)
+    k, v = c.fill()
+    q = as_type(c.rng.standard_normal((c.rows, 4, 64)), L.DT_BF16)
+    want, size, reach = R.attention(as_f64(q, L.DT_BF16), k, v, lens, q_lens, 0, 0.1)
+    close(attend(eng, c, q, 4, L.DT_BF16, scale=0.1), want, size, reach, L.DT_BF16)
+    c.free()
 
 
 # A score is the sum over groups of s (q . n) and b sum(q), both of which may be larger than the sum of q_d k_d: its error is
