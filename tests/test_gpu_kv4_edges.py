@@ -266,3 +266,25 @@ def test_groups_of_equal_values(eng, dtype, lens, q_lens):  # noqa: F811
         close(got, want, size, reach, dtype)
         assert np.all(got[..., 64:128] == 0.0)
         c.free()
+
+
+# ─── gates ──────────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("lens,q_lens", [([40] * 600, [1] * 600), ([9000, 40], [1, 1]), ([700, 600], [700, 600]), ([300], [200])])
+@pytest.mark.parametrize("big", [1.0, 1e30])
+def test_gates_of_any_size(eng, big, lens, q_lens, dtype):  # noqa: F811
+    """The gated result against the same call's without gates, times sigmoid(gate) in 64 bits; whether a sequence was one CTA's or
+    several's.  f32: exp to 2 ulp (2^-22) in numerator and denominator, a product, a sum and a quotient (3 x 2^-24), the
+    rounding of the result without gates (2^-24): below 2^-20.  bf16: two roundings of half a step, 2 x 2^-8, and 2^-13."""
+    c = Case(eng, lens, q_lens, kv_heads=2, dim=64, page=16, seed=16)
+    k, v = (c.rng.standard_normal((sum(lens), 2, 64)).astype(np.float32) for _ in range(2))
+    store(eng, c, k, v * np.float32(big))
+    q = as_type(c.rng.standard_normal((c.rows, 16, 64)), dtype)
+    g = as_type(c.rng.uniform(-87, 87, (c.rows, 16, 64)), dtype)
+    plain = attend(eng, c, q, 16, dtype, scale=0.1)
+    got = attend(eng, c, q, 16, dtype, scale=0.1, gate=g)
+    want = plain / (1 + np.exp(-as_f64(g, dtype)))
+    assert np.isfinite(got).all() and np.abs(plain).max() > 0.1 * big
+    err = np.abs(got - want) / (np.abs(want) * (2.0 ** -20 if dtype == L.DT_F32 else 2.0 ** -7 + 2.0 ** -13) + 2.0 ** -126)
+    assert err.max() <= 1, err.max()
+    c.free()
