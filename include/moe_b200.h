@@ -358,7 +358,8 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  * the cache, touch no memory; they are MOE_ERR_INVALID at the next moe_engine_sync.
  *
  * moe_kv4_append_dev     stores the rows' keys and values [n_tokens, num_kv_heads, head_dim] (f32 or bf16, element strides),
- *                        keys rotated on the way when rope is given: by the position, or by rope_positions_dev[row].  Each
+ *                        keys rotated on the way when rope is given: by the position, or by rope_positions_dev[row].  A row
+ *                        whose position the table does not hold is not stored, neither key nor value, and reported.  Each
  *                        position of the cache is written at most once per call (sequences share no pages being written).
  *                        Values are finite; a group of 64 that holds an infinity or NaN is stored as NaN.
  * moe_kv4_gather_dev     the rows' stored keys and values as f32 or bf16 [n_tokens, num_kv_heads, head_dim], contiguous;

@@ -101,30 +101,50 @@ __device__ __forceinline__ int kv4_k_offset(int l, int t) {
     return (g / U) * (512 * U) + ((t & 1) * 8 + (t >> 1)) * (32 * U) + c * (8 * U) + (g % U) * 8 + j * 4;
 }
 
-// Stores four positions' words and pairs; [lo, hi): which of the four exist.
+// Of a quad's rows row0 + i (positions q0 + i), those that exist (lo <= i < hi) and that the rotary table has a row for, as bits:
+// the others are reported, their keys and values not stored.  at: their positions in the table.
+__device__ __forceinline__ unsigned kv4_live(const Kv4AppendArgs& a, int64_t row0, int q0, int lo, int hi, int (&at)[4], unsigned int* err) {
+    unsigned live = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        at[i] = 0;
+        if (i < lo || i >= hi) continue;
+        if (a.table) {
+            at[i] = a.rope_positions ? a.rope_positions[row0 + i] : q0 + i;
+            if (at[i] < 0 || at[i] >= a.n_positions) {
+                atomicExch(err, kErrRopePos);
+                continue;
+            }
+        }
+        live |= 1u << i;
+    }
+    return live;
+}
+
+// Stores four positions' words and pairs; live: which of the four there are.
 template <int D>
-__device__ __forceinline__ void kv4_store(uint8_t* nib, bool is_v, int l, int t0, int lo, int hi, const uint32_t (&word)[4], uint32_t pair) {
+__device__ __forceinline__ void kv4_store(uint8_t* nib, bool is_v, int l, int t0, unsigned live, const uint32_t (&word)[4], uint32_t pair) {
     if (!is_v) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i >= lo && i < hi) *reinterpret_cast<uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i)) = word[i];
+            if (live >> i & 1) *reinterpret_cast<uint32_t*>(nib + kv4_k_offset<D>(l, t0 + i)) = word[i];
     } else {
         // bytes of the four positions, elements (2x, 2x + 1): word x of the lane's 16
         uint8_t* dst = nib + (l >> 3) * 512 + (l & 7) * 64 + (t0 >> 2) * 16;
         uint32_t w[4];
         transpose_bytes(word, w);
-        if (lo <= 0 && hi == 4) {
+        if (live == 15u) {
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
             for (int x4 = 0; x4 < 4; ++x4)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (i >= lo && i < hi) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
+                    if (live >> i & 1) dst[4 * x4 + i] = (uint8_t)(w[x4] >> (8 * i));
         }
     }
     const int mine = l & 7;
-    if (mine >= lo && mine < hi) *(reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0 + mine) = pair;
+    if (mine < 4 && (live >> mine & 1)) *(reinterpret_cast<uint32_t*>(nib + 8 * D) + (l >> 3) * 16 + t0 + mine) = pair;
 }
 
 enum { kRotNone = 0, kRotHalf = 1, kRotInter = 2 };
@@ -164,18 +184,13 @@ __global__ void __launch_bounds__(D, 512 / D) kv4_append_heads_kernel(Kv4AppendA
     const float* turn_at[4];   // half: where those of the lane's eight elements are
     const int half = a.rotary >> 1;
     const bool turns = kRot != kRotNone && !is_v && 8 * l < a.rotary, second = kRot == kRotHalf && 8 * l >= half;
-    unsigned turned = 0;
+    int at[4];
+    const unsigned live = kv4_live(a, row0, q0, lo, hi, at, err), turned = turns ? live : 0;
     if (turns) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i < lo || i >= hi) continue;
-            const int64_t pos = a.rope_positions ? a.rope_positions[row0 + i] : q0 + i;
-            if (pos < 0 || pos >= a.n_positions) {
-                atomicExch(err, kErrRopePos);
-                continue;
-            }
-            turned |= 1u << i;
-            turn_at[i] = a.table + pos * a.rotary + (kRot == kRotInter ? 4 * l : second ? 8 * l - half : 8 * l);
+            if (!(turned >> i & 1)) continue;
+            turn_at[i] = a.table + (int64_t)at[i] * a.rotary + (kRot == kRotInter ? 4 * l : second ? 8 * l - half : 8 * l);
             if constexpr (kRot == kRotInter) {
                 *reinterpret_cast<float4*>(cs[i]) = *reinterpret_cast<const float4*>(turn_at[i]);
                 *reinterpret_cast<float4*>(sn[i]) = *reinterpret_cast<const float4*>(turn_at[i] + half);
@@ -230,7 +245,7 @@ __global__ void __launch_bounds__(D, 512 / D) kv4_append_heads_kernel(Kv4AppendA
         }
         uint32_t word[4];
         const uint32_t pair = kv4_quant(x, word);
-        if (blk && hi > lo) kv4_store<D>(blk + (h - h0) * head_bytes + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, lo, hi, word, pair);
+        if (blk && live) kv4_store<D>(blk + (h - h0) * head_bytes + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, live, word, pair);
     }
 }
 
@@ -250,22 +265,19 @@ __global__ void __launch_bounds__(D, 1024 / D) kv4_append_kernel(Kv4AppendArgs a
     const int lo = max(first - q0, 0), hi = min(s.len - q0, 4);
     uint8_t* const blk = kv4_block(a.cache, a.seqs, b, h, p0, kv4_block_bytes(D), err);
 
+    int at[4];
+    const unsigned live = kv4_live(a, (int64_t)row_of + q0, q0, lo, hi, at, err);
     float x[4][8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
-        if (i < lo || i >= hi) continue;
+        if (!(live >> i & 1)) continue;
         const int64_t row = row_of + (q0 + i);
         const T* src = is_v ? (const T*)a.v + row * a.vt + (int64_t)h * a.vh : (const T*)a.k + row * a.kt + (int64_t)h * a.kh;
         ld_act8(src + 8 * l, is_v ? a.vec_v : a.vec_k, x[i]);
         if (is_v || !a.table || 8 * l >= a.rotary) continue;
-        const int64_t pos = a.rope_positions ? a.rope_positions[row] : q0 + i;
-        if (pos < 0 || pos >= a.n_positions) {
-            atomicExch(err, kErrRopePos);
-            continue;
-        }
-        const float* cs = a.table + pos * a.rotary;
+        const float* cs = a.table + (int64_t)at[i] * a.rotary;
         const int half = a.rotary >> 1;
         if (a.interleaved) {
             float ct[4], st[4];
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(D, 1024 / D) kv4_append_kernel(Kv4AppendArgs a
     }
     uint32_t word[4];
     const uint32_t pair = kv4_quant(x, word);
-    if (blk && hi > lo) kv4_store<D>(blk + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, lo, hi, word, pair);
+    if (blk && live) kv4_store<D>(blk + (is_v ? 9 * D : 0), is_v, l, q0 % kKv4Block, live, word, pair);
 }
 
 // The way back: same mapping, values = nibble * scale + bias (the product is exact, so one rounding).

@@ -288,3 +288,39 @@ def test_gates_of_any_size(eng, big, lens, q_lens, dtype):  # noqa: F811
     err = np.abs(got - want) / (np.abs(want) * (2.0 ** -20 if dtype == L.DT_F32 else 2.0 ** -7 + 2.0 ** -13) + 2.0 ** -126)
     assert err.max() <= 1, err.max()
     c.free()
+
+
+# ─── rotary positions outside the table ─────────────────────────────────────
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("lens,q_lens,kv_heads,dim,rotary,interleaved", [([40, 21], [19, 2], 2, 128, 64, 0), ([40, 21], [19, 2], 2, 128, 20, 1), ([40, 21], [19, 2], 1, 64, 64, 1),
+                                                                         ([1813, 1502], [1810, 1502], 8, 64, 32, 1), ([1813, 1502], [1810, 1502], 6, 256, 64, 0)])
+def test_append_skips_rows_without_a_rotation(eng, lens, q_lens, kv_heads, dim, rotary, interleaved, dtype):  # noqa: F811
+    """A row whose position the table does not hold is reported, and neither its key nor its value is stored; the others are."""
+    from moe_infer_b200.native import RopeTable, rope_table
+    c = Case(eng, lens, q_lens, kv_heads=kv_heads, dim=dim, page=48, seed=17)
+    k_old, v_old = c.fill()
+    k, v = (as_type(c.rng.standard_normal((c.rows, kv_heads, dim)), dtype) for _ in range(2))
+    tab = rope_table(rotary, 500, 1e4)
+    pos = c.rng.integers(0, 500, c.rows).astype(np.int32)
+    bad = c.rng.random(c.rows) < 0.2
+    bad[[0, c.rows - 1]] = True
+    pos[bad] = c.rng.choice([-1, 500, 1 << 30, -(1 << 31)], bad.sum())
+    rope = RopeTable(c.up(tab).ptr, 500, rotary, interleaved)
+    eng.kv4_append_dev(c.cache, c.batch, c.up(k).ptr, c.up(v).ptr, dtype, rope=rope, rope_positions=c.up(pos).ptr)
+    with pytest.raises(ValueError, match="rotary table"):
+        eng.sync()
+    ko, vo = c.up(np.zeros(k.shape, np.float32)), c.up(np.zeros(k.shape, np.float32))
+    eng.kv4_gather_dev(c.cache, c.batch, ko.ptr, vo.ptr, L.DT_F32)
+    eng.sync()
+    own = np.concatenate([np.arange(sum(lens[:b]) + n - nq, sum(lens[:b]) + n) for b, (n, nq) in enumerate(zip(lens, q_lens))])
+    kf, vf = as_f64(k, dtype).astype(np.float32), as_f64(v, dtype).astype(np.float32)
+    k_new = R.codec(R.rotate_f32(kf, tab[np.where(bad, 0, pos)], interleaved))
+    np.testing.assert_array_equal(ko.download(np.float32, k.shape), np.where(bad[:, None, None], k_old[own], k_new))
+    np.testing.assert_array_equal(vo.download(np.float32, k.shape), np.where(bad[:, None, None], v_old[own], R.codec(vf)))
+    # the same for positions that follow from the cache and pass the table's end
+    short = RopeTable(c.up(tab).ptr, max(lens) - 1, rotary, interleaved) if max(lens) <= 500 else None
+    if short:
+        eng.kv4_append_dev(c.cache, c.batch, c.up(k).ptr, c.up(v).ptr, dtype, rope=short)
+        with pytest.raises(ValueError, match="rotary table"):
+            eng.sync()
+    c.free()
