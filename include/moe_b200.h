@@ -376,7 +376,7 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        over keys with a group below 2^-11 of its 128 neighbours' largest, or values with one below 2^-9 of their
  *                        position's, zeros aside, is computed without f16 keys and values, more slowly.)  A row that sees a value stored as NaN is NaN in that group of
  *                        64 (in a prompt, in the whole row).  Prompts of bf16 rows need a work area, the positions they see as
- *                        f16 (4 head_dim bytes per position and KV head), grown on demand and kept by the engine; calls whose
+ *                        f16 (4 head_dim bytes per position and KV head), grown on demand (by half at least) and kept by the engine; calls whose
  *                        bounds could need more than 4 GB of it run without, more slowly.
  * head_dim is 64, 128 or 256; page_size a multiple of 16. */
 typedef struct {

@@ -1065,16 +1065,23 @@ void kv4_destroy(moe_engine* e) {
 int kv4_reserve(moe_engine* e, size_t bytes) {
     if (bytes <= e->kv4.work_bytes) return MOE_OK;
     MOE_CUDA(cudaStreamSynchronize(e->stream));
+    // by half at least: the chunks of a prompt need a little more each time
+    size_t want = e->kv4.work_bytes + e->kv4.work_bytes / 2;
+    if (want < bytes) want = bytes;
     if (e->kv4.work) cudaFree(e->kv4.work);
     e->kv4.work = nullptr;
     e->kv4.work_bytes = 0;
-    const cudaError_t err = cudaMalloc(&e->kv4.work, bytes);
+    cudaError_t err = cudaMalloc(&e->kv4.work, want);
+    if (err != cudaSuccess && want > bytes) {
+        cudaGetLastError();
+        err = cudaMalloc(&e->kv4.work, want = bytes);
+    }
     if (err != cudaSuccess) {
         cudaGetLastError();  // the next call starts clean
         e->kv4.work = nullptr;
         return cuda_fail(err, "kv4_attention: work area", __FILE__, __LINE__);
     }
-    e->kv4.work_bytes = bytes;
+    e->kv4.work_bytes = want;
     return MOE_OK;
 }
 

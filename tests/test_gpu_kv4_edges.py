@@ -324,3 +324,29 @@ def test_append_skips_rows_without_a_rotation(eng, lens, q_lens, kv_heads, dim, 
         with pytest.raises(ValueError, match="rotary table"):
             eng.sync()
     c.free()
+
+
+# ─── the call's work area ───────────────────────────────────────────────────
+def test_work_area_grows_in_steps(native_lib):
+    """A prompt in chunks: each call may need a little more than the one before, and few of them allocate."""
+    import ctypes
+    from moe_infer_b200.native import Dims, NativeEngine
+    cu, free, total = ctypes.CDLL("libcuda.so.1"), ctypes.c_size_t(), ctypes.c_size_t()
+    e = NativeEngine(Dims(num_experts=4, top_k=4, num_layers=1))
+    n = 64 * 128
+    c = Case(e, [n], [128], kv_heads=8, dim=256, page=16, seed=22)
+    c.fill()
+    q = c.up(as_type(c.rng.standard_normal((128, 8, 256)), L.DT_BF16))
+    out = c.up(np.zeros((128, 8, 256), np.uint16))
+    changes, last = 0, None
+    for chunk in range(1, 65):
+        e.kv4_attention_dev(c.cache, c.batch_of([0, 128], 128, 128, [128 * chunk]), q.ptr, out.ptr, L.DT_BF16, 8, scale=0.1)
+        e.sync()
+        c.keep.pop().free(), c.keep.pop().free(), c.keep.pop().free()  # the batch's arrays
+        assert cu.cuMemGetInfo_v2(ctypes.byref(free), ctypes.byref(total)) == 0
+        changes += last is not None and abs(free.value - last) >= 1 << 20
+        last = free.value
+    # from 1 tile to 64 by a factor of 1.5 each: 11 steps
+    assert changes <= 12, changes
+    c.free()
+    e.close()
