@@ -39,6 +39,10 @@ struct Kv4Seqs {               // moe_kv4_batch_t as the kernels take it
     int n_seqs, n_tokens, max_pages, max_seq_len, max_q_len;
 };
 
+int check_kv4(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b);
+Kv4View kv4_view(const moe_kv4_cache_t* c);
+Kv4Seqs kv4_seqs(const moe_kv4_batch_t* b);
+
 // device error codes (engine error word); mapped to messages in engine.cu
 constexpr unsigned kErrKv4Page = 12u;    // page table entry outside the cache
 constexpr unsigned kErrRopePos = 13u;    // position outside the rotary table

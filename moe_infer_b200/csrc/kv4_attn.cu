@@ -1177,10 +1177,6 @@ static int launch_attn(moe_engine* e, const AttnArgs& a) {
     return launch_rows<D, T>(e, a, (int64_t)a.seqs.max_q_len * a.group);
 }
 
-int check_kv4(const moe_kv4_cache_t* c, const moe_kv4_batch_t* b);
-Kv4View kv4_view(const moe_kv4_cache_t* c);
-Kv4Seqs kv4_seqs(const moe_kv4_batch_t* b);
-
 }  // namespace moe
 
 using namespace moe;

@@ -327,6 +327,26 @@ def test_append_skips_rows_without_a_rotation(eng, lens, q_lens, kv_heads, dim, 
 
 
 # ─── the call's work area ───────────────────────────────────────────────────
+def test_capture_is_refused(eng):  # noqa: F811
+    """The work area moves when it grows, so attention is not captured; the capture itself and the engine go on."""
+    import ctypes
+    cu = ctypes.CDLL("libcuda.so.1")
+    c = Case(eng, [300], [300], kv_heads=1, dim=64, page=16, seed=21)
+    k, v = c.fill()
+    stream, graph = ctypes.c_void_p(eng.stream()), ctypes.c_void_p()
+    for dtype in (L.DT_F32, L.DT_BF16):
+        q = as_type(c.rng.standard_normal((c.rows, 4, 64)), dtype)
+        qb, out = c.up(q), c.up(np.zeros_like(q))
+        assert cu.cuStreamBeginCapture_v2(stream, 2) == 0
+        with pytest.raises(L.MoeError, match="captured"):
+            eng.kv4_attention_dev(c.cache, c.batch, qb.ptr, out.ptr, dtype, 4, scale=0.1)
+        assert cu.cuStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert cu.cuGraphDestroy(graph) == 0
+        want, size, reach = R.attention(as_f64(q, dtype), k, v, [300], [300], 0, 0.1)
+        close(attend(eng, c, q, 4, dtype, scale=0.1), want, size, reach, dtype)
+    c.free()
+
+
 def test_work_area_grows_in_steps(native_lib):
     """A prompt in chunks: each call may need a little more than the one before, and few of them allocate."""
     import ctypes
