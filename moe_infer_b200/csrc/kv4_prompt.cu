@@ -27,6 +27,9 @@ constexpr int kPtTile = 128;                 // positions of a tile, rows of a C
 // ints per tile: exponent of K; twice that of V, and 1 if every position has an exponent of its own; four words of "value is
 // NaN" bits; the positions' exponents (f32) from the eighth on
 constexpr int kPtMeta = 8 + kPtTile;
+// exponents of tiles and positions, and the power of two that a row's sum of weights is held in: weights reach 2^15 2^100 where the
+// values are all zero, 2^24 of them 2^139
+constexpr int kPtLow = -100, kPtHigh = 114, kPtSum = -12;
 constexpr float kKeySpan = 1.0f / 2048, kValueSpan = 1.0f / 512, kEven = 1.0f / 8;
 
 template <int D>
@@ -126,8 +129,8 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     const bool here = tid < kPtTile && p0 + tid < s.len && blocks[(tid & (kPtTile - 1)) >> 4];
     if (is_v ? here && least < top * kValueSpan : tid == 0 && mn < mx * kKeySpan) a.wide[b] = a.call;
     const bool uneven = __syncthreads_or(is_v && here && top < mx * kEven);
-    // scaled into [1, 2); what is all zero keeps a harmless exponent
-    auto exponent = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126); };
+    // scaled into [1, 2) (from 2^115 on into up to 2^14); what is all zero lifts nothing
+    auto exponent = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) - 127, kPtLow), kPtHigh); };
     const int e = exponent(mx);
     if (tid < kPtTile) down[tid] = pow2f(-(uneven ? exponent(top) : e));
     __syncthreads();
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             float l_uneven = 0.0f;
             if (uneven) {
 #pragma unroll
-                for (int k = 0; k < 64; ++k) l_uneven += exp2_approx(v[k >> 5][k & 31] + off - e_of(k));
+                for (int k = 0; k < 64; ++k) l_uneven += exp2_approx(v[k >> 5][k & 31] + off - e_of(k) + (float)kPtSum);
             }
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             uint32_t w[32];
@@ -505,7 +508,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
             umma::fence_smem_to_async();
             umma::fence_before_sync();
             mbar_arrive(p_ready);
-            l = uneven ? l + l_uneven : fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(-ev), l);
+            l = uneven ? l + l_uneven : fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2f(kPtSum - ev), l);
             if (nb[0] | nb[1]) {  // values that are NaN: held as 0; rows that see one become NaN
                 for (int t = 0; t < 64; ++t)
                     if ((nb[t >> 5] >> (t & 31) & 1u) && t0 + t <= see_hi && t0 + t >= see_lo) l = NAN;
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
         tops[half * 128 + row] = l;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         l += tops[(half ^ 1) * 128 + row];
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : pow2f(kPtSum) / l;
         // through shared memory (where K and V were: every product has been waited for), so that rows are written whole
         float* stage = reinterpret_cast<float*>(sm + C::OFF_K);
 #pragma unroll 1

@@ -189,6 +189,25 @@ def test_values_of_zero_with_the_largest_weight(eng, big, dtype, lens, q_lens): 
 
 
 @pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
+@pytest.mark.parametrize("small", [0.0, 1e-12, 1e-30])
+def test_long_runs_of_zeros(eng, small, dtype):  # noqa: F811
+    """Thousands of positions whose values are zeros (or tiny) take all of the weight, scores a little above the first ones'."""
+    n, rows = 20000, 200
+    c = Case(eng, [n], [rows], kv_heads=1, dim=64, page=64, seed=23)
+    k, v = (0.01 * c.rng.standard_normal((n, 1, 64)).astype(np.float32) for _ in range(2))
+    k[128:, 0, 0] = 1.369  # 7.9 powers of two above the first 128
+    v[:n - rows] *= np.float32(small)
+    k[n - rows:, 0, 0] = 0.0
+    kc, vc = store(eng, c, k, v)
+    qf = c.rng.standard_normal((rows, 4, 64))
+    qf[..., 0] = 40.0
+    q = as_type(qf, dtype)
+    want, size, reach = R.attention(as_f64(q, dtype), kc, vc, [n], [rows], 0, 0.1)
+    close(attend(eng, c, q, 4, dtype, scale=0.1), want, size, reach, dtype)
+    c.free()
+
+
+@pytest.mark.parametrize("dtype", [L.DT_F32, L.DT_BF16])
 @pytest.mark.parametrize("window", [0, 90])
 def test_sequences_of_unequal_and_ordinary_values_in_one_call(eng, window, dtype):  # noqa: F811
     """Prompts, verifications and single tokens, some of them over values and keys of very unequal size, gated; twice, so that
