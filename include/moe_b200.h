@@ -373,9 +373,9 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        (2^-12), and for sequences of at least 128 rows x query heads per KV head (prompts) keys and values
  *                        too; scores, sums and the softmax f32.  Sizes of keys and values may differ as they like: what is lost
  *                        is relative to the weighted |values| and ranges of the same group of 64 that the row sees.  (A prompt
- *                        over keys with a group below 2^-11 of its 128 neighbours' largest, or values with one below 2^-9 of their
- *                        position's, zeros aside, is computed without f16 keys and values, more slowly.)  A row that sees a value stored as NaN is NaN in that group of
- *                        64 (in a prompt, in the whole row).  Prompts of bf16 rows need a work area, the positions they see as
+ *                        over keys with a group below 2^-12 of its 128 neighbours' largest, or values with one below 2^-12 of
+ *                        their position's, zeros aside, is computed without f16 keys and values, more slowly.)  A row that sees
+ *                        a value stored as NaN is NaN in that group of 64 (in a prompt, in the whole row).  Prompts of bf16 rows need a work area, the positions they see as
  *                        f16 (4 head_dim bytes per position and KV head), grown on demand (by half at least) and kept by the engine; calls whose
  *                        bounds could need more than 4 GB of it run without, more slowly.
  * head_dim is 64, 128 or 256; page_size a multiple of 16. */

@@ -3,10 +3,11 @@
 // With hundreds of rows per position the products dominate (4 D flops per row, head and position) and every position is
 // read by many row tiles, so the positions the call sees are first expanded, once, into f16 tiles of 128 positions that
 // lie in memory exactly as the MMAs want them in shared memory (K-major, 128-byte swizzle): a tile then arrives by plain
-// bulk copies.  Keys of a tile are scaled by a power of two, values by one per tile or, where the tile's positions differ by
-// more than 2^3, one per position, which the weights carry: so only what a row sees decides how its weights are scaled.  f16
-// keeps 11 bits down to 2^-14: a sequence with a key group of 64 below 2^-11 of its tile's largest key, or a value group below
-// 2^-9 of its position's largest value (groups of zeros aside), is left to the kernel of few rows, which has no such limit.
+// bulk copies.  f16 keeps 11 bits down to 2^-14.  Keys of a tile are scaled by a power of two, values by one per tile or, where
+// positions differ by more than 2^5 or a group of 64 lies below 2^-12 of the tile's largest, by one per position, which the
+// weights carry: so only what a row sees decides how its weights are scaled (8,192 rows: 505 us, with every tile of the second kind
+// 837).  A sequence with a key group below 2^-12 of its tile's largest key or a value group below 2^-12 of its position's
+// largest (zeros aside) is left to the kernel of few rows, which has no such limits (6.2 ms).
 //
 // Attention kernel: a CTA owns 128 rows (of the query heads that share a KV head) and walks its positions.  One thread
 // copies, one issues MMAs, eight warps hold a row per pair of threads (half a tile's positions, then half of O, each):
@@ -30,7 +31,7 @@ constexpr int kPtMeta = 8 + kPtTile;
 // exponents of tiles and positions, and the power of two that a row's sum of weights is held in: weights reach 2^15 2^100 where the
 // values are all zero, 2^24 of them 2^139
 constexpr int kPtLow = -100, kPtHigh = 114, kPtSum = -12;
-constexpr float kKeySpan = 1.0f / 2048, kValueSpan = 1.0f / 512, kEven = 1.0f / 8;
+constexpr float kSpan = 1.0f / 4096, kEven = 1.0f / 32;
 
 template <int D>
 struct PtCfg {
@@ -127,8 +128,8 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(AttnArgs a, int tiles_p
     mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     mn = fminf(fminf(red[8], red[9]), fminf(red[10], red[11]));
     const bool here = tid < kPtTile && p0 + tid < s.len && blocks[(tid & (kPtTile - 1)) >> 4];
-    if (is_v ? here && least < top * kValueSpan : tid == 0 && mn < mx * kKeySpan) a.wide[b] = a.call;
-    const bool uneven = __syncthreads_or(is_v && here && top < mx * kEven);
+    if (is_v ? here && least < top * kSpan : tid == 0 && mn < mx * kSpan) a.wide[b] = a.call;
+    const bool uneven = __syncthreads_or(is_v && here && (top < mx * kEven || least < mx * kSpan));
     // scaled into [1, 2) (from 2^115 on into up to 2^14); what is all zero lifts nothing
     auto exponent = [](float m) { return min(max((int)(__float_as_uint(m) >> 23) - 127, kPtLow), kPtHigh); };
     const int e = exponent(mx);

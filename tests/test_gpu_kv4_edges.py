@@ -104,7 +104,7 @@ def test_widest_windows(eng, lens, q_lens, window, dtype):  # noqa: F811
 # that a row does not see hold adds nothing to it.
 @pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("big", [2.0 ** 11, 1e5, 1e8, 1e30])
+@pytest.mark.parametrize("big", [2.0 ** 4, 2.0 ** 11, 1e5, 1e8, 1e30])
 def test_large_values_that_rows_do_not_see(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
     """Positions behind a row's own, or before its window, in the tile it reads: large values (and keys) there change nothing."""
     for window, keys in ((0, 1), (0, 0), (20, 1), (20, 0)):
@@ -133,7 +133,7 @@ def test_large_values_that_rows_do_not_see(eng, big, dim, dtype, lens, q_lens): 
 
 @pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
 @pytest.mark.parametrize("dim", [128, 256])
-@pytest.mark.parametrize("big", [2.0 ** 11, 1e5, 1e8, 1e30, 1e-8, 1e-30])
+@pytest.mark.parametrize("big", [2.0 ** 5, 2.0 ** 11, 2.0 ** 13, 1e5, 1e8, 1e30, 1e-3, 1e-8, 1e-30])
 def test_groups_of_unequal_size(eng, big, dim, dtype, lens, q_lens):  # noqa: F811
     """One group of 64 of a head holds values `big` times the others', at all positions or at a few."""
     for every in (1, 97):
