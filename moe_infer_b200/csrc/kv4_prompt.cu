@@ -458,6 +458,12 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                 break;
             }
             top = fmaxf(top, other);  // (NaN where a row's scores all are: the weights then carry it)
+            if (fabsf(top) > 65536.0f && top > -INFINITY) {  // scores whose own rounding exp2 would show: rounded first, like top
+#pragma unroll
+                for (int k = 0; k < 64; ++k) v[k >> 5][k & 31] = fmaf(v[k >> 5][k & 31], f, e_top);
+                f = 1.0f;
+                e_top = 0.0f;
+            }
             // weights of 2^7 to 2^15 at the largest: the top of f16's range, so that the smallest keep most bits
             const bool grow = top > m_ref + 15.0f || (m_ref == -INFINITY && top > -INFINITY);
             float fix = 1.0f;

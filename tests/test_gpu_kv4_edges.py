@@ -242,6 +242,50 @@ def test_prompts_among_many_sequences(eng):  # noqa: F811
     c.free()
 
 
+@pytest.mark.parametrize("dtype,lens,q_lens", FORMS)
+@pytest.mark.parametrize("big", [1e3, 1e5, 1e15])
+def test_scores_of_any_size(eng, big, dtype, lens, q_lens):  # noqa: F811
+    """Scores up to 10^31: the position with the largest one (by a thousandth of what scores are made of) is the result."""
+    c = Case(eng, lens, q_lens, kv_heads=1, dim=64, page=16, seed=24)
+    k, v = (c.rng.standard_normal((sum(lens), 1, 64)).astype(np.float32) for _ in range(2))
+    kc, vc = store(eng, c, k * np.float32(big), v)
+    q = as_type(c.rng.standard_normal((c.rows, 8, 64)) * big, dtype)
+    got = attend(eng, c, q, 8, dtype, scale=0.1)
+    assert np.isfinite(got).all()
+    qd, at, seen = as_f64(q, dtype), 0, 0
+    for b, (n, nq) in enumerate(zip(lens, q_lens)):
+        kb, vb = (x[sum(lens[:b]):sum(lens[:b]) + n, 0].astype(np.float64) for x in (kc, vc))
+        for h in range(8):
+            s = 0.1 * qd[at:at + nq, h] @ kb.T
+            s[np.arange(n)[None] > np.arange(n - nq, n)[:, None]] = -np.inf
+            best = s.argmax(1)
+            rest = s.copy()
+            rest[np.arange(nq), best] = -np.inf
+            sure = s.max(1) - rest.max(1) > 1e-3 * 0.1 * (np.abs(qd[at:at + nq, h]) @ np.abs(kb).max(0))
+            err = np.abs(got[at:at + nq, h] - vb[best])[sure]
+            # one weight, 1: what is left is the value's own rounding (2^-8, or 2^-19 of the group's range and |value|)
+            assert np.all(err <= np.abs(vb[best])[sure] * 2.0 ** -8 + 8 * 2.0 ** (-19 if dtype == L.DT_F32 else -11))
+            seen += sure.sum()
+        at += nq
+    assert seen > 0
+    c.free()
+
+
+@pytest.mark.parametrize("heads", [128, 130])
+def test_many_heads_per_kv_head(eng, heads):  # noqa: F811
+    """One token's query heads alone are a prompt's rows; with values that such a kernel leaves to the other."""
+    lens, q_lens = [300, 200, 50, 0, 90], [1, 4, 20, 1, 90]
+    for big in (1.0, 1e6):
+        c = Case(eng, lens, q_lens, kv_heads=1, dim=128, page=16, seed=25)
+        k, v = (c.rng.standard_normal((sum(lens), 1, 128)).astype(np.float32) for _ in range(2))
+        v[10:320:20, :, 64:] *= big
+        kc, vc = store(eng, c, k, v)
+        q = as_type(c.rng.standard_normal((c.rows, heads, 128)), L.DT_BF16)
+        want, size, reach = R.attention(as_f64(q, L.DT_BF16), kc, vc, lens, q_lens, 0, 0.1)
+        close(attend(eng, c, q, heads, L.DT_BF16, scale=0.1), want, size, reach, L.DT_BF16)
+        c.free()
+
+
 # A score is the sum over groups of s (q . n) and b sum(q), both of which may be larger than the sum of q_d k_d: its error is
 # relative to sum |q_d| (|k_d| + 15 s), not to sum |q_d k_d| alone.  2^-24 of it for each of the (at most three) f32 roundings of
 # a group's terms, 2^-23 for the 22-bit query operands, some 2^-22 for the MMA's sums: 2^-21, and a weight is off by twice that.
