@@ -12,8 +12,8 @@
 // of two; for f32 rows they are split into a high and a low f16 term (22 bits) that two MMAs add into the same sums, for bf16
 // rows one term is exact (queries) or three bits finer than the result's type (weights).  Sums and the softmax are f32.
 //
-// Weights are w = exp2(x - ref), one reference per row, a whole number: it moves only when a score passes it, then to 2^8
-// above.  As operands the products w s are scaled by a power of two, one per row and group, that moves only when a
+// Weights are w = exp2(x - ref), one reference per row: it moves only when a score passes it, then to 2^8 above (so the largest
+// weight, which counts most, is a power of two and loses nothing as an operand).  As operands the products w s are scaled by a power of two, one per row and group, that moves only when a
 // product would leave f16's range: a group's bits depend on the products that the row sees in that group, not on other groups
 // or on positions hidden from it.
 //
@@ -438,10 +438,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
             }
         }
 
-        // row r's products times 2^k from now on, its sums so far times 2^by (not above 1)
-        auto set_power = [&](int nt, int k, int by) {
+        // row r's products times 2^k from now on, its sums so far times 2^(by + part) (not above 1)
+        auto set_power = [&](int nt, int k, int by, float part) {
             power[nt] = pow2f(k);
-            const float f = pow2f(max(by, -126));
+            const float f = pow2f(max(by, -126)) * exp2_approx(part);
             const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);  // of rows 2 c, 2 c + 1
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                 for (int e = 0; e < 2; ++e) {
                     const bool mv = use[nt][e] > ref[nt][e];
                     moved |= mv;
-                    use[nt][e] = mv ? ceilf(use[nt][e]) + kRefAbove : ref[nt][e];
+                    use[nt][e] = mv ? use[nt][e] + kRefAbove : ref[nt][e];
                     const float off = use[nt][e] == -INFINITY ? 0.0f : use[nt][e];
                     sum[nt][e] = 0.0f;
 #pragma unroll
@@ -629,9 +629,10 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                     const float x0 = __shfl_sync(0xffffffffu, fix[0], r >> 1), x1 = __shfl_sync(0xffffffffu, fix[1], r >> 1);
                     const float u0 = __shfl_sync(0xffffffffu, up[0], r >> 1), u1 = __shfl_sync(0xffffffffu, up[1], r >> 1);
                     o_bias[nt] *= (r & 1) ? x1 : x0;
-                    // the sums of the products stay as they are, their power of two grows with the reference
-                    const int k = exponent_of(power[nt]) + (int)fminf((r & 1) ? u1 : u0, 1000.0f);
-                    set_power(nt, min(k, 126), min(126 - k, 0));
+                    // the sums of the products stay what they are, their power of two grows with the reference
+                    const float u = fminf((r & 1) ? u1 : u0, 1000.0f), whole_u = floorf(u);
+                    const int k = exponent_of(power[nt]) + (int)whole_u;
+                    set_power(nt, min(k, 126), min(126 - k, 0), whole_u - u);
                 }
                 compute_barrier();
             }
@@ -736,7 +737,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                     m[nt] = fmaxf(m[nt], __shfl_xor_sync(0xffffffffu, m[nt], 1));
                     m[nt] = fmaxf(m[nt], __shfl_xor_sync(0xffffffffu, m[nt], 2));
                     const int old = exponent_of(power[nt]), k = m[nt] * power[nt] > kProdTop ? min(kProdSet - exponent_of(m[nt]), 126) : old;
-                    set_power(nt, k, k - old);
+                    set_power(nt, k, k - old, 0.0f);
                 }
             };
             Pairs b[C::F32 ? 1 : PB];
