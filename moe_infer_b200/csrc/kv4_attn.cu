@@ -821,6 +821,12 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
                     const int j = over_group(rr, a.by_group);
                     ld_act8(gatep + (int64_t)(u.row0 + j) * a.gt + (int64_t)(u.h * a.group + rr - j * a.group) * a.gh + d0, a.vec_gate, gt[nt][e]);
                 }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) gt[nt][e][n] = sigmoid<T>(gt[nt][e][n]);
         }
         compute_barrier();
         float* slot = nullptr;
@@ -870,7 +876,7 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 #pragma unroll
                         for (int n = 0; n < 8; ++n) {
                             y[n] *= inv;
-                            if (gatep) y[n] = gated<T>(y[n], gt[nt][e][n]);
+                            if (gatep) y[n] *= gt[nt][e][n];
                         }
                         st_act8(outp + ((int64_t)(u.row0 + j) * a.heads + u.h * a.group + rr - j * a.group) * D + d0, true, y);
                     }
@@ -1049,7 +1055,7 @@ __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int spli
     if (a.gate) {
         const T* gp = (const T*)a.gate + (int64_t)(s.row0 + j) * a.gt + (int64_t)hq * a.gh + 4 * col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = gated<T>(y[i], ld_act(gp + i));
+        for (int i = 0; i < 4; ++i) y[i] *= sigmoid<T>(ld_act(gp + i));
     }
     T* dst = (T*)a.out + ((int64_t)(s.row0 + j) * a.heads + hq) * D + 4 * col;
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);

@@ -110,12 +110,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));  // without ftz the compiler adds three instructions for results below 2^-126
     return r;
 }
-// y * sigmoid(g), as y t / (1 + t) or y / (1 + t) with t = exp(-|g|), which never overflows; the quotient to 2 ulp.  f32 rows: t to
-// 2 ulp, all of it below 2^-20; bf16 rows: t to 2 + 1.2 |g| ulp, a 2^-14th where |g| reaches 87.
+// sigmoid(g), as t / (1 + t) or 1 / (1 + t) with t = exp(-|g|), which never overflows; the quotient to 2 ulp.  f32 rows: t to 2 ulp,
+// all of it below 2^-20; bf16 rows: t to 2 + 1.2 |g| ulp, a 2^-14th where |g| reaches 87.
 template <typename T>
-__device__ __forceinline__ float gated(float y, float g) {
+__device__ __forceinline__ float sigmoid(float g) {
     const float t = sizeof(T) == 4 ? expf(-fabsf(g)) : __expf(-fabsf(g));
-    return __fdividef(g < 0.0f ? y * t : y, 1.0f + t);
+    return __fdividef(g < 0.0f ? t : 1.0f, 1.0f + t);
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }

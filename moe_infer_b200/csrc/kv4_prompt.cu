@@ -563,8 +563,8 @@ __global__ void __launch_bounds__(320) kv4_prompt_kernel(AttnArgs a, int tiles_p
                     const uint32_t w[4] = {graw[i].x, graw[i].y, graw[i].z, graw[i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        y[2 * k] = gated<__nv_bfloat16>(y[2 * k], __uint_as_float(w[k] << 16));
-                        y[2 * k + 1] = gated<__nv_bfloat16>(y[2 * k + 1], __uint_as_float(w[k] & 0xFFFF0000u));
+                        y[2 * k] *= sigmoid<__nv_bfloat16>(__uint_as_float(w[k] << 16));
+                        y[2 * k + 1] *= sigmoid<__nv_bfloat16>(__uint_as_float(w[k] & 0xFFFF0000u));
                     }
                 }
                 st_act8((__nv_bfloat16*)a.out + ((int64_t)(s.row0 + jj) * a.heads + h * a.group + rr2 - jj * a.group) * D + 8 * lc, true, y);

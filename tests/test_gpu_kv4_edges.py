@@ -337,7 +337,7 @@ def test_groups_of_equal_values(eng, dtype, lens, q_lens):  # noqa: F811
 @pytest.mark.parametrize("big", [1.0, 1e30])
 def test_gates_of_any_size(eng, big, lens, q_lens, dtype):  # noqa: F811
     """The gated result against the same call's without gates, times sigmoid(gate) in 64 bits; whether a sequence was one CTA's or
-    several's.  f32: exp to 2 ulp (2^-22) in the numerator, half of that in the denominator, a product and a sum (2 x 2^-24), a
+    several's.  f32: exp to 2 ulp (2^-22) in the numerator, half of that in the denominator, a sum and a product (2 x 2^-24), a
     quotient to 2 ulp (2^-22), the rounding of the result without gates (2^-24): below 2^-20.  bf16: two roundings of half a
     step, 2 x 2^-8, and 2^-13."""
     c = Case(eng, lens, q_lens, kv_heads=2, dim=64, page=16, seed=16)
