@@ -117,10 +117,18 @@ __device__ AttnPlan attn_scan(const AttnArgs& a, int nthreads, long long (&red)[
     __syncthreads();
     long long total = 0;
     for (int w = 0; w < nw; ++w) total += red[w];
-    const long long parts = min((long long)gridDim.x, total);
+    long long step = 1;  // the line is cut at its tiles
+    if constexpr (!C::F32 && C::NT == 2) {  // (whole: prompts of bf16 rows, which have more than eight)
+        if (a.whole && total > 0) {
+            int rts, lo, tiles;
+            attn_seq_tiles<C>(a, attn_seq(a, 0, err), rts, lo, tiles);
+            step = tiles + kUnitCost;
+        }
+    }
+    const long long steps = total / step, parts = min((long long)gridDim.x, steps);
     if (blockIdx.x >= parts) return p;
-    p.begin = total * blockIdx.x / parts;
-    p.end = total * (blockIdx.x + 1) / parts;
+    p.begin = steps * blockIdx.x / parts * step;
+    p.end = steps * (blockIdx.x + 1) / parts * step;
     const long long at = p.begin;
     long long carry = 0;
     for (int b0 = 0; b0 < a.seqs.n_seqs; b0 += nthreads) {
@@ -902,10 +910,6 @@ __global__ void __launch_bounds__(128) __maxnreg__(C::NT == 1 ? 128 : 168) kv4_a
 template <class C, typename T>
 __global__ void __launch_bounds__(256) kv4_attn_join_kernel(AttnArgs a, int splits, int row_tiles, int by_border, int parts, unsigned int* err) {
     constexpr int D = C::D, ROWS = C::ROWS;
-    if (a.wide_too && a.hi_rows == 0 && a.seqs.n_seqs == 1 && a.wide[0] != a.call) {  // the prompt kernel took it
-        pdl_wait();
-        return;
-    }
     __shared__ long long red[8], found[4];
     __shared__ float4 acc_s[256];
     __shared__ float m_s[256], l_s[256];
@@ -1122,7 +1126,7 @@ static int run_attn(moe_engine* e, AttnArgs a, int variant, int64_t units, int64
         a.part = e->kv4.work;
         MOE_CUDA(launch_kernel(dependent, kernel, dim3((unsigned)grid), dim3(128), C::SMEM, e->stream, a, err));
         e->launches++;
-        if (grid == 1) return MOE_OK;  // nothing can be split
+        if (grid == 1 || a.whole) return MOE_OK;  // nothing can be split
         const int64_t all = (int64_t)a.seqs.n_seqs * a.cache.kv_heads * row_tiles;
         const bool by_border = all > grid - 1;
         const int64_t x = by_border ? grid - 1 : all;
@@ -1166,7 +1170,10 @@ static int launch_attn(moe_engine* e, const AttnArgs& a) {
             const int64_t all_rows = (int64_t)a.seqs.max_q_len * a.group;
             few.hi_rows = 0;
             few.wide_too = 1;
-            if (a.seqs.n_seqs == 1) return launch_rows<D, T>(e, few, all_rows, true);  // (the sequence is its, however many rows it has)
+            if (a.seqs.n_seqs == 1) {  // it is its, however many rows it has, or as a whole the other kernel's
+                few.whole = 1;
+                return launch_rows<D, T>(e, few, all_rows, true);
+            }
             few.wide_too = 0;
             // the sequences of fewer rows (the host knows bounds only): single tokens in as small a tile as they need, then the others
             const int one = (a.group + 7) / 8 * 8;

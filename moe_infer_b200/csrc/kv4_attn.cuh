@@ -34,6 +34,7 @@ struct AttnArgs {
     unsigned* wide;          // prompts: [sequence] == call where its values are too unequal for f16 tiles
     unsigned call;
     int wide_too;            // those sequences are this launch's too
+    int whole;               // one sequence: its units are dealt whole, nothing to join
     float* part;             // work area of the call
 };
 
