@@ -361,7 +361,8 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        keys rotated on the way when rope is given: by the position, or by rope_positions_dev[row].  A row
  *                        whose position the table does not hold is not stored, neither key nor value, and reported.  Each
  *                        position of the cache is written at most once per call (sequences share no pages being written).
- *                        Values are finite; a group of 64 that holds an infinity or NaN is stored as NaN.
+ *                        Values are finite; a group of 64 that holds an infinity or NaN, or spans more than bf16 can hold, is
+ *                        stored as NaN.
  * moe_kv4_gather_dev     the rows' stored keys and values as f32 or bf16 [n_tokens, num_kv_heads, head_dim], contiguous;
  *                        with q_start the running sum of seq_lens it reads whole sequences back.
  * moe_kv4_attention_dev  softmax attention of the rows' queries [n_tokens, num_heads, head_dim], already rotated, over the
@@ -369,7 +370,7 @@ int moe_rope_dev(moe_engine_t* e, const moe_rope_t* rope, const void* x_dev, int
  *                        h / (num_heads / num_kv_heads); scale multiplies the scores.  With gate the result is multiplied by
  *                        sigmoid(gate) (the output gate of the full-attention layers, src/engine/qwen35_moe/cpu.rs:218-347).
  *                        out is [n_tokens, num_heads, head_dim] of the queries' type, contiguous; it must not overlap them.
- *                        f32 rows: operands in two f16 terms, results to about 2^-21; bf16 rows: weights rounded to f16
+ *                        f32 rows: operands in two f16 terms, results to about 2^-20; bf16 rows: weights rounded to f16
  *                        (2^-12), and for sequences of at least 128 rows x query heads per KV head (prompts) keys and values
  *                        too; scores, sums and the softmax f32.  Sizes of keys and values may differ as they like: what is lost
  *                        is relative to the weighted |values| and ranges of the same group of 64 that the row sees.  (A prompt

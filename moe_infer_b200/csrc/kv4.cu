@@ -8,8 +8,8 @@
 // requested before the page is known.  A sub-warp of D / 8 lanes takes one quad (four positions that share words of V) of
 // the keys or values; a lane holds eight elements of the four positions, so a group's minimum and maximum are three
 // shuffles, the rotation partner is a second (cached) load or sits in the same lane, a lane's eight nibbles are one word of
-// K, and the four positions' bytes of V meet in the lane that stores them.  8,192 f32 rows of two heads of 256 (38 MB): 18 us
-// to store, 14 to read back; 14,000 bf16 rows of eight heads of 128 (73 MB): 24 and 16 us.
+// K, and the four positions' bytes of V meet in the lane that stores them.  8,192 f32 rows of two heads of 256 (38 MB): 16 us
+// to store, 13 to read back; 14,000 bf16 rows of eight heads of 128 (73 MB): 25 and 16 us.
 #include "kv4.cuh"
 
 namespace moe {
@@ -444,7 +444,7 @@ int moe_kv4_append_dev(moe_engine_t* e, const moe_kv4_cache_t* cache, const moe_
     const bool whole = a.vec_k && a.vec_v && (!rope || (a.vec_table && a.rotary % (a.interleaved ? 8 : 16) == 0));
     // up to four heads to a CTA where that still leaves every SM four CTAs (14,000 bf16 rows of eight heads: 46 us with one head
     // each, 24 us with four; with few CTAs the one-head kernel's smaller register count is worth more: 8,192 f32 rows of two
-    // heads, 18 us against 30)
+    // heads, 16 us against 30)
     int per = 1;
     while (whole && per < 4 && per * 2 <= cache->num_kv_heads && blocks_of(batch) * batch->n_seqs * cache->num_kv_heads / (per * 2) >= 4 * e->sm_count) per *= 2;
     if (per > 1) {

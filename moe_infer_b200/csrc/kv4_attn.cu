@@ -26,8 +26,9 @@
 // sequences of any lengths balance; units that cross CTAs leave partial sums that a second kernel joins.  Many rows
 // (f32 prompts; bf16 ones have kv4_prompt.cu): one CTA per unit over the positions its rows see, nothing to join.
 //
-// Bound by issue slots and dependent instructions: about 850 instructions per 16 positions and head of 256, 54 % of the slots
-// used at four CTAs per SM (barrier and MMA latency take the rest); 250,001 positions of two heads, f32, eight query heads each: 55.6 us, 2.6 TB/s.
+// Bound by issue slots and dependent instructions: about 860 instructions per 16 positions and head of 256, 54 % of the slots
+// used at four CTAs per SM (barrier and MMA latency take the rest); 250,001 positions of two heads, f32, eight query heads each:
+// 57.4 us, 2.5 TB/s (55.6 with one power of two per tile, for all groups and rows).
 #include <math.h>
 
 #include <type_traits>
@@ -59,7 +60,7 @@ struct AttnCfg {
     static constexpr int RED_BYTES = (TP - 1) * ROWS * D * 4;       // partial sums of the value pass meet in the same place
     static constexpr int P_TOTAL = 2 * P_BYTES > RED_BYTES ? 2 * P_BYTES : RED_BYTES;
     static constexpr int OFF_M = OFF_P + P_TOTAL;                   // [2][4][ROWS] references the warps used for a tile
-    static constexpr int OFF_FL = OFF_M + 8 * ROWS * 4;             // [2][4] what the warps have to say about a tile
+    static constexpr int OFF_FL = OFF_M + 8 * ROWS * 4;             // [2][4] whether a warp moved a row's reference
     static constexpr int OFF_QS = OFF_FL + 32;                      // [G][ROWS] sums of the queries' groups
     static constexpr int OFF_RF = OFF_QS + G * ROWS * 4;            // [ROWS] factor that makes a score of the MMA's sum
     static constexpr int OFF_L = OFF_RF + ROWS * 4;                 // [4][ROWS] sums of the warps' weights
@@ -179,9 +180,9 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint4& a, uint
 // The eight nibbles of a word as four pairs of f16 subnormals: the pattern n is n 2^-24, n << 4 is 16 n 2^-24, both exact.
 // bf16 rows: where the nibbles lie, a mask per pair (words 1 and 3 count 16 times: the other operand or the sum makes up for
 // it).  The tensor core aligns products by their exponents, and a subnormal's is that of 2^-14, so n << 4 keeps four more bits
-// of a sum: kWide (f32 rows) moves all of them there.  Measured (250,001 positions, f32): 54.3 us and 6.5e-6 off where they
-// lie, 57.3 us and 9.6e-7 wide, 57.5 us and 6.0e-7 with n - 8 made a normal number (two instructions more per pair); the ragged
-// bf16 batch 61.1 us with n - 8, 57.4 now.  kFlip: words 2 and 3 hold 15 - n.
+// of a sum: kWide (f32 rows) moves all of them there.  Measured when chosen (250,001 positions, f32): 54.3 us and 6.5e-6 off
+// where they lie, 57.3 us and 9.6e-7 wide, 57.5 us and 6.0e-7 with n - 8 made a normal number (two instructions more per pair);
+// the ragged bf16 batch 61.1 us with n - 8, 57.4 where they lie.  kFlip: words 2 and 3 hold 15 - n.
 constexpr float kSub = 16777216.0f;  // 2^24
 template <bool kWide, bool kFlip = false>
 __device__ __forceinline__ void nibbles_sub(uint32_t w, uint32_t (&o)[4]) {

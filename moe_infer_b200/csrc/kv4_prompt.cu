@@ -5,8 +5,8 @@
 // lie in memory exactly as the MMAs want them in shared memory (K-major, 128-byte swizzle): a tile then arrives by plain
 // bulk copies.  f16 keeps 11 bits down to 2^-14.  Keys of a tile are scaled by a power of two, values by one per tile or, where
 // positions differ by more than 2^5 or a group of 64 lies below 2^-12 of the tile's largest, by one per position, which the
-// weights carry: so only what a row sees decides how its weights are scaled (8,192 rows: 505 us, with every tile of the second kind
-// 837).  A sequence with a key group below 2^-12 of its tile's largest key or a value group below 2^-12 of its position's
+// weights carry: so only what a row sees decides how its weights are scaled (8,192 rows in a short run: 500 us, with every tile of
+// the second kind 840).  A sequence with a key group below 2^-12 of its tile's largest key or a value group below 2^-12 of its position's
 // largest (zeros aside) is left to the kernel of few rows, which has no such limits (6.2 ms).
 //
 // Attention kernel: a CTA owns 128 rows (of the query heads that share a KV head) and walks its positions.  One thread
@@ -15,8 +15,8 @@
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 (the weights of a row
 // share one reference, so the result does not depend on when).  QK of the next tile runs under the softmax of this one.
 //
-// A tile of heads of 256 takes 2,750 cycles; its MMAs need 2,370 (N = 128: 84 cycles for K = 16), its exponentials 1,030.
-// 8,192 rows of 16 heads over two KV heads: 549 us, 1.0 PFLOP/s; four warps with a row per thread: 752 us.
+// A tile of heads of 256 takes some 2,800 cycles; its MMAs need 2,370 (N = 128: 84 cycles for K = 16), its exponentials 1,030.
+// 8,192 rows of 16 heads over two KV heads: 560 us, 0.98 PFLOP/s; four warps with a row per thread: 752 us.
 #include <math.h>
 
 #include "kv4_attn.cuh"
